@@ -268,6 +268,94 @@ SS_API int ss_ragged_paged_attention_noalloc(
     int positions_is_int64, void* out, const int64_t out_strides[3], int64_t tokens, int heads,
     int kv_heads, int head_dim, int64_t num_pages, float sm_scale, void* stream);
 
+/* ---- 8-bit KV pool ---------------------------------------------------------------------
+ *
+ * The pool holds one byte per K / V value, codes [num_pages, 16, kv_heads, head_dim] for K and
+ * for V, and fp32 scales [num_pages, kv_heads, 2] (K, V): code c of a page and head stands for
+ * c * scale.  Scales must be finite and >= 0.  No counterpart in the reference, whose pool is
+ * bf16 (shardserve/cache.py:37-45); slots, block tables and positions mean what they mean there.
+ * head_dim is 64 or 128.  Strides are in elements; any non-negative stride works, and rows of
+ * codes that are 16-byte addressable (unit head_dim stride, other strides multiples of 16,
+ * 16-byte aligned base) are read by the fast kernels.
+ */
+#define SS_CODE_INT8 0 /* signed 8-bit integers in [-127, 127] */
+#define SS_CODE_E4M3 1 /* e4m3 numbers, largest 448            */
+
+/*
+ * Quantising slot-mapped append.  For every page the call writes to, and per head and tensor:
+ *     s = max |x| over the new rows / qmax  (qmax = 127 or 448; finite values only; 0 if < 2^-100)
+ *     new scale = max(old scale, s); the old scale counts as 0 if the call writes row 0 of the page
+ *     codes of the page's other rows <- round(c * (old / new));  new rows <- round(x * (1 / new))
+ * so a call that writes row 0 starts the page anew (its other rows become zeros).  Rounding is to
+ * nearest even, infinities saturate, NaN becomes 0 (int8) or stays NaN (e4m3).  The result does
+ * not depend on the order of the tokens; of two tokens with one slot the later one is kept.
+ * Slot -1 marks a padding token and is skipped; any other slot outside the pool is skipped and
+ * sets SS_DEVERR_SLOT.  k, v: bf16 [tokens, kv_heads, head_dim].
+ * workspace: optional error word, as ss_kv_append.
+ */
+SS_API int ss_kv_append_q8(const void* k, const int64_t k_strides[3], const void* v,
+                    const int64_t v_strides[3], void* k_pool, const int64_t k_pool_strides[4],
+                    void* v_pool, const int64_t v_pool_strides[4], int code_format, float* scales,
+                    const int64_t scale_strides[3], const void* slots, int slots_is_int64,
+                    int64_t tokens, int64_t num_pages, int kv_heads, int head_dim, void* workspace,
+                    void* stream);
+
+/*
+ * Reads rows back: k_out[i] = bf16(code * scale) of slot slots[i], and v_out likewise (bf16
+ * [tokens, kv_heads, head_dim]).  Slot -1 gives zeros; any other slot outside the pool gives
+ * zeros and sets SS_DEVERR_SLOT.  workspace: optional error word.
+ */
+SS_API int ss_kv_read_q8(const void* k_pool, const int64_t k_pool_strides[4], const void* v_pool,
+                  const int64_t v_pool_strides[4], int code_format, const float* scales,
+                  const int64_t scale_strides[3], const void* slots, int slots_is_int64,
+                  void* k_out, const int64_t k_out_strides[3], void* v_out,
+                  const int64_t v_out_strides[3], int64_t tokens, int64_t num_pages, int kv_heads,
+                  int head_dim, void* workspace, void* stream);
+
+/* Workspace size of ss_ragged_paged_attention_q8 on `device` for this geometry (any number of
+ * tokens).  A workspace must be zero when it is first used and is left ready for the next call;
+ * it is not shared with ss_ragged_paged_attention's, nor by calls that may overlap in time. */
+SS_API int ss_q8_workspace_bytes(int device, int heads, int kv_heads, int head_dim, size_t* bytes);
+
+/*
+ * Ragged paged attention over the 8-bit pool: ss_ragged_paged_attention with keys
+ * k_code * k_scale and values v_code * v_scale.  Sequence id -1 marks a padding token (a zero
+ * output row, no error bit).  A page id outside the pool reads as zeros (SS_DEVERR_PAGE).
+ */
+SS_API int ss_ragged_paged_attention_q8(
+    const void* q, const int64_t q_strides[3], const void* k_pool, const int64_t k_pool_strides[4],
+    const void* v_pool, const int64_t v_pool_strides[4], int code_format, const float* scales,
+    const int64_t scale_strides[3], const void* block_tables, const int64_t bt_strides[2],
+    int64_t bt_rows, int64_t bt_cols, int bt_is_int64, const void* query_seq_ids,
+    int seq_ids_is_int64, const void* positions, int positions_is_int64, void* out,
+    const int64_t out_strides[3], int64_t tokens, int heads, int kv_heads, int head_dim,
+    int64_t num_pages, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A step's block tables and flat token arrays from request lengths.  Row r holds cached_lens[r]
+ * tokens (its pages stand in block_tables) and gets new_lens[r] more: the pages it lacks are
+ * taken from free_pages, from entry *free_head on, in row order, and written into block_tables;
+ * its new tokens get consecutive places in the flat batch.
+ * cached_lens, new_lens: [rows] int32 / int64;  block_tables: [rows, cols] int32 / int64 (updated)
+ * free_pages: [num_free] int32 / int64;  free_head: one int32
+ * seqs int32, positions / slots int64 [tokens]: row, position and append slot of every new token;
+ *     places past the last new token hold -1 (padding that append and attention skip)
+ * last int64 [rows]: place of the row's last new token, -1 if it has none
+ * lens int32 [rows]: cached + new (may be cached_lens itself);  free_head_out: the head after the
+ *     call (may be free_head)
+ * Negative lengths count as 0, tokens past the table's columns get slot -1, tokens past the
+ * batch are left out (all SS_DEVERR_POS); where the free list runs out the entry and the slots
+ * are -1 (SS_DEVERR_PAGE).  rows <= 12288.
+ * workspace: required (256 zeroed bytes, kept between calls; any of this library's workspaces).
+ */
+SS_API int ss_build_block_tables(const void* cached_lens, int cached_is_int64, const void* new_lens,
+                          int new_is_int64, void* block_tables, const int64_t bt_strides[2],
+                          int64_t rows, int64_t cols, int bt_is_int64, const void* free_pages,
+                          int free_is_int64, int64_t num_free, const int32_t* free_head,
+                          int64_t tokens, int32_t* seqs, int64_t* positions, int64_t* slots,
+                          int64_t* last, int32_t* lens, int32_t* free_head_out, void* workspace,
+                          void* stream);
+
 /*
  * Reads (and, if clear != 0, zeroes) the device error word at the start of `workspace`.
  * Synchronises `stream`.  For tests and debugging, not for the hot path.
@@ -288,7 +376,8 @@ SS_API int ss_noalloc_fetch_device_errors(int device, int clear, uint32_t* flags
  * used: 1 = TMA/tensor-core split-K kernel, 2 = generic strided kernel (layouts the TMA
  * path cannot describe), 3 = split-K kernel for isolated tokens plus tcgen05 tiles for the
  * chunked-prefill runs, 4 = split-K kernel with the KV append folded in
- * (ss_append_ragged_paged_attention), 0 = none yet.  Lets tests assert the fast path really ran.
+ * (ss_append_ragged_paged_attention), 5 / 6 / 7 = ss_ragged_paged_attention_q8 on its split-K
+ * kernel / its generic strided kernel / its split-K kernel plus tcgen05 tiles, 0 = none yet.  Lets tests assert the fast path really ran.
  */
 SS_API int ss_last_attention_path(void);
 

@@ -18,10 +18,17 @@ from .kernel import (  # noqa: F401
     rope_kv_append,
 )
 from .cache import Cache  # noqa: F401
-from .metadata import DeviceMetadata  # noqa: F401
+from .metadata import DeviceMetadata, build_block_tables  # noqa: F401
+from .quantized import (  # noqa: F401
+    QuantizedCache,
+    kv_append_q8,
+    kv_read_q8,
+    ragged_attention_q8,
+)
 
 __all__ = [
     "KernelUnsupported", "SUPPORTED_BLOCK_SIZE", "SUPPORTED_RAGGED_HEAD_DIMS", "kv_append",
     "kv_append_attention",
     "ragged_attention_direct", "rope_kv_append", "Cache", "DeviceMetadata",
+    "QuantizedCache", "build_block_tables", "kv_append_q8", "kv_read_q8", "ragged_attention_q8",
 ]

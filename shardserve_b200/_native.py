@@ -33,6 +33,9 @@ SS_DEVERR_POS = 0x4
 SS_DEVERR_SLOT = 0x8
 SS_DEVERR_TIMEOUT = 0x10
 
+SS_CODE_INT8 = 0
+SS_CODE_E4M3 = 1
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "ss_version": (ctypes.c_int, []),
@@ -75,6 +78,24 @@ SIGNATURES = {
         _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int, _vp, _i64p, ctypes.c_int64,
         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_float, _vp]),
+    "ss_kv_append_q8": (ctypes.c_int, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, ctypes.c_int, _vp, _i64p, _vp,
+        ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, _vp]),
+    "ss_kv_read_q8": (ctypes.c_int, [
+        _vp, _i64p, _vp, _i64p, ctypes.c_int, _vp, _i64p, _vp, ctypes.c_int, _vp, _i64p, _vp,
+        _i64p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, _vp]),
+    "ss_q8_workspace_bytes": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+        ctypes.POINTER(ctypes.c_size_t)]),
+    "ss_ragged_paged_attention_q8": (ctypes.c_int, [
+        _vp, _i64p, _vp, _i64p, _vp, _i64p, ctypes.c_int, _vp, _i64p, _vp, _i64p, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int, _vp, _i64p,
+        ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
+        _vp, ctypes.c_size_t, _vp]),
+    "ss_build_block_tables": (ctypes.c_int, [
+        _vp, ctypes.c_int, _vp, ctypes.c_int, _vp, _i64p, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp,
+        _vp, _vp, _vp, _vp]),
     "ss_fetch_device_errors": (ctypes.c_int, [
         _vp, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32), _vp]),
     "ss_noalloc_fetch_device_errors": (ctypes.c_int, [
@@ -120,7 +141,9 @@ def strides(seq) -> ctypes.Array:
 
 
 _BOUND = ("ss_ragged_paged_attention", "ss_append_ragged_paged_attention", "ss_kv_append",
-          "ss_rope_kv_append", "ss_attention_workspace_bytes", "ss_last_error_message")
+          "ss_rope_kv_append", "ss_attention_workspace_bytes", "ss_last_error_message",
+          "ss_kv_append_q8", "ss_kv_read_q8", "ss_q8_workspace_bytes",
+          "ss_ragged_paged_attention_q8", "ss_build_block_tables")
 
 
 def ops():

@@ -125,6 +125,8 @@ void set_error_message(const char* fmt, ...) {
   va_end(ap);
   g_message = buf;
 }
+void count_launches(unsigned n) { count_launch(n); }
+void set_last_path(int path) { g_last_path = path; }
 }  // namespace ss
 
 extern "C" {

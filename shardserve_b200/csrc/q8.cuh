@@ -1,0 +1,121 @@
+// 8-bit paged KV pool: shared declarations of the quantising append, the read-back and the
+// attention kernels.
+//
+// A pool holds codes [pages, 16, kv_heads, head_dim], one byte each, for K and for V, and fp32
+// scales [pages, kv_heads, 2] (K, V): code c of a page and head stands for c * scale.  Codes are
+// signed 8-bit integers in [-127, 127] (SS_CODE_INT8) or e4m3 numbers (SS_CODE_E4M3, largest
+// 448).  Scales are finite and >= 0.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "attention.cuh"
+
+namespace ss {
+
+// A pool and the scales of its pages; strides in elements (bytes for the codes).
+struct Q8Pool {
+  uint8_t* k;
+  long long k_sn, k_ss, k_sh, k_sd;
+  uint8_t* v;
+  long long v_sn, v_ss, v_sh, v_sd;
+  float* scales;
+  long long s_sn, s_sh, s_sw;
+  long long N;  // pages
+  int KVH, D;
+  int fmt;  // SS_CODE_*
+};
+
+struct Q8AttnArgs {
+  AttnArgs a;  // queries, tables, output (its pool pointers are unused)
+  Q8Pool p;
+};
+
+struct Q8AppendArgs {
+  Q8Pool p;
+  const __nv_bfloat16* k;
+  long long k_st, k_sh, k_sd;
+  const __nv_bfloat16* v;
+  long long v_st, v_sh, v_sd;
+  const void* slots;
+  int slots64;
+  long long T;
+  unsigned* err;  // may be null
+};
+
+struct Q8ReadArgs {
+  Q8Pool p;
+  __nv_bfloat16* k;
+  long long k_st, k_sh, k_sd;
+  __nv_bfloat16* v;
+  long long v_st, v_sh, v_sd;
+  const void* slots;
+  int slots64;
+  long long T;
+  unsigned* err;  // may be null
+};
+
+struct BlockTablesArgs {
+  const void* cached;
+  int cached64;
+  const void* fresh;  // new tokens of each row
+  int fresh64;
+  long long B;  // rows
+  void* tables;
+  long long t_sb, t_sn, W;
+  int tables64;
+  const void* free_pages;
+  int free64;
+  long long F;  // entries of the free list
+  const int* head;
+  int* head_out;
+  long long T;
+  int* seqs;
+  long long* positions;
+  long long* slots;
+  long long* last;
+  int* lens;
+  unsigned* err;     // workspace word 0
+  unsigned* ticket;  // workspace word 20: zero between calls
+};
+
+// Largest magnitude a code stands for before its scale.
+__host__ __device__ constexpr float q8_max(int fmt) { return fmt == SS_CODE_INT8 ? 127.f : 448.f; }
+// Blocks whose scale would fall below this hold zeros: 1 / scale stays finite, and no bf16 value
+// of a model is that small.
+constexpr float kQ8Tiny = 0x1p-100f;
+
+__device__ __forceinline__ float q8_decode(int fmt, uint8_t c) {
+  if (fmt == SS_CODE_INT8) return static_cast<float>(static_cast<int8_t>(c));
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+// Nearest code, ties to even; values past the largest code (infinities among them) saturate.
+// NaN becomes 0 as an integer code and stays NaN as an e4m3 code.
+__device__ __forceinline__ uint8_t q8_encode(int fmt, float x) {
+  if (fmt == SS_CODE_INT8) {
+    const float r = rintf(x);
+    return static_cast<uint8_t>(static_cast<int8_t>(
+        static_cast<int>(r != r ? 0.f : fminf(fmaxf(r, -127.f), 127.f))));
+  }
+  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
+}
+
+// As token_info, but sequence id -1 marks a padding token: no keys, and no error bit.
+__device__ __forceinline__ TokInfo q8_token_info(const AttnArgs& a, long long t, bool report) {
+  const long long seq = ld_index(a.seq, a.seq64, t);
+  if (seq == -1) return TokInfo{-1, 0, 0};
+  return token_info_from(a, seq, ld_index(a.pos, a.pos64, t), report);
+}
+
+cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream);
+cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream);
+cudaError_t launch_q8_generic(const Q8AttnArgs& a, cudaStream_t stream);
+cudaError_t launch_block_tables(const BlockTablesArgs& a, cudaStream_t stream);
+int block_tables_max_rows();
+
+// Bookkeeping of the C-ABI layer (capi.cu).
+void count_launches(unsigned n);
+void set_last_path(int path);
+
+}  // namespace ss

@@ -1,0 +1,335 @@
+// Quantising slot-mapped append into the 8-bit paged pool, and the read-back.
+//
+// Append.  Token t's K / V row goes to row slot % 16 of page slot / 16.  Per page, KV head and
+// tensor the codes share one scale, so a call computes, over the rows R it writes to a page,
+//     s   = max |x| over R and head_dim / qmax     (finite values; 0 below 2^-100)
+//     new = max(old, s)     old = the page's scale, or 0 where the call writes row 0 of the page
+//     codes held by the page <- round(c * (old / new)),  new rows <- round(x * (1 / new))
+// A call that writes row 0 starts the page anew: what a former request left there becomes zeros.
+// The result does not depend on the order of the call's tokens (a maximum does not), except that
+// of two tokens with the same slot the later one is kept.
+//
+// Every page must be handled once, by one warp per (head, tensor), wherever its tokens stand in
+// the call.  CTA c owns the pages first met in its window of tokens: it puts the window's pages
+// into a hash table in shared memory, then reads all T slots (from L2) to find the pages' rows
+// and the pages that an earlier window owns.  T slots per CTA cost little while a window holds
+// 1/148 of the call: 8192 tokens are 64 KB per SM, ~1 us.
+//
+// Bound: HBM for prompts (3 bytes per value), latency for decode steps.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "ptx.cuh"
+#include "q8.cuh"
+
+namespace ss {
+
+namespace {
+
+constexpr int kMaxWindow = 512;          // tokens of one CTA
+constexpr int kHash = 2 * kMaxWindow;    // hash slots (at most half full)
+
+struct AppendSmem {
+  int key[kHash];              // page of a hash slot, -1: empty
+  int idx[kHash];              // its index in the lists below
+  int page[kMaxWindow];
+  int earlier[kMaxWindow];     // an earlier window owns the page
+  int row[kMaxWindow][kPage];  // last token that writes each row, -1: none
+  int n;
+};
+
+__device__ __forceinline__ unsigned hash_page(int page) {
+  return (static_cast<unsigned>(page) * 2654435769u) >> 22;  // 10 bits
+}
+static_assert(kHash == 1024, "hash_page gives 10 bits");
+
+// D / 32 consecutive bf16 values of a row, as packed pairs.
+template <int PER>
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, long long sd, int vec, int lane,
+                                         uint32_t (&w)[PER / 2]) {
+  if (vec) {
+    if constexpr (PER == 4) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p) + lane);
+      w[0] = u.x;
+      w[1] = u.y;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const unsigned*>(p) + lane);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) {
+      const __nv_bfloat16* e = p + (lane * PER + 2 * i) * sd;
+      w[i] = static_cast<uint32_t>(__bfloat16_as_ushort(e[0])) |
+             static_cast<uint32_t>(__bfloat16_as_ushort(e[sd])) << 16;
+    }
+  }
+}
+template <int PER>
+__device__ __forceinline__ float value_of(const uint32_t (&w)[PER / 2], int i) {
+  return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+}
+template <int PER>
+__device__ __forceinline__ void store_codes(uint8_t* p, long long sd, int vec, int lane,
+                                            const uint8_t (&c)[PER]) {
+  if (vec) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) w |= static_cast<uint32_t>(c[i]) << (8 * i);
+    if (PER == 4)
+      reinterpret_cast<uint32_t*>(p)[lane] = w;
+    else
+      reinterpret_cast<uint16_t*>(p)[lane] = static_cast<uint16_t>(w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) p[(lane * PER + i) * sd] = c[i];
+  }
+}
+template <int PER>
+__device__ __forceinline__ void load_codes(const uint8_t* p, long long sd, int vec, int lane,
+                                           uint8_t (&c)[PER]) {
+  if (vec) {
+    const uint32_t w = PER == 4 ? reinterpret_cast<const uint32_t*>(p)[lane]
+                                : reinterpret_cast<const uint16_t*>(p)[lane];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c[i] = static_cast<uint8_t>(w >> (8 * i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c[i] = p[(lane * PER + i) * sd];
+  }
+}
+
+// One page, head and tensor by one warp; `rows` = last token per row of the page.
+template <int D, int FMT>
+__device__ __forceinline__ void append_block(const int* rows, const __nv_bfloat16* x, long long x_st,
+                                             long long x_sd, int xvec, uint8_t* codes,
+                                             long long c_ss, long long c_sd, int cvec,
+                                             float* scale, int lane) {
+  constexpr int PER = D / 32;
+  int has = 0;
+  uint32_t xs[kPage][PER / 2];
+#pragma unroll
+  for (int r = 0; r < kPage; ++r) {
+    const int t = rows[r];
+    if (t < 0) continue;
+    has |= 1 << r;
+    load_row<PER>(x + t * x_st, x_sd, xvec, lane, xs[r]);
+  }
+  const bool fresh = has & 1;
+  const float old = fresh ? 0.f : *scale;
+  float amax = 0.f;
+#pragma unroll
+  for (int r = 0; r < kPage; ++r) {
+    if (!(has >> r & 1)) continue;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float v = fabsf(value_of<PER>(xs[r], i));
+      if (v < __int_as_float(0x7f800000)) amax = fmaxf(amax, v);  // false for inf and NaN
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float s = __fdiv_rn(amax, q8_max(FMT));
+  if (s < kQ8Tiny) s = 0.f;
+  const float now = fmaxf(old, s);
+  const float recip = now > 0.f ? __fdiv_rn(1.f, now) : 0.f;
+  if (fresh || now != old || now == 0.f) {  // the page's other rows follow the new scale
+    const float ratio = now > 0.f ? __fdiv_rn(old, now) : 0.f;
+#pragma unroll
+    for (int r = 0; r < kPage; ++r) {
+      if (has >> r & 1) continue;
+      uint8_t c[PER];
+      uint8_t* p = codes + r * c_ss;
+      if (fresh) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] = 0;
+      } else {
+        load_codes<PER>(p, c_sd, cvec, lane, c);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] = q8_encode(FMT, __fmul_rn(q8_decode(FMT, c[i]), ratio));
+      }
+      store_codes<PER>(p, c_sd, cvec, lane, c);
+    }
+    __syncwarp();  // every lane has read the old scale
+    if (lane == 0) *scale = now;
+  }
+#pragma unroll
+  for (int r = 0; r < kPage; ++r) {
+    if (!(has >> r & 1)) continue;
+    uint8_t c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c[i] = q8_encode(FMT, __fmul_rn(value_of<PER>(xs[r], i), recip));
+    store_codes<PER>(codes + r * c_ss, c_sd, cvec, lane, c);
+  }
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(1024) q8_append_kernel(const Q8AppendArgs a, int window,
+                                                         int kvec, int vvec, int kcvec, int vcvec) {
+  griddep_wait();  // k / v, the slots and the pool may come from the preceding kernel
+  extern __shared__ uint8_t smem_raw[];
+  AppendSmem& sm = *reinterpret_cast<AppendSmem*>(smem_raw);
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const long long w0 = static_cast<long long>(blockIdx.x) * window;
+  const long long w1 = min(w0 + window, a.T);
+  for (int i = tid; i < kHash; i += nt) sm.key[i] = -1;
+  for (int i = tid; i < window; i += nt) sm.earlier[i] = 0;
+  for (int i = tid; i < window * kPage; i += nt) (&sm.row[0][0])[i] = -1;
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+  const long long limit = a.p.N * kPage;
+  for (long long t = w0 + tid; t < w1; t += nt) {
+    const long long slot = ld_index(a.slots, a.slots64, t);
+    if (slot < 0 || slot >= limit) {
+      if (a.err && slot != -1) atomicOr(a.err, SS_DEVERR_SLOT);
+      continue;
+    }
+    const int page = static_cast<int>(slot / kPage);
+    for (unsigned h = hash_page(page);; h = (h + 1) & (kHash - 1)) {
+      const int was = atomicCAS(&sm.key[h], -1, page);
+      if (was == -1) {
+        const int i = atomicAdd(&sm.n, 1);
+        sm.idx[h] = i;
+        sm.page[i] = page;
+        break;
+      }
+      if (was == page) break;
+    }
+  }
+  __syncthreads();
+  const int n = sm.n;
+  if (n == 0) return;
+  for (long long t = tid; t < a.T; t += nt) {
+    const long long slot = ld_index(a.slots, a.slots64, t);
+    if (slot < 0 || slot >= limit) continue;
+    const int page = static_cast<int>(slot / kPage);
+    for (unsigned h = hash_page(page);; h = (h + 1) & (kHash - 1)) {
+      const int key = sm.key[h];
+      if (key == -1) break;
+      if (key == page) {
+        const int i = sm.idx[h];
+        if (t < w0)
+          sm.earlier[i] = 1;
+        else
+          atomicMax(&sm.row[i][slot % kPage], static_cast<int>(t));
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  const int warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
+  const int per_page = 2 * a.p.KVH;
+  for (int item = warp; item < n * per_page; item += warps) {
+    const int i = item / per_page, rest = item % per_page, h = rest >> 1;
+    if (sm.earlier[i]) continue;
+    const long long page = sm.page[i];
+    float* scale = a.p.scales + page * a.p.s_sn + h * a.p.s_sh + (rest & 1) * a.p.s_sw;
+    if ((rest & 1) == 0)
+      append_block<D, FMT>(sm.row[i], a.k + h * a.k_sh, a.k_st, a.k_sd, kvec,
+                           a.p.k + page * a.p.k_sn + h * a.p.k_sh, a.p.k_ss, a.p.k_sd, kcvec, scale,
+                           lane);
+    else
+      append_block<D, FMT>(sm.row[i], a.v + h * a.v_sh, a.v_st, a.v_sd, vvec,
+                           a.p.v + page * a.p.v_sn + h * a.p.v_sh, a.p.v_ss, a.p.v_sd, vcvec, scale,
+                           lane);
+  }
+}
+
+// One thread per 8 values of a row (or per value where a row is not 8-byte addressable).
+template <bool VEC>
+__global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadArgs a) {
+  griddep_wait();
+  constexpr int E = VEC ? 8 : 1;
+  const long long per_row = static_cast<long long>(a.p.KVH) * a.p.D / E;
+  const long long total = a.T * per_row, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < 2 * total;
+       i += step) {
+    const bool is_v = i >= total;
+    const long long j = is_v ? i - total : i;
+    const long long t = j / per_row;
+    const int e = static_cast<int>(j % per_row) * E, h = e / a.p.D, d = e % a.p.D;
+    const long long slot = ld_index(a.slots, a.slots64, t);
+    const bool ok = slot >= 0 && slot < a.p.N * kPage;
+    if (!ok && slot != -1 && a.err && e == 0 && !is_v) atomicOr(a.err, SS_DEVERR_SLOT);
+    const long long page = ok ? slot / kPage : 0, row = ok ? slot % kPage : 0;
+    const float s = ok ? a.p.scales[page * a.p.s_sn + h * a.p.s_sh + (is_v ? a.p.s_sw : 0)] : 0.f;
+    const uint8_t* src = is_v ? a.p.v + page * a.p.v_sn + row * a.p.v_ss + h * a.p.v_sh + d * a.p.v_sd
+                              : a.p.k + page * a.p.k_sn + row * a.p.k_ss + h * a.p.k_sh + d * a.p.k_sd;
+    __nv_bfloat16* dst = is_v ? a.v + t * a.v_st + h * a.v_sh + d * a.v_sd
+                              : a.k + t * a.k_st + h * a.k_sh + d * a.k_sd;
+    if (VEC) {
+      const uint2 c = ok ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
+      uint32_t o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t w = (k < 2 ? c.x : c.y) >> (16 * (k & 1));
+        o[k] = pack_bf16(q8_decode(a.p.fmt, static_cast<uint8_t>(w)) * s,
+                         q8_decode(a.p.fmt, static_cast<uint8_t>(w >> 8)) * s);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      *dst = __float2bfloat16(ok ? q8_decode(a.p.fmt, *src) * s : 0.f);
+    }
+  }
+}
+
+// Rows of `align` bytes: unit head_dim stride, base and the other strides multiples of it.
+bool rows_ok(const void* p, long long esize, long long align, long long s0, long long s1,
+             long long s2, long long sd) {
+  return sd == 1 && reinterpret_cast<uintptr_t>(p) % align == 0 && s0 * esize % align == 0 &&
+         s1 * esize % align == 0 && s2 * esize % align == 0;
+}
+
+void one_after_another(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+}
+
+}  // namespace
+
+cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream) {
+  // One window per SM, so that T slots are read once per SM; small calls get one page each.
+  const long long window = std::min<long long>(std::max<long long>((a.T + 147) / 148, 1), kMaxWindow);
+  long long warps = 4;
+  while (warps < 32 && warps < window * 2 * a.p.KVH) warps *= 2;
+  const int D = a.p.D;
+  const int kvec = rows_ok(a.k, 2, D / 16, a.k_st, a.k_sh, 0, a.k_sd);
+  const int vvec = rows_ok(a.v, 2, D / 16, a.v_st, a.v_sh, 0, a.v_sd);
+  const int kcvec = rows_ok(a.p.k, 1, D / 32, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd);
+  const int vcvec = rows_ok(a.p.v, 1, D / 32, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((a.T + window - 1) / window));
+  cfg.blockDim = dim3(static_cast<unsigned>(32 * warps));
+  cfg.dynamicSmemBytes = sizeof(AppendSmem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  one_after_another(cfg, attr);
+  const int w = static_cast<int>(window);
+  if (D == 128)
+    return a.p.fmt == SS_CODE_INT8
+               ? cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_INT8>, a, w, kvec, vvec, kcvec, vcvec)
+               : cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_E4M3>, a, w, kvec, vvec, kcvec, vcvec);
+  return a.p.fmt == SS_CODE_INT8
+             ? cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_INT8>, a, w, kvec, vvec, kcvec, vcvec)
+             : cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_E4M3>, a, w, kvec, vvec, kcvec, vcvec);
+}
+
+cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream) {
+  const bool vec = rows_ok(a.k, 2, 16, a.k_st, a.k_sh, 0, a.k_sd) &&
+                   rows_ok(a.v, 2, 16, a.v_st, a.v_sh, 0, a.v_sd) &&
+                   rows_ok(a.p.k, 1, 8, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd) &&
+                   rows_ok(a.p.v, 1, 8, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
+  const long long work = 2 * a.T * a.p.KVH * a.p.D / (vec ? 8 : 1);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(std::max<long long>((work + 255) / 256, 1), 148 * 32)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  one_after_another(cfg, attr);
+  return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<true>, a)
+             : cudaLaunchKernelEx(&cfg, q8_read_kernel<false>, a);
+}
+
+}  // namespace ss

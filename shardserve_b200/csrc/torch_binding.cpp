@@ -40,6 +40,11 @@ decltype(&ss_append_ragged_paged_attention) p_append_attention = nullptr;
 decltype(&ss_kv_append) p_append = nullptr;
 decltype(&ss_rope_kv_append) p_rope = nullptr;
 decltype(&ss_attention_workspace_bytes) p_ws_bytes = nullptr;
+decltype(&ss_kv_append_q8) p_append_q8 = nullptr;
+decltype(&ss_kv_read_q8) p_read_q8 = nullptr;
+decltype(&ss_q8_workspace_bytes) p_ws_bytes_q8 = nullptr;
+decltype(&ss_ragged_paged_attention_q8) p_attention_q8 = nullptr;
+decltype(&ss_build_block_tables) p_block_tables = nullptr;
 decltype(&ss_last_error_message) p_last_error = nullptr;
 PyObject* g_unsupported = nullptr;  // shardserve_b200.kernel.KernelUnsupported (a ValueError)
 
@@ -372,6 +377,256 @@ at::Tensor rope_kv_append(const at::Tensor& q, const at::Tensor& k, const at::Te
   return out;
 }
 
+// ---- 8-bit pool -----------------------------------------------------------------------------
+// Its workspace (error word, row counters, split-K partial states) is a second per-device
+// buffer: the counters must stay zero between calls, and the bf16 path's scratch moves with the
+// call's shape.
+auto* g_ws_q8 = new std::map<int, at::Tensor>();
+auto* g_ws_q8_need = new std::map<std::tuple<int, int, int, int>, size_t>();
+
+at::Tensor ensure_workspace_q8(const at::Device& dev, int heads, int kv_heads, int head_dim,
+                               const char* what) {
+  const int idx = dev.index();
+  std::lock_guard<std::mutex> lock(g_ws_mu);
+  size_t need = 0;
+  if (heads > 0) {
+    const auto key = std::make_tuple(idx, heads, kv_heads, head_dim);
+    auto nit = g_ws_q8_need->find(key);
+    if (nit != g_ws_q8_need->end()) {
+      need = nit->second;
+    } else {
+      check_rc(p_ws_bytes_q8(idx, heads, kv_heads, head_dim, &need), "ss_q8_workspace_bytes");
+      (*g_ws_q8_need)[key] = need;
+    }
+  }
+  auto it = g_ws_q8->find(idx);
+  if (it != g_ws_q8->end() && static_cast<size_t>(it->second.numel()) >= need) return it->second;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(idx).stream(), &status) ==
+          cudaSuccess &&
+      status != cudaStreamCaptureStatusNone)
+    throw std::runtime_error(std::string(what) +
+                             ": workspace must grow during CUDA graph capture; run the same "
+                             "shapes once before capturing");
+  // Room for any geometry on the device, so that the buffer is not replaced later.
+  const int64_t size = std::max<int64_t>(static_cast<int64_t>(need), int64_t{8} << 20);
+  at::Tensor ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(dev));
+  if (it != g_ws_q8->end()) g_ws_retired->push_back(it->second);
+  (*g_ws_q8)[idx] = ws;
+  return ws;
+}
+
+py::object workspace_for_q8(int device_index) {
+  std::lock_guard<std::mutex> lock(g_ws_mu);
+  auto it = g_ws_q8->find(device_index);
+  if (it == g_ws_q8->end()) return py::none();
+  return py::cast(it->second);
+}
+
+// The error word (null only before the first call on the device, if that is being captured).
+void* err_word_q8(const at::Device& dev) {
+  {
+    std::lock_guard<std::mutex> lock(g_ws_mu);
+    auto it = g_ws_q8->find(dev.index());
+    if (it != g_ws_q8->end()) return it->second.data_ptr();
+  }
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(dev.index()).stream(), &status) !=
+          cudaSuccess ||
+      status != cudaStreamCaptureStatusNone)
+    return nullptr;
+  return ensure_workspace_q8(dev, 0, 0, 0, "kv_append_q8").data_ptr();
+}
+
+// Checks the pools and their scales; returns SS_CODE_*.
+int check_pools_q8(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& scales) {
+  if (!k_pool.is_cuda()) unsupported("the 8-bit KV pool must be CUDA tensors");
+  const auto type = k_pool.scalar_type();
+  if ((type != at::kChar && type != at::kFloat8_e4m3fn) || v_pool.scalar_type() != type)
+    unsupported("8-bit KV pools must both be int8 or both float8_e4m3fn");
+  if (k_pool.sizes() != v_pool.sizes() || k_pool.dim() != 4 || k_pool.size(1) != kBlockSize)
+    unsupported("8-bit K/V pools must have identical shapes [pages, 16, kv_heads, head_dim]");
+  if (k_pool.size(3) != 64 && k_pool.size(3) != 128)
+    unsupported("8-bit pools hold head_dim 64 or 128, got " + shape_str(k_pool));
+  if (k_pool.size(0) < 1 || k_pool.size(2) < 1) unsupported("8-bit KV pools cannot be empty");
+  if (scales.scalar_type() != at::kFloat || scales.dim() != 3 ||
+      scales.size(0) != k_pool.size(0) || scales.size(1) != k_pool.size(2) || scales.size(2) != 2)
+    unsupported("scales must be float32 [pages, kv_heads, 2], got " + shape_str(scales));
+  const std::pair<const char*, const at::Tensor*> same_device[] = {{"v_pool_layer", &v_pool},
+                                                                   {"scales", &scales}};
+  for (const auto& nt : same_device)
+    if (nt.second->device() != k_pool.device())
+      unsupported(std::string(nt.first) + " must be on " + k_pool.device().str());
+  return type == at::kChar ? SS_CODE_INT8 : SS_CODE_E4M3;
+}
+
+at::Tensor ragged_attention_q8(const at::Tensor& q, const at::Tensor& k_pool,
+                               const at::Tensor& v_pool, const at::Tensor& scales,
+                               const at::Tensor& block_tables, const at::Tensor& query_seq_ids,
+                               const at::Tensor& positions, double sm_scale) {
+  require_bound();
+  if (!q.is_cuda() || q.scalar_type() != at::kBFloat16)
+    unsupported("ragged kernel requires BF16 CUDA queries");
+  if (q.dim() != 3 || (q.size(-1) != 64 && q.size(-1) != 128))
+    unsupported("ragged q must be [tokens, heads, 64|128], got " + shape_str(q));
+  const int fmt = check_pools_q8(k_pool, v_pool, scales);
+  if (k_pool.size(-1) != q.size(-1)) unsupported("query and KV head dimensions differ");
+  if (block_tables.device() != q.device() || block_tables.dim() != 2)
+    unsupported("block_tables must be a device-resident rank-2 tensor");
+  if (query_seq_ids.numel() != q.size(0) || positions.numel() != q.size(0))
+    unsupported("one sequence id and absolute position are required per query");
+  if (q.size(0) < 1) unsupported("ragged batch cannot be empty");
+  const int heads = static_cast<int>(q.size(1)), head_dim = static_cast<int>(q.size(2));
+  const int kv_heads = static_cast<int>(k_pool.size(2));
+  if (heads < 1 || heads % kv_heads) unsupported("query heads must be divisible by KV heads");
+  const std::pair<const char*, const at::Tensor*> same_device[] = {
+      {"k_pool_layer", &k_pool}, {"query_seq_ids", &query_seq_ids}, {"positions", &positions}};
+  for (const auto& nt : same_device)
+    if (nt.second->device() != q.device())
+      unsupported(std::string(nt.first) + " must be on " + q.device().str());
+  const int bt64 = index_flag(block_tables, "block_tables");
+  const int seq64 = index_flag(query_seq_ids, "query_seq_ids");
+  const int pos64 = index_flag(positions, "positions");
+  const at::Tensor seqs = flat_index(query_seq_ids);
+  const at::Tensor pos = flat_index(positions);
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  at::Tensor out = at::empty_like(q);
+  const at::Tensor ws =
+      ensure_workspace_q8(q.device(), heads, kv_heads, head_dim, "ragged_attention_q8");
+  const Strides<3> qs(q), os(out), ss(scales);
+  const Strides<4> ks(k_pool), vs(v_pool);
+  const Strides<2> bs(block_tables);
+  check_rc(p_attention_q8(q.data_ptr(), qs.v, k_pool.data_ptr(), ks.v, v_pool.data_ptr(), vs.v,
+                          fmt, static_cast<const float*>(scales.data_ptr()), ss.v,
+                          block_tables.data_ptr(), bs.v, block_tables.size(0),
+                          block_tables.size(1), bt64, seqs.data_ptr(), seq64, pos.data_ptr(),
+                          pos64, out.data_ptr(), os.v, q.size(0), heads, kv_heads, head_dim,
+                          k_pool.size(0), static_cast<float>(sm_scale), ws.data_ptr(),
+                          static_cast<size_t>(ws.numel()), stream_of(q.device())),
+           "ss_ragged_paged_attention_q8");
+  return out;
+}
+
+void kv_append_q8(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& scales,
+                  const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots) {
+  require_bound();
+  const int fmt = check_pools_q8(k_pool, v_pool, scales);
+  const int64_t kv_heads = k_pool.size(2), head_dim = k_pool.size(3);
+  check_kv(k, v, kv_heads, head_dim);
+  const std::pair<const char*, const at::Tensor*> same_device[] = {
+      {"k", &k}, {"v", &v}, {"slots", &slots}};
+  for (const auto& nt : same_device)
+    if (nt.second->device() != k_pool.device())
+      unsupported(std::string(nt.first) + " must be on " + k_pool.device().str());
+  if (slots.numel() != k.size(0)) unsupported("one slot is required per appended token");
+  const int s64 = index_flag(slots, "slots");
+  const at::Tensor sl = flat_index(slots);
+  const c10::cuda::OptionalCUDAGuard guard(k_pool.device());
+  const Strides<3> kst(k), vst(v), sst(scales);
+  const Strides<4> kps(k_pool), vps(v_pool);
+  check_rc(p_append_q8(k.data_ptr(), kst.v, v.data_ptr(), vst.v, k_pool.data_ptr(), kps.v,
+                       v_pool.data_ptr(), vps.v, fmt, static_cast<float*>(scales.data_ptr()),
+                       sst.v, sl.data_ptr(), s64, k.size(0), k_pool.size(0),
+                       static_cast<int>(kv_heads), static_cast<int>(head_dim),
+                       err_word_q8(k_pool.device()), stream_of(k_pool.device())),
+           "ss_kv_append_q8");
+}
+
+py::tuple kv_read_q8(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& scales,
+                     const at::Tensor& slots) {
+  require_bound();
+  const int fmt = check_pools_q8(k_pool, v_pool, scales);
+  const int64_t kv_heads = k_pool.size(2), head_dim = k_pool.size(3);
+  if (slots.device() != k_pool.device())
+    unsupported("slots must be on " + k_pool.device().str());
+  const int s64 = index_flag(slots, "slots");
+  const at::Tensor sl = flat_index(slots);
+  const c10::cuda::OptionalCUDAGuard guard(k_pool.device());
+  const auto opts = at::TensorOptions().dtype(at::kBFloat16).device(k_pool.device());
+  at::Tensor k = at::empty({sl.numel(), kv_heads, head_dim}, opts);
+  at::Tensor v = at::empty({sl.numel(), kv_heads, head_dim}, opts);
+  const Strides<3> kst(k), vst(v), sst(scales);
+  const Strides<4> kps(k_pool), vps(v_pool);
+  check_rc(p_read_q8(k_pool.data_ptr(), kps.v, v_pool.data_ptr(), vps.v, fmt,
+                     static_cast<const float*>(scales.data_ptr()), sst.v, sl.data_ptr(), s64,
+                     k.data_ptr(), kst.v, v.data_ptr(), vst.v, sl.numel(), k_pool.size(0),
+                     static_cast<int>(kv_heads), static_cast<int>(head_dim),
+                     err_word_q8(k_pool.device()), stream_of(k_pool.device())),
+           "ss_kv_read_q8");
+  return py::make_tuple(k, v);
+}
+
+// ---- block tables and slot maps from request lengths ------------------------------------------
+py::dict build_block_tables(const at::Tensor& cached_lens, const at::Tensor& new_lens,
+                            const at::Tensor& block_tables, const at::Tensor& free_pages,
+                            const at::Tensor& free_head, int64_t tokens, const py::object& out) {
+  require_bound();
+  if (!block_tables.is_cuda() || block_tables.dim() != 2)
+    unsupported("block_tables must be a device-resident rank-2 tensor");
+  const at::Device dev = block_tables.device();
+  const std::pair<const char*, const at::Tensor*> same_device[] = {
+      {"cached_lens", &cached_lens}, {"new_lens", &new_lens},
+      {"free_pages", &free_pages}, {"free_head", &free_head}};
+  for (const auto& nt : same_device)
+    if (nt.second->device() != dev)
+      unsupported(std::string(nt.first) + " must be on " + dev.str());
+  const int64_t rows = block_tables.size(0);
+  if (cached_lens.numel() != rows || new_lens.numel() != rows)
+    unsupported("one cached and one new length are required per block-table row");
+  if (rows > 0 && block_tables.size(1) < 1) unsupported("block_tables must be non-empty");
+  if (tokens < 0) unsupported("tokens must be >= 0");
+  if (free_head.numel() != 1 || free_head.scalar_type() != at::kInt)
+    unsupported("free_head must be one int32");
+  const int c64 = index_flag(cached_lens, "cached_lens"), n64 = index_flag(new_lens, "new_lens");
+  const int b64 = index_flag(block_tables, "block_tables");
+  const int f64 = index_flag(free_pages, "free_pages");
+  const at::Tensor cl = flat_index(cached_lens), nl = flat_index(new_lens);
+  const at::Tensor fp = flat_index(free_pages);
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  auto take_out = [&](const char* name, at::ScalarType type, int64_t n) -> at::Tensor {
+    if (!out.is_none()) {
+      const py::dict d = out;
+      if (d.contains(name)) {
+        at::Tensor t = d[name].cast<at::Tensor>();
+        if (t.dim() != 1 || t.size(0) != n || t.scalar_type() != type || t.device() != dev ||
+            !t.is_contiguous())
+          unsupported(std::string("out['") + name + "'] must be a contiguous " +
+                      (type == at::kInt ? "int32" : "int64") + " [" + std::to_string(n) +
+                      "] tensor on " + dev.str());
+        return t;
+      }
+    }
+    return at::empty({n}, at::TensorOptions().dtype(type).device(dev));
+  };
+  const at::Tensor seqs = take_out("seqs", at::kInt, tokens);
+  const at::Tensor pos = take_out("positions", at::kLong, tokens);
+  const at::Tensor slots = take_out("slots", at::kLong, tokens);
+  const at::Tensor last = take_out("last", at::kLong, rows);
+  const at::Tensor lens = take_out("lens", at::kInt, rows);
+  const at::Tensor head = take_out("free_head", at::kInt, 1);
+  const at::Tensor ws = ensure_workspace_q8(dev, 0, 0, 0, "build_block_tables");
+  const Strides<2> bs(block_tables);
+  check_rc(p_block_tables(cl.data_ptr(), c64, nl.data_ptr(), n64, block_tables.data_ptr(), bs.v,
+                          rows, block_tables.size(1), b64, fp.data_ptr(), f64, fp.numel(),
+                          static_cast<const int32_t*>(free_head.data_ptr()), tokens,
+                          static_cast<int32_t*>(seqs.data_ptr()),
+                          static_cast<int64_t*>(pos.data_ptr()),
+                          static_cast<int64_t*>(slots.data_ptr()),
+                          static_cast<int64_t*>(last.data_ptr()),
+                          static_cast<int32_t*>(lens.data_ptr()),
+                          static_cast<int32_t*>(head.data_ptr()), ws.data_ptr(), stream_of(dev)),
+           "ss_build_block_tables");
+  py::dict d;
+  d["tables"] = block_tables;
+  d["seqs"] = seqs;
+  d["positions"] = pos;
+  d["slots"] = slots;
+  d["last"] = last;
+  d["lens"] = lens;
+  d["free_head"] = head;
+  return d;
+}
+
 template <typename F>
 void take(const py::dict& addrs, const char* name, F*& slot) {
   slot = reinterpret_cast<F*>(static_cast<uintptr_t>(addrs[name].cast<uint64_t>()));
@@ -385,6 +640,11 @@ void bind(const py::dict& addrs, const py::object& unsupported_cls) {
   take(addrs, "ss_rope_kv_append", p_rope);
   take(addrs, "ss_attention_workspace_bytes", p_ws_bytes);
   take(addrs, "ss_last_error_message", p_last_error);
+  take(addrs, "ss_kv_append_q8", p_append_q8);
+  take(addrs, "ss_kv_read_q8", p_read_q8);
+  take(addrs, "ss_q8_workspace_bytes", p_ws_bytes_q8);
+  take(addrs, "ss_ragged_paged_attention_q8", p_attention_q8);
+  take(addrs, "ss_build_block_tables", p_block_tables);
   PyObject* cls = unsupported_cls.ptr();
   Py_INCREF(cls);
   Py_XDECREF(g_unsupported);
@@ -415,4 +675,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                   tokens, heads, kv_heads, head_dim);
         });
   m.def("workspace_for", &workspace_for);
+  m.def("ragged_attention_q8", &ragged_attention_q8, py::arg("q"), py::arg("k_pool_layer"),
+        py::arg("v_pool_layer"), py::arg("scales"), py::arg("block_tables"),
+        py::arg("query_seq_ids"), py::arg("positions"), py::arg("sm_scale"));
+  m.def("kv_append_q8", &kv_append_q8, py::arg("k_pool_layer"), py::arg("v_pool_layer"),
+        py::arg("scales"), py::arg("k"), py::arg("v"), py::arg("slots"));
+  m.def("kv_read_q8", &kv_read_q8, py::arg("k_pool_layer"), py::arg("v_pool_layer"),
+        py::arg("scales"), py::arg("slots"));
+  m.def("build_block_tables", &build_block_tables, py::arg("cached_lens"), py::arg("new_lens"),
+        py::arg("block_tables"), py::arg("free_pages"), py::arg("free_head"), py::arg("tokens"),
+        py::arg("out") = py::none());
+  m.def("workspace_for_q8", &workspace_for_q8);
 }

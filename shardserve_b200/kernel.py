@@ -47,25 +47,29 @@ def workspace_for(device):
 
 
 def device_errors(device, clear: bool = True) -> int:
-    """Reads the SS_DEVERR_* bits accumulated on `device` (synchronises; debug only)."""
+    """Reads the SS_DEVERR_* bits accumulated on `device`, by the bf16 and the 8-bit calls
+    (synchronises; debug only)."""
     import torch
 
-    ws = workspace_for(device)
-    if ws is None:
-        return 0
-    flags = ctypes.c_uint32(0)
+    bits = 0
     stream = torch.cuda.current_stream(device).cuda_stream
-    rc = _native.lib().ss_fetch_device_errors(ctypes.c_void_p(ws.data_ptr()), int(clear),
-                                              ctypes.byref(flags), ctypes.c_void_p(stream))
-    if rc != _native.SS_OK:
-        raise RuntimeError(_native.last_error())
-    return flags.value
+    for ws in (workspace_for(device), _native.ops().workspace_for_q8(device.index)):
+        if ws is None:
+            continue
+        flags = ctypes.c_uint32(0)
+        rc = _native.lib().ss_fetch_device_errors(ctypes.c_void_p(ws.data_ptr()), int(clear),
+                                                  ctypes.byref(flags), ctypes.c_void_p(stream))
+        if rc != _native.SS_OK:
+            raise RuntimeError(_native.last_error())
+        bits |= flags.value
+    return bits
 
 
 def last_attention_path() -> int:
     """1 = TMA tensor-core split-K kernel, 2 = generic strided kernel, 3 = split-K kernel
     plus tcgen05 chunked-prefill tiles, 4 = split-K kernel with the KV append folded in
-    (kv_append_attention), 0 = none yet."""
+    (kv_append_attention), 5 / 6 / 7 = ragged_attention_q8 on its split-K kernel / its generic
+    kernel / its split-K kernel plus tcgen05 tiles, 0 = none yet."""
     return _native.lib().ss_last_attention_path()
 
 

@@ -160,6 +160,29 @@ class DeviceMetadata:
                 raise KernelUnsupported(f"out[{key!r}] must be {dtype} {shape} on {self.device}")
 
 
+def build_block_tables(cached_lens: Any, new_lens: Any, block_tables: Any, free_pages: Any,
+                       free_head: Any, tokens: int, out: dict | None = None) -> dict:
+    """A step's block tables, slot map and flat token arrays from request lengths alone, in one
+    launch and with nothing made on the host.
+
+    Row r holds cached_lens[r] tokens, whose pages stand in block_tables [rows, cols], and gets
+    new_lens[r] more.  The pages it lacks come from free_pages, from entry free_head (one int32)
+    on, in row order, and are written into block_tables.  `tokens` is the flat batch's size: the
+    sum of new_lens, or more (a captured graph's bucket), the rest being padding.
+
+    Returns a dict: tables (block_tables itself), seqs int32 / positions int64 / slots int64
+    [tokens] for `kv_append*` and `ragged_attention*` (-1 in padding), last int64 [rows] (place of
+    the row's last new token, -1: none), lens int32 [rows] (cached + new), free_head int32 [1].
+    `out` gives tensors to write into; out["lens"] may be cached_lens and out["free_head"] may be
+    free_head, so a captured step advances itself.
+
+    Lengths below 0 count as 0 and tokens past the table's columns get slot -1 (SS_DEVERR_POS);
+    an empty free list leaves -1 in the table and the slots (SS_DEVERR_PAGE): see
+    `shardserve_b200.kernel.device_errors`."""
+    return _native.ops().build_block_tables(cached_lens, new_lens, block_tables, free_pages,
+                                            free_head, int(tokens), out)
+
+
 _builders: dict = {}
 
 

@@ -1,0 +1,619 @@
+"""8-bit KV pool on the GPU against its plain 64-bit forms (oracle/quantized.py).
+
+Tolerances, from the number formats:
+* a code is the nearest one to x / scale; the kernel's x * (1 / scale) in fp32 is off by at most
+  3 roundings of 2^-24, so an int8 code lies within 0.5 + 127 * 3 * 2^-24 < 0.5001 of x / scale,
+  and an e4m3 code within half a step of its binade (2^-4 of it) plus the same share;
+* scales: one fp32 division, 2^-23 relative;
+* attention: the output is rounded to bf16 (2^-9 of it); a probability carries the rounding of
+  P to fp16 (2^-11) and, through the fp32 score, about 2^-13 for scores up to 2^7: 2^-10 of
+  sum p|v| covers both.  Twice both bounds is asserted.
+"""
+import numpy as np
+import pytest
+import torch
+
+import shardserve_b200 as sb
+from oracle import quantized as oq
+from shardserve_b200 import _native
+from shardserve_b200 import kernel as K
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+QMAX = {"int8": 127.0, "e4m3": 448.0}
+
+
+def pool_like(codes, order):
+    """Codes [N, 16, KVH, D] laid out with each head's page (head) or each row's heads (token) in
+    one run, in rows that are not 16-byte addressable (odd), or with strided values (every)."""
+    if order == "head":
+        return codes.transpose(1, 2).contiguous().transpose(1, 2)
+    if order == "odd":
+        N, P, H, D = codes.shape
+        base = torch.zeros((N, P, H, D + 4), dtype=torch.int8, device=codes.device)
+        out = base.view(codes.dtype)[..., :D]
+        out.view(torch.int8).copy_(codes.view(torch.int8))
+        return out
+    if order == "every":
+        base = torch.zeros(codes.shape + (2,), dtype=torch.int8, device=codes.device)
+        out = base.view(codes.dtype)[..., 1]
+        out.view(torch.int8).copy_(codes.view(torch.int8))
+        return out
+    return codes.contiguous()
+
+
+def make_pool(pages, kvh, d, codes, order="head", seed=0, spread=0.4):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    pools, scales = [], torch.empty(pages, kvh, 2, device=DEV)
+    for which in (0, 1):
+        x = torch.randn(pages, 16, kvh, d, device=DEV, generator=g)
+        x *= torch.exp(spread * torch.randn(pages, 1, kvh, 1, device=DEV, generator=g))
+        s = x.abs().amax(dim=(1, 3)) / QMAX[codes]
+        scales[:, :, which] = s
+        x = x / s[:, None, :, None]
+        c = torch.round(x).to(torch.int8) if codes == "int8" else x.to(TYPES[codes])
+        pools.append(pool_like(c, order))
+    return pools[0], pools[1], scales
+
+
+def numbers(pool):
+    return pool.contiguous().float().cpu().double().numpy()
+
+
+def batch(spans, pages, seed=0, width=None, dtype=torch.int32):
+    """Block tables over scattered pages and the flat arrays of rows (cached, new)."""
+    rng = np.random.RandomState(seed)
+    need = [(c + n + 15) // 16 for c, n in spans]
+    perm = rng.permutation(pages)
+    tables = np.zeros((len(spans), width or max(need)), np.int64)
+    at = 0
+    for i, n in enumerate(need):
+        tables[i, :n] = perm[at:at + n]
+        at += n
+    seqs = np.repeat(np.arange(len(spans)), [n for _, n in spans])
+    pos = np.concatenate([np.arange(c, c + n) for c, n in spans])
+    slots = tables[seqs, pos // 16] * 16 + pos % 16
+    return tables, seqs, pos, slots
+
+
+def dev(x, dtype):
+    return torch.as_tensor(np.asarray(x)).to(DEV, dtype)
+
+
+def check_attention(out, q, k, v, scales, tables, seqs, pos, sm_scale):
+    want, weight = oq.attention(q.float().cpu().double().numpy(), numbers(k), numbers(v),
+                                scales.cpu().double().numpy(), np.asarray(tables), np.asarray(seqs),
+                                np.asarray(pos), sm_scale)
+    got = out.float().cpu().double().numpy()
+    assert np.isfinite(got).all()
+    bound = 2 * (2.0 ** -9 * np.abs(want) + 2.0 ** -10 * weight) + 1e-30
+    worst = np.max(np.abs(got - want) / bound)
+    assert worst <= 1.0, worst
+    return want
+
+
+# ---- attention -----------------------------------------------------------------------------
+DECODE = [1, 2, 15, 16, 17, 31, 33, 100, 257, 600]
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kvh", [(1, 1), (4, 4), (8, 2), (14, 2), (16, 2), (16, 1), (24, 1), (64, 1)])
+def test_decode_rows(codes, d, heads, kvh):
+    spans = [(n - 1, 1) for n in DECODE]
+    k, v, s = make_pool(100, kvh, d, codes, seed=heads + d)
+    tables, seqs, pos, _ = batch(spans, 100)
+    q = torch.randn(len(spans), heads, d, device=DEV).bfloat16()
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), d ** -0.5)
+    check_attention(out, q, k, v, s, tables, seqs, pos, d ** -0.5)
+
+
+@pytest.mark.parametrize("order", ["head", "token", "odd", "every"])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_layouts_and_index_types(order, index):
+    spans = [(0, 1), (40, 1), (299, 1), (15, 1), (16, 1)]
+    k, v, s = make_pool(40, 2, 128, "int8", order, seed=3)
+    if order != "head":
+        s = torch.stack([s, s], dim=3)[..., 1]  # strided scales
+    tables, seqs, pos, _ = batch(spans, 40)
+    q = torch.randn(5, 16, 2, 128, device=DEV).bfloat16()[:, :, 1]  # strided queries
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, index), dev(seqs, index),
+                                 dev(pos, index), 0.09)
+    check_attention(out, q, k, v, s, tables, seqs, pos, 0.09)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("d,heads,kvh", [(128, 16, 2), (64, 16, 4), (128, 8, 1), (128, 2, 2), (128, 14, 2), (64, 16, 1)])
+def test_chunks_beside_decode_rows(codes, d, heads, kvh):
+    spans = [(100, 1), (0, 70), (33, 1), (130, 2), (7, 3), (0, 1), (250, 45), (16, 16), (5, 33)]
+    k, v, s = make_pool(80, kvh, d, codes, seed=heads)
+    tables, seqs, pos, _ = batch(spans, 80)
+    q = torch.randn(len(seqs), heads, d, device=DEV).bfloat16()
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), d ** -0.5)
+    check_attention(out, q, k, v, s, tables, seqs, pos, d ** -0.5)
+
+
+@pytest.mark.parametrize("sm_scale", [0.0, -0.1, 1.0])
+@pytest.mark.parametrize("spans", [[(200, 1), (31, 1)], [(20, 50), (0, 40)]])
+def test_scale_signs(sm_scale, spans):
+    k, v, s = make_pool(40, 2, 128, "int8", seed=8)
+    tables, seqs, pos, _ = batch(spans, 40)
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), sm_scale)
+    check_attention(out, q, k, v, s, tables, seqs, pos, sm_scale)
+
+
+@pytest.mark.parametrize("spans", [[(699, 1), (63, 1)], [(500, 80), (0, 30)]])
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_page_scales_far_apart(codes, spans):
+    """V scales over 12 orders of magnitude and zero pages: the page with the largest scale must
+    not cost the others their precision, and a page whose scale is 0 holds zeros."""
+    k, v, s = make_pool(60, 2, 128, codes, seed=5)
+    tables, seqs, pos, _ = batch(spans, 60)
+    g = np.random.RandomState(0)
+    s[:, :, 1] *= dev(10.0 ** g.uniform(-6, 6, (60, 2)), torch.float32)
+    s[tables[0, 2], :, 1] = 0.0
+    s[tables[0, 3], :, 0] = 0.0
+    s[tables[1, 0]] = 0.0
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    args = (q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64))
+    check_attention(sb.ragged_attention_q8(*args, 0.5), q, k, v, s, tables, seqs, pos, 0.5)
+    s[:, :, 1] = 0.0
+    assert (sb.ragged_attention_q8(*args, 0.5) == 0).all()
+
+
+@pytest.mark.parametrize("spans", [[(30, 1), (5, 1), (16, 1)], [(0, 21), (16, 19)]])
+def test_what_lies_past_a_row_is_not_read(spans):
+    """Rows of the last page past the position hold NaN codes; the table's spare entries hold ids
+    outside the pool, and the spare pages' scales NaN."""
+    k, v, s = make_pool(20, 2, 128, "e4m3", seed=2)
+    tables, seqs, pos, _ = batch(spans, 16, width=9)
+    for r, (c, n) in enumerate(spans):
+        p, row = divmod(c + n, 16)
+        if row:
+            for pool in (k, v):
+                pool.view(torch.uint8)[tables[r, p], row:] = 0x7f
+        tables[r, (c + n + 15) // 16:] = [-7, 10 ** 6, 20, -1, 5][r]
+    s[16:] = float("nan")
+    k.view(torch.uint8)[16:] = 0x7f
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    K.device_errors(torch.device(DEV))
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), 0.1)
+    assert K.device_errors(torch.device(DEV)) == 0
+    kz, vz, sz = k.clone(), v.clone(), torch.nan_to_num(s)
+    for pool in (kz, vz):
+        raw = pool.view(torch.uint8)
+        raw[raw == 0x7f] = 0
+    check_attention(out, q, kz, vz, sz, tables, seqs, pos, 0.1)
+
+
+def test_rows_without_keys_and_bad_metadata():
+    k, v, s = make_pool(20, 2, 128, "int8", seed=1)
+    tables, seqs, pos, _ = batch([(20, 1)] * 8 + [(0, 12)], 20, width=2)
+    seqs, pos = seqs.copy(), pos.copy()
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    device = torch.device(DEV)
+
+    def call():
+        return sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32),
+                                      dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+
+    K.device_errors(device)
+    seqs[0] = seqs[10] = -1                    # padding, in a decode row and inside a run
+    pos[0] = pos[10] = -1
+    out = call()
+    assert K.device_errors(device) == 0
+    assert (out[0] == 0).all() and (out[10] == 0).all()
+    check_attention(out, q, k, v, s, tables, seqs, pos, 0.1)
+    for change, bit in (("seq", _native.SS_DEVERR_SEQ), ("low", _native.SS_DEVERR_POS),
+                        ("high", _native.SS_DEVERR_POS), ("page", _native.SS_DEVERR_PAGE)):
+        keep = seqs.copy(), pos.copy(), tables.copy()
+        if change == "seq":
+            seqs[2], seqs[12] = 9, -5
+        elif change == "low":
+            pos[2], pos[12] = -1, -3
+        elif change == "high":
+            pos[2] = pos[12] = 40              # clamped to the 32 keys the table can name
+        else:
+            tables[2, 0], tables[8, 0] = 20, -1
+        out = call()
+        assert K.device_errors(device) == bit, change
+        check_attention(out, q, k, v, s, tables, seqs, pos, 0.1)
+        seqs, pos, tables = keep
+
+
+def test_infinite_and_nan_queries_stay_in_their_row():
+    k, v, s = make_pool(40, 2, 128, "int8", seed=4)
+    tables, seqs, pos, _ = batch([(60, 1), (70, 1), (10, 40)], 40)
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    clean = q.clone()
+    q[0, 3, 5] = float("nan")
+    q[5, 9, 0] = float("nan")
+    q[7, 2, 1] = float("inf")
+    args = (k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    out, ref = sb.ragged_attention_q8(q, *args), sb.ragged_attention_q8(clean, *args)
+    for t, h in ((0, 3), (5, 9), (7, 2)):
+        assert out[t, h].isnan().all()
+        out[t, h] = ref[t, h]
+    assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("magnitude", [1e-30, 1e-3, 1e4, 1e30])
+def test_query_magnitudes(magnitude):
+    k, v, s = make_pool(40, 2, 128, "int8", seed=6)
+    tables, seqs, pos, _ = batch([(60, 1), (170, 1), (10, 40)], 40)
+    q = (torch.randn(len(seqs), 16, 128, device=DEV) * magnitude).bfloat16()
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), 0.1 / magnitude)
+    check_attention(out, q, k, v, s, tables, seqs, pos, 0.1 / magnitude)
+
+
+@pytest.mark.parametrize("rows", [[20000], [9000, 3, 4000], [1] * 300 + [700] * 9])
+def test_long_and_many_rows(rows):
+    pages = sum((n + 15) // 16 for n in rows)
+    k, v, s = make_pool(pages, 1, 128, "int8", seed=9)
+    tables, seqs, pos, _ = batch([(n - 1, 1) for n in rows], pages)
+    q = torch.randn(len(rows), 8, 128, device=DEV).bfloat16()
+    args = (q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    out = sb.ragged_attention_q8(*args)
+    check_attention(out, q, k, v, s, tables, seqs, pos, 0.1)
+    for _ in range(3):
+        assert torch.equal(out, sb.ragged_attention_q8(*args))
+
+
+@pytest.mark.parametrize("spans", [[(900, 1), (70, 1)], [(100, 60), (3, 1)]])
+def test_offsets_past_32_bits(spans):
+    """A pool of 4.3 GB per tensor whose used pages lie at its far end."""
+    pages, kvh, d = (1 << 21) + (1 << 17), 1, 128
+    k = torch.zeros((pages, 16, kvh, d), dtype=torch.int8, device=DEV)
+    v = torch.zeros_like(k)
+    s = torch.zeros((pages, kvh, 2), device=DEV)
+    sk, sv, ss = make_pool(100, kvh, d, "int8", "token", seed=7)
+    k[-100:], v[-100:], s[-100:] = sk, sv, ss
+    tables, seqs, pos, slots = batch(spans, 100)
+    q = torch.randn(len(seqs), 8, d, device=DEV).bfloat16()
+    far = dev(tables + pages - 100, torch.int32)
+    out = sb.ragged_attention_q8(q, k, v, s, far, dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    check_attention(out, q, sk, sv, ss, tables, seqs, pos, 0.1)
+    kn, vn = (torch.randn(len(seqs), kvh, d, device=DEV).bfloat16() for _ in range(2))
+    sb.kv_append_q8(k, v, s, kn, vn, dev(slots, torch.int64) + (pages - 100) * 16)
+    sb.kv_append_q8(sk, sv, ss, kn, vn, dev(slots, torch.int64))
+    assert torch.equal(k[-100:], sk) and torch.equal(v[-100:], sv) and torch.equal(s[-100:], ss)
+    assert not k[:-100].any() and not v[:-100].any() and not s[:-100].any()
+    got = sb.kv_read_q8(k, v, s, dev(slots, torch.int64) + (pages - 100) * 16)
+    for a, b in zip(got, sb.kv_read_q8(sk, sv, ss, dev(slots, torch.int64))):
+        assert torch.equal(a, b)
+
+
+# ---- append and read-back --------------------------------------------------------------------
+def check_append(codes, k, v, s, x, slots):
+    """`k, v, s` before the call, x = (k rows, v rows): runs the append and checks every page."""
+    before = [numbers(k), numbers(v)]
+    s0 = s.cpu().double().numpy().copy()
+    sb.kv_append_q8(k, v, s, x[0], x[1], dev(slots, torch.int64))
+    after, s1 = [numbers(k), numbers(v)], s.cpu().double().numpy()
+    share = 4 * 2.0 ** -24
+    for which in (0, 1):
+        rows = x[which].float().cpu().double().numpy()
+        want, written = oq.append_scales(s0[:, :, which], rows, slots, QMAX[codes])
+        assert np.all(np.abs(s1[:, :, which] - want) <= 2.0 ** -23 * want)
+        new = s1[:, :, which]
+        for page in range(len(want)):
+            if page not in written:
+                assert np.array_equal(after[which][page], before[which][page])
+                continue
+            for row in range(16):
+                with np.errstate(invalid="ignore", divide="ignore"):
+                    if row in written[page]:
+                        y = rows[written[page][row]] / new[page][:, None]
+                    else:
+                        old = 0.0 if 0 in written[page] else s0[page, :, which]
+                        y = before[which][page, row] * (old / new[page])[:, None]
+                y = np.where(new[page][:, None] > 0, y, 0.0)
+                y = np.clip(y, -QMAX[codes], QMAX[codes])
+                if codes == "int8":
+                    y = np.nan_to_num(y)
+                    half = 0.5
+                else:
+                    step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(np.nan_to_num(y)), 2.0 ** -6))) - 3)
+                    half = step / 2
+                got = after[which][page, row]
+                assert np.array_equal(np.isnan(got), np.isnan(y))
+                off = np.nan_to_num(np.abs(got - y)) - half
+                assert np.all(off <= QMAX[codes] * share + half * 1e-6), (page, row, off.max())
+    return after, s1
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("d,kvh,order", [(128, 2, "head"), (128, 1, "token"), (64, 4, "head"), (64, 3, "odd"), (128, 2, "every")])
+def test_append(codes, d, kvh, order):
+    k, v, s = make_pool(60, kvh, d, codes, order, seed=d)
+    spans = [(31, 1), (0, 1), (16, 1), (5, 40), (47, 17), (64, 16), (3, 2), (0, 16)]
+    _, _, _, slots = batch(spans, 60, seed=2)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    mag = torch.exp(torch.randn(len(slots), 1, 1, device=DEV, generator=g))
+    x = [(torch.randn(len(slots), kvh, d, device=DEV, generator=g) * mag).bfloat16() for _ in (0, 1)]
+    copies = [pool_like(k.clone(), order), pool_like(v.clone(), order), s.clone()]
+    check_append(codes, k, v, s, x, slots)
+    # The order of the tokens does not matter.
+    perm = np.random.RandomState(3).permutation(len(slots))
+    sb.kv_append_q8(*copies, x[0][perm], x[1][perm], dev(slots[perm], torch.int32))
+    for a, b in zip(copies, (k, v, s)):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    rk, rv = sb.kv_read_q8(k, v, s, dev(slots, torch.int64))
+    for which, (pool, got) in enumerate(((k, rk), (v, rv))):
+        want = (pool.float()[slots // 16, slots % 16]
+                * s[torch.from_numpy(slots // 16).to(DEV), :, which][:, :, None]).bfloat16()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 147, 148, 149, 700, 5000])
+def test_append_windows(tokens):
+    """Pages whose rows fall into several windows of the call, in scattered order."""
+    pages = (tokens + 15) // 16 + 3
+    k, v, s = make_pool(pages, 1, 64, "int8", seed=4)
+    rng = np.random.RandomState(tokens)
+    slots = rng.permutation(pages * 16)[:tokens].astype(np.int64)
+    x = [torch.randn(tokens, 1, 64, device=DEV).bfloat16() for _ in (0, 1)]
+    check_append("int8", k, v, s, x, slots)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_append_edges(codes):
+    k, v, s = make_pool(12, 1, 64, codes, seed=6)
+    # duplicates (the later token stays), zeros, tiny values, NaN and infinities, a zero old scale
+    slots = np.array([3, 3, 16, 17, 32, 50, 66, 81, 98, 113, 130, 130, 130], np.int64)
+    x = [torch.randn(len(slots), 1, 64, device=DEV).bfloat16() for _ in (0, 1)]
+    for t in x:
+        t[2:4] = 0.0
+        t[4] = 1e-35
+        t[5] = 1e-35
+        t[6, 0, 7] = float("nan")
+        t[7, 0, 9] = float("inf")
+        t[7, 0, 10] = float("-inf")
+        t[8] = 3e38
+        t[9] = 0.0
+    s[7] = 0.0                                 # page 7: an all-zero page whose codes are stale
+    check_append(codes, k, v, s, x, slots)
+    assert (s[1] == 0).all() and (s[2] == 0).all() and not numbers(k)[1:3].any()
+
+
+def test_append_skips_and_flags():
+    k, v, s = make_pool(4, 1, 64, "int8", seed=6)
+    keep = k.clone(), v.clone(), s.clone()
+    x = torch.randn(5, 1, 64, device=DEV).bfloat16()
+    K.device_errors(torch.device(DEV))
+    sb.kv_append_q8(k, v, s, x, x, dev([-1] * 5, torch.int64))
+    assert K.device_errors(torch.device(DEV)) == 0
+    sb.kv_append_q8(k, v, s, x, x, dev([64, -2, 1 << 40, -1, -1], torch.int64))
+    assert K.device_errors(torch.device(DEV)) == _native.SS_DEVERR_SLOT
+    assert all(torch.equal(a, b) for a, b in zip(keep, (k, v, s)))
+    sb.kv_append_q8(k, v, s, x[:0], x[:0], dev([], torch.int64))
+    rk, rv = sb.kv_read_q8(k, v, s, dev([-1, 5], torch.int64))
+    assert K.device_errors(torch.device(DEV)) == 0
+    assert not rk[0].any() and not rv[0].any() and rk[1].any()
+    rk, _ = sb.kv_read_q8(k, v, s, dev([64, 5], torch.int64))
+    assert K.device_errors(torch.device(DEV)) == _native.SS_DEVERR_SLOT and not rk[0].any()
+    assert sb.kv_read_q8(k, v, s, dev([], torch.int64))[0].shape == (0, 1, 64)
+
+
+def test_token_by_token_stays_near_the_values():
+    """Sixteen appends into one page: each growth of the scale rounds the older codes once more,
+    by at most half a step of the scale it grows to; the steps sum to at most 16 halves."""
+    k, v, s = (t.clone() for t in make_pool(2, 1, 128, "int8", seed=1))
+    x = torch.randn(16, 1, 128, device=DEV).bfloat16() * torch.linspace(0.2, 3, 16, device=DEV)[:, None, None]
+    x = x.bfloat16()
+    for t in range(16):
+        sb.kv_append_q8(k, v, s, x[t:t + 1], x[t:t + 1], dev([16 + t], torch.int64))
+    step = float(s[1, 0, 0])
+    got = k[1].float() * step
+    assert float((got - x.float()).abs().max()) <= 16 * step / 2 * 1.001
+    assert abs(step - float(x.abs().max()) / 127) <= 1e-6
+
+
+# ---- block tables ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 3, 64, 700, 5000])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_block_tables(rows, index):
+    rng = np.random.RandomState(rows)
+    cached = rng.randint(0, 200, rows)
+    new = np.where(rng.rand(rows) < 0.1, rng.randint(0, 120, rows), rng.randint(0, 2, rows))
+    width = 21
+    tables = rng.randint(0, 10 ** 6, (rows, width))
+    free = rng.permutation(10 ** 6)[:rows * 10]
+    tokens = int(new.sum()) + rng.randint(0, 40)
+    want = oq.block_tables(cached, new, tables, free, 5, tokens)
+    t = dev(tables, index)
+    head = torch.tensor([5], dtype=torch.int32, device=DEV)
+    K.device_errors(torch.device(DEV))
+    got = sb.build_block_tables(dev(cached, index), dev(new, index), t, dev(free, index), head, tokens)
+    assert K.device_errors(torch.device(DEV)) == 0
+    assert got["tables"] is t
+    for key, value in want.items():
+        assert np.array_equal(got[key].cpu().numpy(), value), key
+
+
+def test_block_tables_steps_in_place_and_runs_out():
+    rng = np.random.RandomState(0)
+    cached, new = np.array([0, 15, 16, 31]), np.array([1, 1, 1, 1])
+    tables, free = np.full((4, 4), -1), rng.permutation(100)[:9]
+    tables[1, 0], tables[2, 0], tables[3, :2] = 90, 91, (92, 93)
+    lens, head = dev(cached, torch.int32), torch.zeros(1, dtype=torch.int32, device=DEV)
+    t = dev(tables, torch.int32)
+    h = 0
+    K.device_errors(torch.device(DEV))
+    for step in range(34):
+        want = oq.block_tables(cached, new, tables, free, h, 6)
+        got = sb.build_block_tables(lens, dev(new, torch.int32), t, dev(free, torch.int32), head, 6,
+                                    out={"lens": lens, "free_head": head})
+        for key, value in want.items():
+            assert np.array_equal(got[key].cpu().numpy(), value), (step, key)
+        cached, tables, h = want["lens"], want["tables"], int(want["free_head"][0])
+        bits = K.device_errors(torch.device(DEV))
+        past = (cached > 64).any()
+        assert bool(bits & _native.SS_DEVERR_POS) == past
+    assert h == 9 and (tables == -1).any()      # the free list ran out: -1 entries
+
+
+def test_block_tables_bad_lengths():
+    cached, new = np.array([-3, 60, 10]), np.array([2, 10, -4])
+    tables, free = np.zeros((3, 4), np.int64), np.arange(1, 40)
+    want = oq.block_tables(cached, new, tables, free, 0, 7)   # 12 new tokens, 7 places
+    K.device_errors(torch.device(DEV))
+    got = sb.build_block_tables(dev(cached, torch.int32), dev(new, torch.int32),
+                                dev(tables, torch.int32), dev(free, torch.int32),
+                                torch.zeros(1, dtype=torch.int32, device=DEV), 7)
+    assert K.device_errors(torch.device(DEV)) == _native.SS_DEVERR_POS
+    for key, value in want.items():
+        assert np.array_equal(got[key].cpu().numpy(), value), key
+
+
+# ---- streams, graphs, refusals -----------------------------------------------------------------
+def test_other_stream_and_graph():
+    """Tables, append and attention on a stream of their own and in a captured graph that advances
+    itself, against the same steps run eagerly."""
+    rows, steps = 6, 20
+
+    def state():
+        k, v, s = make_pool(64, 2, 128, "int8", seed=11)
+        cached = np.array([0, 5, 15, 16, 100, 31])
+        tables = np.full((rows, 10), -1)
+        at = 0
+        for r, c in enumerate(cached):
+            n = (c + 15) // 16
+            tables[r, :n] = np.arange(at, at + n)
+            at += n
+        return dict(k=k, v=v, s=s, lens=dev(cached, torch.int32), t=dev(tables, torch.int32),
+                    free=torch.arange(at, 64, dtype=torch.int32, device=DEV),
+                    head=torch.zeros(1, dtype=torch.int32, device=DEV),
+                    one=torch.ones(rows, dtype=torch.int32, device=DEV),
+                    q=torch.zeros(8, 16, 128, device=DEV).bfloat16(),
+                    kn=torch.zeros(8, 2, 128, device=DEV).bfloat16(),
+                    vn=torch.zeros(8, 2, 128, device=DEV).bfloat16())
+
+    def step(st):
+        m = sb.build_block_tables(st["lens"], st["one"], st["t"], st["free"], st["head"], 8,
+                                  out={"lens": st["lens"], "free_head": st["head"]})
+        sb.kv_append_q8(st["k"], st["v"], st["s"], st["kn"], st["vn"], m["slots"])
+        return sb.ragged_attention_q8(st["q"], st["k"], st["v"], st["s"], m["tables"], m["seqs"],
+                                      m["positions"], 0.1)
+
+    g = torch.Generator(device=DEV).manual_seed(0)
+    feeds = [[torch.randn(x.shape, device=DEV, generator=g).bfloat16() for x in
+              (torch.empty(8, 16, 128), torch.empty(8, 2, 128), torch.empty(8, 2, 128))]
+             for _ in range(steps)]
+
+    def feed(st, i):
+        for name, x in zip(("q", "kn", "vn"), feeds[i]):
+            st[name].copy_(x)
+
+    eager = state()
+    want = []
+    for i in range(steps):
+        feed(eager, i)
+        want.append(step(eager).clone())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    a = state()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = []
+        for i in range(steps):
+            feed(a, i)
+            got.append(step(a).clone())
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    b = state()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(b)
+    for i in range(steps):
+        feed(b, i)
+        graph.replay()
+        assert torch.equal(out, want[i]), i
+    assert torch.equal(b["lens"], eager["lens"]) and torch.equal(b["t"], eager["t"])
+    assert K.device_errors(torch.device(DEV)) == 0
+
+
+def test_cache_class():
+    from helpers import FreeListPages
+
+    cfg = dict(num_hidden_layers=2, num_key_value_heads=2, hidden_size=2048, num_attention_heads=16)
+    for dtype in (None, torch.float8_e4m3fn):
+        c = sb.QuantizedCache(cfg, 1, 20, DEV, dtype, allocator=FreeListPages)
+        assert c.shape == (2, 28, 16, 2, 128) and tuple(c.k.shape) == c.shape
+        codes = "int8" if dtype is None else "e4m3"
+        spans = [(0, 40), (0, 17)]
+        tables, seqs, pos, slots = batch(spans, 20)
+        x = [torch.randn(57, 2, 128, device=DEV).bfloat16() for _ in (0, 1)]
+        c.write(1, x[0], x[1], dev(slots, torch.int64))
+        assert not c.k[0].view(torch.uint8).any()
+        q = torch.randn(57, 16, 128, device=DEV).bfloat16()
+        out = c.attend(1, q, dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+        check_attention(out, q, c.k[1], c.v[1], c.scales[1], tables, seqs, pos, 0.1)
+        k, _ = c.read(1, dev(slots, torch.int64))
+        # half a step: of 1 / 127 of the block's largest, or 32 of 448 in e4m3's top binade
+        assert float((k.float() - x[0].float()).abs().max()) <= float(x[0].abs().max()) * (
+            2.0 ** -9 + (1 / 254 if codes == "int8" else 16 / 448))
+    with pytest.raises(sb.KernelUnsupported):
+        sb.QuantizedCache(cfg, 1, 20, DEV, torch.bfloat16, allocator=FreeListPages)
+    with pytest.raises(sb.KernelUnsupported):
+        sb.QuantizedCache(cfg, 1, 20, "cpu", allocator=FreeListPages)
+    with pytest.raises(sb.KernelUnsupported):
+        sb.QuantizedCache(cfg, 1, 20, DEV, allocator=FreeListPages, scratch_pages=-1)
+
+
+def _refusals():
+    k, v, s = make_pool(8, 2, 128, "int8")
+    q = torch.zeros(3, 16, 128, device=DEV).bfloat16()
+    bt = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    i = torch.zeros(3, dtype=torch.int32, device=DEV)
+    x = torch.zeros(3, 2, 128, device=DEV).bfloat16()
+    attend = dict(q=q, k=k, v=v, s=s, bt=bt, seq=i, pos=i)
+    append = dict(k=k, v=v, s=s, kn=x, vn=x, slots=i)
+    for name, value in [("q", q.half()), ("q", q.cpu()), ("q", q[0]), ("q", q[..., :96]),
+                        ("q", q[:, :15]), ("q", q[:0]), ("q", q[..., :64]), ("k", k[:, :8]),
+                        ("k", k.float()), ("v", v.view(torch.uint8)), ("v", v[:4]), ("s", s[:4]),
+                        ("s", s.half()), ("s", s.cpu()), ("s", s[:, :, :1]), ("bt", bt[0]),
+                        ("bt", bt.cpu()), ("bt", bt.float()), ("bt", bt[:, :0]), ("seq", i[:2]),
+                        ("seq", i.float()), ("pos", i[:2]), ("pos", i.cpu()), ("v", v.cpu())]:
+        yield "attend", dict(attend, **{name: value})
+    for name, value in [("k", k.cpu()), ("k", k[..., :96]), ("v", v[:4]), ("s", s[:, :1]),
+                        ("kn", x[:2]), ("kn", x.float()), ("vn", x[:, :1]), ("vn", x.cpu()),
+                        ("slots", i[:2]), ("slots", i.float()), ("slots", i.cpu())]:
+        yield "append", dict(append, **{name: value})
+    read = dict(k=k, v=v, s=s, slots=i)
+    for name, value in [("slots", i.cpu()), ("slots", i.float()), ("k", k.cpu()), ("s", s[:4])]:
+        yield "read", dict(read, **{name: value})
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    two = torch.zeros(2, dtype=torch.int32, device=DEV)
+    tables = dict(c=two, n=two, bt=bt, f=i, h=one, t=3, out=None)
+    for name, value in [("c", i), ("n", i), ("c", two.cpu()), ("bt", bt[0]), ("bt", bt.cpu()),
+                        ("bt", bt[:, :0]), ("f", i.cpu()), ("f", i.float()), ("h", two),
+                        ("h", one.long()), ("t", -1), ("n", two.float()),
+                        ("out", {"slots": i}), ("out", {"seqs": i[:2]}), ("out", {"lens": two.cpu()})]:
+        yield "tables", dict(tables, **{name: value})
+    big = torch.zeros(12289, dtype=torch.int32, device=DEV)
+    yield "tables", dict(tables, c=big, n=big, bt=torch.zeros(12289, 1, dtype=torch.int32, device=DEV))
+
+
+def test_refusals():
+    call = {"attend": lambda a: sb.ragged_attention_q8(a["q"], a["k"], a["v"], a["s"], a["bt"], a["seq"], a["pos"], 0.1),
+            "append": lambda a: sb.kv_append_q8(a["k"], a["v"], a["s"], a["kn"], a["vn"], a["slots"]),
+            "read": lambda a: sb.kv_read_q8(a["k"], a["v"], a["s"], a["slots"]),
+            "tables": lambda a: sb.build_block_tables(a["c"], a["n"], a["bt"], a["f"], a["h"], a["t"], a["out"])}
+    for op, args in _refusals():
+        with pytest.raises(sb.KernelUnsupported):
+            call[op](args)
+    k, v, sc = make_pool(8, 2, 128, "int8")
+    i = torch.zeros(3, dtype=torch.int32, device=DEV)
+    with pytest.raises(sb.KernelUnsupported):
+        sb.ragged_attention_q8(torch.zeros(3, 16, 128, device=DEV).bfloat16(), k, v, sc,
+                               torch.zeros(2, 4, dtype=torch.int32, device=DEV), i, i, float("nan"))
