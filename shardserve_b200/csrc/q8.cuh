@@ -111,6 +111,12 @@ __device__ __forceinline__ TokInfo q8_token_info(const AttnArgs& a, long long t,
 cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_generic(const Q8AttnArgs& a, cudaStream_t stream);
+// Split-K kernel (q8_decode.cu): workspace bytes, the layouts it addresses, and the launch
+// (*launches: kernels enqueued).  Tokens of runs of at least min_run tokens are left out (0: none).
+size_t q8_decode_workspace(int device);
+bool q8_decode_supported(const Q8AttnArgs& g);
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, int min_run, int device, void* workspace,
+                             cudaStream_t stream, int* launches);
 cudaError_t launch_block_tables(const BlockTablesArgs& a, cudaStream_t stream);
 int block_tables_max_rows();
 

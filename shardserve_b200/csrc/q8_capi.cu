@@ -115,8 +115,7 @@ int ss_q8_workspace_bytes(int device, int heads, int kv_heads, int head_dim, siz
   if (head_dim != 64 && head_dim != 128) return invalid("head_dim must be 64 or 128");
   if (heads < 1 || kv_heads < 1 || heads % kv_heads)
     return invalid("query heads must be divisible by KV heads");
-  (void)device;
-  *bytes = ss::kWsHeader;
+  *bytes = ss::q8_decode_workspace(device);
   return SS_OK;
 }
 
@@ -143,11 +142,15 @@ int ss_ragged_paged_attention_q8(
   if (!nonneg(q_strides, 3) || !nonneg(bt_strides, 2) || !nonneg(out_strides, 3))
     return invalid("negative strides are not supported");
   if (!std::isfinite(sm_scale)) return invalid("sm_scale must be finite");
+  if (!workspace) {
+    ss::set_error_message("a workspace is required");
+    return SS_ERR_WORKSPACE;
+  }
   int device = 0;
-  cudaError_t e = cudaSuccess;
-  size_t need = 0;
-  if (ss_q8_workspace_bytes(device, heads, kv_heads, head_dim, &need) != SS_OK) return SS_ERR_INVALID;
-  if (!workspace || workspace_bytes < need) {
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_failed(e, "cudaGetDevice");
+  const size_t need = ss::q8_decode_workspace(device);
+  if (workspace_bytes < need) {
     ss::set_error_message("a workspace of at least %zu bytes is required", need);
     return SS_ERR_WORKSPACE;
   }
@@ -168,6 +171,14 @@ int ss_ragged_paged_attention_q8(
   a.sm_scale = sm_scale;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.err = static_cast<unsigned*>(workspace);
+  if (ss::q8_decode_supported(g)) {
+    int launches = 0;
+    e = ss::launch_q8_decode(g, 0, device, workspace, static_cast<cudaStream_t>(stream), &launches);
+    ss::count_launches(static_cast<unsigned>(launches));
+    if (e != cudaSuccess) return cuda_failed(e, "q8 split-K attention launch");
+    ss::set_last_path(5);
+    return SS_OK;
+  }
   e = ss::launch_q8_generic(g, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_failed(e, "q8 attention launch");
   ss::count_launches(1);

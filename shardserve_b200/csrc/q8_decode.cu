@@ -1,0 +1,772 @@
+// Split-K ragged paged attention over the 8-bit pool for decode-style query tokens.
+//
+// Mathematics, per query token and KV head (G query heads share the head's codes):
+//   x_ih = (q_h . Kc_i) * ks_page * sm_scale * log2 e + log2(vs_page),   w_ih = 2^(x_ih - r_h)
+//   O_h  = sum_i w_ih Vc_i,   l_h = sum_i w_ih / vs_page,   out_h = O_h / l_h
+// with Kc / Vc the codes and ks / vs their page's scales: the V scale rides in the exponent, so
+// the products see the codes themselves, exact in fp16 and tf32, and no page's scale costs
+// another page precision.  r_h is raised only when a weight would pass 2^20, found by a vote: most
+// pages need no warp reduction.  Q.K is an fp16 product (q is exact there once its row's power of
+// two is taken out).  The weights are rounded to tf32: 11 bits like fp16, but with fp32's range
+// (fp16 would flush weights 2^30 below the row's largest, which are all there is of an output
+// dimension whose leading keys hold code 0; bf16 has the range and three bits less).  Everything
+// else is fp32.
+//
+// What bounds it: HBM (2 * head_dim bytes per key and KV head), once the ~300 instructions per
+// 4 KiB page (two thirds of them widen bytes) stay below the issue rate.
+//
+// Layout in registers.  The operands of mma.sync are wider than the codes, so the bytes pass
+// through registers anyway; they are loaded there straight from global memory in fragment order,
+// with no shared memory in between.  The order of head_dim and of the keys inside a product is
+// free as long as both operands agree.  Lane (g, t) = (lane / 4, lane % 4):
+//   S = Q K^T       m16n8k16, M = query heads (of one KV head), N = 8 keys.  The lane loads bytes
+//                   [64 c + 16 t, +16) of keys g and g + 8 (16-byte loads); Q is loaded to match.
+//   O^T = V^T P^T   m16n8k8, M = 16 values of head_dim, N = 8 heads, K = 8 keys.  The lane loads
+//                   bytes [D/8 g, +D/8) of keys 2t, 2t+1, 2t+8, 2t+9, which are the keys whose
+//                   weights for head g it already holds: S's accumulators are P^T's operand.
+// A lane's V bytes are consecutive, so its outputs are 32 consecutive bytes of an output row.
+// K's registers are refilled for the next page as soon as the page's scores are done, V's when
+// its product is: 4 KiB in flight per warp, 64 KiB per SM.
+//
+// Work split.  Unit = (row, page), row = (token, KV head).  One CTA per SM takes an equal run of
+// units and every warp an equal run of the CTA's.  A row inside a warp's run goes straight to the
+// output.  Rows cut by warp boundaries leave fp32 partial states in shared memory, combined by
+// the CTA; rows cut by CTA boundaries leave one state per CTA in the workspace, and the CTA that
+// arrives last at the row's counter combines them in CTA order (no CTA waits for another one, and
+// the bits do not depend on who arrives last).
+#include <cuda_bf16.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "ptx.cuh"
+#include "q8.cuh"
+
+namespace ss {
+
+namespace {
+
+constexpr int kMaxTok = 6144;     // query tokens per launch (row lists in shared memory)
+constexpr int kMaxCtas = 1024;    // counters in the workspace
+constexpr int kCounterBytes = 4 * kMaxCtas;
+constexpr float kSlack = 20.f;    // weights stay below 2^20 (of the reference they started with)
+constexpr float kMinVs = 0x1p-80f;  // smaller V scales count as 0
+
+template <int D, int NG>
+struct DecTraits {
+  static constexpr int kWarps = NG == 1 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int KT = 128 / D;         // 16-key tiles (pages) per step
+  static constexpr int C = D / 64;           // 64-byte chunks of a K row
+  static constexpr int MT = D / 16;          // 16-value tiles of the output
+  static constexpr int VW = D / 32;          // 32-bit words a lane holds of a V row
+  static constexpr int kRows = 8 * NG;       // query heads of a row (padded)
+  static constexpr int kState = kRows * D + 2 * kRows;  // floats of a partial state: O, r, l
+};
+
+struct Piece {  // a warp's part of a row that others share
+  int row;      // -1: none
+  int first;    // the row's first page is inside
+  int last;     // the row's last page is inside
+};
+
+// Four int8 codes as two fp16 pairs: byte u + 128 under exponent 2^10 reads 1152 + u.
+__device__ __forceinline__ uint32_t sub_1152(uint32_t h) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
+  return r;
+}
+template <int FMT>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == SS_CODE_INT8) {
+    w ^= 0x80808080u;
+    lo = sub_1152(__byte_perm(w, 0x64646464u, 0x4140));
+    hi = sub_1152(__byte_perm(w, 0x64646464u, 0x4342));
+  } else {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+// Four codes of a word as fp32 (tf32 holds them exactly).  2^23 + u is the integer u's fp32
+// pattern under exponent 2^23.
+template <int FMT>
+__device__ __forceinline__ void widen_f32(uint32_t w, uint32_t (&f)[4]) {
+  if constexpr (FMT == SS_CODE_INT8) {
+    w ^= 0x80808080u;
+    const uint64_t off = f2pack(-8388736.f, -8388736.f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t v = add2(f2pack(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + 2 * i)),
+                                     __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441 + 2 * i))),
+                              off);
+      f[2 * i] = static_cast<uint32_t>(v);
+      f[2 * i + 1] = static_cast<uint32_t>(v >> 32);
+    }
+  } else {
+    uint32_t h[2];
+    widen<FMT>(w, h[0], h[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      f[2 * i] = __float_as_uint(v.x);
+      f[2 * i + 1] = __float_as_uint(v.y);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Streamed loads: the codes are read once per call.
+__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+struct DecParams {
+  Q8AttnArgs g;
+  int t0, tn;          // tokens of this launch
+  int min_run;         // tokens of runs at least this long belong to the tile kernel (0: none)
+  int min_chunk;       // fewest units of a CTA
+  unsigned* counter;   // [kMaxCtas], zero between calls
+  float* part;         // [2 * grid] partial states
+};
+
+// Folds `n` states, state i at `at(i)`, into one; thread `e` of the group handles float4 e.
+template <int D, int NG, typename At>
+__device__ __forceinline__ void fold(At at, int n, int e, float4& o, float& r, float& l) {
+  using Tr = DecTraits<D, NG>;
+  const int head = e / (D / 4);
+  o = make_float4(0.f, 0.f, 0.f, 0.f);
+  r = -CUDART_INF_F;
+  l = 0.f;
+  constexpr int U = 8;
+  for (int i0 = 0; i0 < n; i0 += U) {
+    float rv[U], lv[U];
+    float4 ov[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      rv[u] = -CUDART_INF_F;
+      lv[u] = 0.f;
+      ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + u < n) {
+        const float* s = at(i0 + u);
+        rv[u] = __ldcg(s + Tr::kRows * D + head);
+        lv[u] = __ldcg(s + Tr::kRows * D + Tr::kRows + head);
+        ov[u] = __ldcg(reinterpret_cast<const float4*>(s) + e);
+      }
+    }
+    float rn = r;
+#pragma unroll
+    for (int u = 0; u < U; ++u) rn = fmaxf(rn, rv[u]);
+    const float ref = rn == -CUDART_INF_F ? 0.f : rn;
+    const float f = ex2(r - ref);
+    o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+    l *= f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = ex2(rv[u] - ref);
+      o.x += ov[u].x * w; o.y += ov[u].y * w; o.z += ov[u].z * w; o.w += ov[u].w * w;
+      l += lv[u] * w;
+    }
+    r = rn;
+  }
+}
+
+template <int D, int NG>
+struct DecSmem {
+  using Tr = DecTraits<D, NG>;
+  alignas(16) float state[Tr::kWarps][2][Tr::kState];
+  Piece piece[Tr::kWarps][2];
+  int pre[kMaxTok + 1];  // units before each token
+  int seq[kMaxTok];
+  int len[kMaxTok];
+  int scan[Tr::kWarps];
+  int arrived;
+};
+
+template <int D, int FMT, int NG>
+__global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
+    q8_decode_kernel(const __grid_constant__ DecParams P) {
+  using Tr = DecTraits<D, NG>;
+  constexpr int NW = Tr::kWarps, NT = Tr::kThreads, KT = Tr::KT, C = Tr::C, MT = Tr::MT, VW = Tr::VW;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  DecSmem<D, NG>& sm = *reinterpret_cast<DecSmem<D, NG>*>(smem_raw);
+  const AttnArgs& a = P.g.a;
+  const Q8Pool& pool = P.g.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ---- units before every token ----------------------------------------------------------
+  const int per = (P.tn + NT - 1) / NT;
+  const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
+  int sum = 0;
+  for (int i = b0; i < b1; ++i) {
+    const long long t = P.t0 + i;
+    const TokInfo ti = q8_token_info(a, t, blockIdx.x == 0);
+    const bool mine = !token_in_long_run(a, P.min_run, t, ti.seq);
+    const int np = mine ? ti.npages : 0;
+    sm.seq[i] = static_cast<int>(ti.seq);
+    sm.len[i] = mine ? ti.L : -1;
+    sm.pre[i] = sum;  // within this thread's run
+    sum += np * a.KVH;
+  }
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 31) sm.scan[warp] = inc;
+  if (tid < 2 * NW) sm.piece[tid >> 1][tid & 1].row = -1;
+  __syncthreads();
+  int before = inc - sum, U = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int s = sm.scan[w];
+    if (w < warp) before += s;
+    U += s;
+  }
+  for (int i = b0; i < b1; ++i) sm.pre[i] += before;
+  if (tid == 0) sm.pre[P.tn] = U;
+  __syncthreads();
+  // Tokens of this launch without keys: zero rows, spread over the CTAs.
+  for (int i = blockIdx.x; i < P.tn; i += gridDim.x) {
+    if (sm.len[i] != 0) continue;
+    for (int e = tid; e < a.H * D; e += NT)
+      a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
+  }
+  const int chunk = max((U + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), P.min_chunk);
+  const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
+  if (c0 >= U) return;
+  const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
+  // Warps 0 .. nwa - 1 hold at least one unit each.
+  const int nwa = min(NW, n_cta), wq = n_cta / nwa, wr = n_cta % nwa;
+  int u = static_cast<int>(c0) + warp * wq + min(warp, wr);
+  const int u1 = warp < nwa ? u + wq + (warp < wr ? 1 : 0) : u;
+
+  const int g = lane >> 2, t4 = lane & 3;
+  int tok = 0;  // token of unit u
+  if (u < u1) {
+    int lo = 0, hi = P.tn;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.pre[mid] <= u) lo = mid; else hi = mid;
+    }
+    tok = lo;
+  }
+  while (u < u1) {
+    while (sm.pre[tok + 1] <= u) ++tok;
+    const int L = sm.len[tok], np = (L + kPage - 1) / kPage;
+    const int rem = u - sm.pre[tok];
+    const int h = rem / np, p0 = rem - h * np;
+    const int cnt = min(np - p0, u1 - u);  // pages of this segment
+    const long long btrow = static_cast<long long>(sm.seq[tok]) * a.bt_sb;
+    const long long t = P.t0 + tok;
+
+    // Page ids, 32 at a time (lane i: page p0 + base + i).
+    auto load_ids = [&](int base) -> int {
+      const int i = base + lane;
+      int id = -1;
+      if (i < cnt) {
+        const long long pid = ld_index(a.bt, a.bt64, btrow + static_cast<long long>(p0 + i) * a.bt_sn);
+        if (pid >= 0 && pid < pool.N)
+          id = static_cast<int>(pid);
+        else
+          atomicOr(a.err, SS_DEVERR_PAGE);
+      }
+      return id;
+    };
+    int ids = load_ids(0), ids_next = load_ids(32);
+
+    uint32_t kr[KT][2][C][4], vr[KT][4][VW];
+    float2 sc[KT], sc_next[KT];
+    const uint8_t* kbase = pool.k + static_cast<long long>(h) * pool.k_sh + 16 * t4;
+    const uint8_t* vbase = pool.v + static_cast<long long>(h) * pool.v_sh + (D / 8) * g;
+    const float* sbase = pool.scales + static_cast<long long>(h) * pool.s_sh;
+    auto page_of = [&](int i) -> int {  // i < cnt + KT, called by the whole warp in order
+      return i < cnt ? __shfl_sync(0xffffffffu, ids, i & 31) : -1;
+    };
+    int pg[KT];
+    auto keys_of = [&](int i) { return i < cnt ? min(kPage, L - (p0 + i) * kPage) : 0; };
+    auto load_k = [&](int i) {  // K codes and scales of pages i .. i + KT - 1
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const int n = pg[k] < 0 ? 0 : keys_of(i + k);
+        sc_next[k] = make_float2(0.f, 1.f);
+        if (n > 0) {
+          const float* s = sbase + pg[k] * pool.s_sn;
+          sc_next[k].x = __ldg(s);
+          sc_next[k].y = __ldg(s + pool.s_sw);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (g + 8 * r < n)
+              v = ld_stream16(kbase + pg[k] * pool.k_sn + (g + 8 * r) * pool.k_ss + 64 * c);
+            kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
+          }
+      }
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const int n = pg[k] < 0 ? 0 : keys_of(i + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = 2 * t4 + (j & 1) + 8 * (j >> 1);
+          const uint8_t* p = vbase + pg[k] * pool.v_sn + key * pool.v_ss;
+          if constexpr (VW == 4) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (key < n) v = ld_stream16(p);
+            vr[k][j][0] = v.x; vr[k][j][1] = v.y; vr[k][j][VW - 2] = v.z; vr[k][j][VW - 1] = v.w;
+          } else {
+            uint2 v = make_uint2(0, 0);
+            if (key < n) v = ld_stream8(p);
+            vr[k][j][0] = v.x; vr[k][j][1] = v.y;
+          }
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < KT; ++k) pg[k] = page_of(k);
+    load_k(0);
+    load_v(0);
+
+    // Queries as fp16 with the row's power of two taken out: lane (g, t) holds head g's values
+    // [64 c + 16 t, +16), the order of the K bytes.
+    uint32_t qf[NG][C][4][2];
+    float qs[NG];  // of head 8 n + g: 2^e * sm_scale * log2 e
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int hd = 8 * n + g;
+      uint32_t raw[C][8];
+      float amax = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (hd < a.group)
+            v = __ldg(reinterpret_cast<const uint4*>(
+                a.q + t * a.q_st + static_cast<long long>(h * a.group + hd) * a.q_sh + 64 * c + 16 * t4 + 8 * w));
+          raw[c][4 * w] = v.x; raw[c][4 * w + 1] = v.y; raw[c][4 * w + 2] = v.z; raw[c][4 * w + 3] = v.w;
+        }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[c][w] << 16)),
+                                   fabsf(__uint_as_float(raw[c][w] & 0xffff0000u))));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[c][w] << 16) * down,
+                                             __uint_as_float(raw[c][w] & 0xffff0000u) * down);
+      qs[n] = up;
+    }
+
+    float acc[NG][MT][4], ref[NG], lsum[NG];  // ref, lsum: of head 8 n + g
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
+      ref[n] = -CUDART_INF_F;
+      lsum[n] = 0.f;
+    }
+
+    for (int i = 0; i < cnt; i += KT) {
+      // ---- scores: x[k][r][j + 2 n] of key 8 r + 2 t + j, head 8 n + g ----------------------
+      float x[KT][2][4];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        sc[k] = sc_next[k];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[k][r][j] = 0.f;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t b0, b1;
+              widen<FMT>(kr[k][r][c][w], b0, b1);
+              mma_f16(x[k][r], qf[0][c][w][0], NG == 2 ? qf[NG - 1][c][w][0] : 0u, qf[0][c][w][1],
+                      NG == 2 ? qf[NG - 1][c][w][1] : 0u, b0, b1);
+            }
+        }
+      }
+      int nk[KT];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) nk[k] = keys_of(i + k);
+      // ---- the next pages' K ---------------------------------------------------------------
+      if (((i + KT) & 31) == 0) {
+        ids = ids_next;
+        ids_next = load_ids(i + KT + 32);
+      }
+#pragma unroll
+      for (int k = 0; k < KT; ++k) pg[k] = page_of(i + KT + k);
+      load_k(i + KT);
+      // ---- weights --------------------------------------------------------------------------
+      bool raise = false;
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const float lv = lg2(fmaxf(sc[k].y, kMinVs));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float f = sc[k].x * qs[n];
+          float top = -CUDART_INF_F;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& v = x[k][r][2 * n + j];
+              v = fmaf(v, f, lv);
+              if (nk[k] < kPage && 8 * r + 2 * t4 + j >= nk[k]) v = -CUDART_INF_F;
+              top = fmaxf(top, v);
+            }
+          raise |= top > ref[n] + kSlack;
+        }
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          float m = ref[n];
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) m = max3(m, x[k][r][2 * n], x[k][r][2 * n + 1]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const float f = m == -CUDART_INF_F ? 1.f : ex2(ref[n] - m);
+          ref[n] = m;
+          lsum[n] *= f;
+          const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+#pragma unroll
+          for (int q = 0; q < MT; ++q) {
+            acc[n][q][0] *= f0;
+            acc[n][q][1] *= f1;
+            acc[n][q][2] *= f0;
+            acc[n][q][3] *= f1;
+          }
+        }
+      }
+      uint32_t pb[KT][NG][2][2];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const float iv = __frcp_rn(fmaxf(sc[k].y, kMinVs));
+        const uint32_t keep = sc[k].y >= kMinVs ? ~0u : 0u;  // a page whose scale is 0 holds zeros
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float base = ref[n] == -CUDART_INF_F ? 0.f : ref[n];
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float w = ex2(x[k][r][2 * n + j] - base);
+              sum += w;
+              pb[k][n][r][j] = to_tf32(w) & keep;
+            }
+          lsum[n] = fmaf(sum, iv, lsum[n]);
+        }
+      }
+      // ---- values ---------------------------------------------------------------------------
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t v0[4], v1[4];  // keys 8 r + 2 t and the one after
+            widen_f32<FMT>(vr[k][2 * r][w], v0);
+            widen_f32<FMT>(vr[k][2 * r + 1][w], v1);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+              mma_tf32(acc[n][2 * w], v0[0], v0[1], v1[0], v1[1], pb[k][n][r][0], pb[k][n][r][1]);
+              mma_tf32(acc[n][2 * w + 1], v0[2], v0[3], v1[2], v1[3], pb[k][n][r][0], pb[k][n][r][1]);
+            }
+          }
+      load_v(i + KT);
+    }
+    // ---- the segment's end ----------------------------------------------------------------
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      lsum[n] += __shfl_xor_sync(0xffffffffu, lsum[n], 1);
+      lsum[n] += __shfl_xor_sync(0xffffffffu, lsum[n], 2);
+    }
+    const bool first = p0 == 0, last = p0 + cnt == np;
+    if (first && last) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int hd = 8 * n + 2 * t4 + j;
+          const float l = __shfl_sync(0xffffffffu, lsum[n], 8 * t4 + 4 * j);
+          if (hd >= a.group) continue;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          uint32_t o[MT];
+#pragma unroll
+          for (int q = 0; q < MT; ++q) o[q] = pack_bf16(acc[n][q][j] * inv, acc[n][q][j + 2] * inv);
+          uint4* dst = reinterpret_cast<uint4*>(a.out + t * a.o_st + static_cast<long long>(h * a.group + hd) * a.o_sh + (D / 8) * g);
+#pragma unroll
+          for (int q = 0; q < MT / 4; ++q) dst[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+    } else {
+      const int slot = first ? 1 : 0;
+      float* st = sm.state[warp][slot];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int hd = 8 * n + 2 * t4 + j;
+          float4* dst = reinterpret_cast<float4*>(st + hd * D + (D / 8) * g);
+#pragma unroll
+          for (int q = 0; q < MT / 2; ++q)
+            dst[q] = make_float4(acc[n][2 * q][j], acc[n][2 * q][j + 2], acc[n][2 * q + 1][j], acc[n][2 * q + 1][j + 2]);
+        }
+      if (t4 == 0)
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          st[Tr::kRows * D + 8 * n + g] = ref[n];
+          st[Tr::kRows * D + Tr::kRows + 8 * n + g] = lsum[n];
+        }
+      if (lane == 0) sm.piece[warp][slot] = Piece{tok * a.KVH + h, first, last};
+    }
+    u += cnt;
+  }
+  __syncthreads();
+
+  // ---- rows cut by warp boundaries --------------------------------------------------------
+  // Pieces stand in unit order: slot 0 (goes on from the warp before), then slot 1 (begins here).
+  // Several groups of kRows * D / 4 threads each take a row at a time.
+  constexpr int GT = Tr::kRows * D / 4;         // threads that hold a state as float4
+  constexpr int NGR = NT >= GT ? NT / GT : 1;   // groups
+  constexpr int ER = GT > NT ? GT / NT : 1;     // float4 per thread where a state is larger
+  const int grp = tid / GT;
+  auto write_row = [&](int row, int e, const float4& o, float l) {
+    const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
+    if (hd >= a.group) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long long t = P.t0 + row / a.KVH;
+    *reinterpret_cast<uint2*>(a.out + t * a.o_st + static_cast<long long>((row % a.KVH) * a.group + hd) * a.o_sh + d) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  };
+  static_assert(2 * NW <= 32, "a warp's lanes hold the pieces");
+  Piece mine{-1, 0, 0};
+  if (lane < 2 * NW) mine = sm.piece[lane >> 1][lane & 1];
+  const unsigned valid = __ballot_sync(0xffffffffu, mine.row >= 0);
+  const unsigned firsts = __ballot_sync(0xffffffffu, mine.row >= 0 && mine.first);
+  const unsigned lasts = __ballot_sync(0xffffffffu, mine.row >= 0 && mine.last);
+  int open_row[2] = {-1, -1};  // rows that other CTAs share (0: begun earlier, 1: begun here)
+  int idx = 0;
+  for (unsigned todo = firsts | (valid & (0u - valid)); todo; todo &= todo - 1, ++idx) {
+    const int i = __ffs(todo) - 1;
+    // Its pieces: this one and the slots 0 of the following warps, up to the row's last.
+    const unsigned from = ~0u << i, fin = lasts & from;
+    const unsigned span = valid & from & (fin ? (fin & (0u - fin)) * 2 - 1 : ~0u);
+    const int n = __popc(span), row = __shfl_sync(0xffffffffu, mine.row, i);
+    const bool begins = firsts >> i & 1, whole = begins && fin;
+    if (!whole) open_row[begins ? 1 : 0] = row;
+    if (idx % NGR != grp) continue;
+    for (int r = 0; r < ER; ++r) {
+      const int e = (tid % GT) + r * NT, head = e / (D / 4);
+      auto state_of = [&](int k) { return sm.state[(i >> 1) + k][k == 0 ? (i & 1) : 0]; };
+      float rr = -CUDART_INF_F, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < n; ++k) rr = fmaxf(rr, state_of(k)[Tr::kRows * D + head]);
+      const float base = rr == -CUDART_INF_F ? 0.f : rr;
+      for (int k = 0; k < n; ++k) {
+        const float* s = state_of(k);
+        const float w = ex2(s[Tr::kRows * D + head] - base);
+        const float4 v = reinterpret_cast<const float4*>(s)[e];
+        o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+        l += s[Tr::kRows * D + Tr::kRows + head] * w;
+      }
+      if (whole) {
+        write_row(row, e, o, l);
+      } else {
+        float* dst = P.part + (2ll * blockIdx.x + (begins ? 1 : 0)) * Tr::kState;
+        __stcg(reinterpret_cast<float4*>(dst) + e, o);
+        if (e % (D / 4) == 0) {
+          __stcg(dst + Tr::kRows * D + head, rr);
+          __stcg(dst + Tr::kRows * D + Tr::kRows + head, l);
+        }
+      }
+    }
+  }
+
+  // ---- rows cut by CTA boundaries ---------------------------------------------------------
+  for (int s = 0; s < 2; ++s) {
+    const int row = open_row[s];
+    if (row < 0) continue;  // uniform: every thread walked the same pieces
+    const int tk = row / a.KVH, h = row % a.KVH;
+    const int np = (sm.len[tk] + kPage - 1) / kPage;
+    const int first_unit = sm.pre[tk] + h * np;
+    const int cf = first_unit / chunk, parts = (first_unit + np - 1) / chunk - cf + 1;
+    __syncthreads();  // the CTA's partial state is written
+    if (tid == 0) sm.arrived = static_cast<int>(atom_add_acq_rel_gpu_u32(P.counter + cf, 1u));
+    __syncthreads();
+    if (sm.arrived != parts - 1) continue;
+    if (tid == 0) P.counter[cf] = 0;
+    fence_acq_rel_gpu();
+    if (NGR == 1 || grp == 0) {
+      for (int r = 0; r < ER; ++r) {
+        const int e = (tid % GT) + r * NT;
+        float4 o;
+        float rr, l;
+        fold<D, NG>([&](int k) { return P.part + (2ll * (cf + k) + (k == 0 ? 1 : 0)) * Tr::kState; },
+                    parts, e, o, rr, l);
+        write_row(row, e, o, l);
+      }
+    }
+  }
+}
+
+int decode_sms(int device) {
+  static std::mutex mu;
+  static int cache[64] = {0};
+  if (device < 0 || device >= 64) return 148;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache[device] == 0 &&
+      cudaDeviceGetAttribute(&cache[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    cache[device] = 148;
+  return std::min(cache[device], kMaxCtas);
+}
+
+template <int D, int FMT, int NG>
+cudaError_t launch_one(const DecParams& p, int grid, cudaStream_t stream) {
+  using Tr = DecTraits<D, NG>;
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&] {
+    err[dev] = cudaFuncSetAttribute(q8_decode_kernel<D, FMT, NG>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(sizeof(DecSmem<D, NG>)));
+  });
+  if (err[dev] != cudaSuccess) return err[dev];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(Tr::kThreads);
+  cfg.dynamicSmemBytes = sizeof(DecSmem<D, NG>);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, q8_decode_kernel<D, FMT, NG>, p);
+}
+
+}  // namespace
+
+size_t q8_decode_workspace(int device) {
+  return kWsHeader + kCounterBytes +
+         2 * static_cast<size_t>(decode_sms(device)) * DecTraits<128, 2>::kState * sizeof(float);
+}
+
+bool q8_decode_supported(const Q8AttnArgs& g) {
+  const AttnArgs& a = g.a;
+  const Q8Pool& p = g.p;
+  auto codes16 = [](const void* base, long long sn, long long ss, long long sh, long long sd) {
+    return sd == 1 && sn % 16 == 0 && ss % 16 == 0 && sh % 16 == 0 &&
+           (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  };
+  auto rows16 = [](const void* base, long long st, long long sh, long long sd) {
+    return sd == 1 && st % 8 == 0 && sh % 8 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  };
+  return a.group <= 16 && codes16(p.k, p.k_sn, p.k_ss, p.k_sh, p.k_sd) &&
+         codes16(p.v, p.v_sn, p.v_ss, p.v_sh, p.v_sd) && rows16(a.q, a.q_st, a.q_sh, a.q_sd) &&
+         rows16(a.out, a.o_st, a.o_sh, a.o_sd);
+}
+
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, int min_run, int device, void* workspace,
+                             cudaStream_t stream, int* launches) {
+  DecParams p;
+  p.g = g;
+  p.min_run = min_run;
+  p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
+  const int sms = decode_sms(device);
+  // Tokens per launch: the row lists' room, and units that fit 31 bits.
+  const long long per_token = g.a.W * g.a.KVH;
+  const long long most = std::max<long long>(1, std::min<long long>(kMaxTok, 0x7fffffffLL / per_token));
+  *launches = 0;
+  for (long long t0 = 0; t0 < g.a.T; t0 += most) {
+    p.t0 = static_cast<int>(t0);
+    p.tn = static_cast<int>(std::min(most, g.a.T - t0));
+    const bool wide = g.a.group > 8;
+    p.min_chunk = wide ? 8 : 16;
+    // No more CTAs than the table could fill (the lengths are on the device).
+    const long long bound = std::max<long long>(1, (per_token * p.tn + p.min_chunk - 1) / p.min_chunk);
+    const int grid = static_cast<int>(std::min<long long>(sms, bound));
+    cudaError_t e;
+#define SS_Q8_DECODE(D, NG)                                                    \
+  e = g.p.fmt == SS_CODE_INT8 ? launch_one<D, SS_CODE_INT8, NG>(p, grid, stream) \
+                              : launch_one<D, SS_CODE_E4M3, NG>(p, grid, stream)
+    if (g.p.D == 128) {
+      if (wide) SS_Q8_DECODE(128, 2); else SS_Q8_DECODE(128, 1);
+    } else {
+      if (wide) SS_Q8_DECODE(64, 2); else SS_Q8_DECODE(64, 1);
+    }
+#undef SS_Q8_DECODE
+    if (e != cudaSuccess) return e;
+    ++*launches;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace ss
