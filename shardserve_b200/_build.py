@@ -20,8 +20,9 @@ LIB_NAME = "libshardserve_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["capi.cu", "decode_attention.cu", "generic_attention.cu", "kv_append.cu", "noalloc.cu",
            "prefill_attention.cu", "rope_append.cu", "metadata.cu", "tp2_oproj.cu",
-           "block_tables.cu", "q8_append.cu", "q8_capi.cu", "q8_decode.cu", "q8_generic.cu"]
-HEADERS = ["attention.cuh", "ptx.cuh", "q8.cuh"]
+           "block_tables.cu", "q8_append.cu", "q8_capi.cu", "q8_decode.cu", "q8_generic.cu",
+           "q8_prefill.cu"]
+HEADERS = ["attention.cuh", "exp2.cuh", "ptx.cuh", "q8.cuh", "q8_widen.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

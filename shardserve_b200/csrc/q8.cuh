@@ -117,6 +117,17 @@ size_t q8_decode_workspace(int device);
 bool q8_decode_supported(const Q8AttnArgs& g);
 cudaError_t launch_q8_decode(const Q8AttnArgs& g, int min_run, int device, void* workspace,
                              cudaStream_t stream, int* launches);
+// tcgen05 tiles of prompt chunks (q8_prefill.cu), for runs of at least kQ8MinRun tokens: workspace
+// bytes of the cut windows' states, the layouts it takes, tokens per launch, and the launches of
+// the tiles and of the join of the cut windows.
+constexpr int kQ8MinRun = 4;
+size_t q8_prefill_workspace(int device);
+bool q8_prefill_supported(const Q8AttnArgs& g, int device);
+int q8_prefill_window();
+cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
+                              void* workspace, void* states, cudaStream_t stream);
+cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* workspace, void* states,
+                            cudaStream_t stream);
 cudaError_t launch_block_tables(const BlockTablesArgs& a, cudaStream_t stream);
 int block_tables_max_rows();
 

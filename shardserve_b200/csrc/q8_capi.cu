@@ -115,7 +115,7 @@ int ss_q8_workspace_bytes(int device, int heads, int kv_heads, int head_dim, siz
   if (head_dim != 64 && head_dim != 128) return invalid("head_dim must be 64 or 128");
   if (heads < 1 || kv_heads < 1 || heads % kv_heads)
     return invalid("query heads must be divisible by KV heads");
-  *bytes = ss::q8_decode_workspace(device);
+  *bytes = ss::q8_decode_workspace(device) + ss::q8_prefill_workspace(device);
   return SS_OK;
 }
 
@@ -149,7 +149,7 @@ int ss_ragged_paged_attention_q8(
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return cuda_failed(e, "cudaGetDevice");
-  const size_t need = ss::q8_decode_workspace(device);
+  const size_t need = ss::q8_decode_workspace(device) + ss::q8_prefill_workspace(device);
   if (workspace_bytes < need) {
     ss::set_error_message("a workspace of at least %zu bytes is required", need);
     return SS_ERR_WORKSPACE;
@@ -172,11 +172,23 @@ int ss_ragged_paged_attention_q8(
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.err = static_cast<unsigned*>(workspace);
   if (ss::q8_decode_supported(g)) {
+    // A batch with more tokens than rows holds a prompt chunk.  (Block counts of the tiles fit
+    // 31 bits for tables of up to 2^20 columns.)
+    const bool tiles = tokens > bt_rows && bt_cols <= (1 << 20) && ss::q8_prefill_supported(g, device);
+    void* states = static_cast<uint8_t*>(workspace) + ss::q8_decode_workspace(device);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    for (int64_t t0 = 0; tiles && t0 < tokens; t0 += ss::q8_prefill_window()) {
+      const int64_t tn = tokens - t0 < ss::q8_prefill_window() ? tokens - t0 : ss::q8_prefill_window();
+      e = ss::launch_q8_prefill(g, t0, tn, device, workspace, states, s);
+      if (e == cudaSuccess) e = ss::launch_q8_merge(g, device, workspace, states, s);
+      if (e != cudaSuccess) return cuda_failed(e, "q8 tile attention launch");
+      ss::count_launches(2);
+    }
     int launches = 0;
-    e = ss::launch_q8_decode(g, 0, device, workspace, static_cast<cudaStream_t>(stream), &launches);
+    e = ss::launch_q8_decode(g, tiles ? ss::kQ8MinRun : 0, device, workspace, s, &launches);
     ss::count_launches(static_cast<unsigned>(launches));
     if (e != cudaSuccess) return cuda_failed(e, "q8 split-K attention launch");
-    ss::set_last_path(5);
+    ss::set_last_path(tiles ? 7 : 5);
     return SS_OK;
   }
   e = ss::launch_q8_generic(g, static_cast<cudaStream_t>(stream));

@@ -1,0 +1,904 @@
+// Prompt chunks over the 8-bit pool as tcgen05 tiles.
+//
+// Tokens of runs of at least kQ8MinRun consecutive query tokens of one sequence are computed here,
+// all others by the split-K kernel (q8_decode.cu).  The mathematics is that kernel's:
+//   x_ij = (q_i . Kc_j) * ks_page * sm_scale * log2 e + log2(vs_page),   w_ij = 2^(x_ij - r_i)
+//   O_i  = sum_j w_ij Vc_j,   l_i = sum_j w_ij / vs_page,   out_i = O_i / l_i
+// K codes and q (its row's power of two taken out) are fp16, which holds both exactly; the weights
+// and the V codes are tf32: fp16 has the bits but not the range (weights 2^30 below the row's
+// largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.  So
+// Q.K costs 512 and P.V 1024 tensor cycles per 128 x 128 x 128, and the tensor floor of a tile pair
+// and key block is 3072 cycles.
+//
+// A window is up to 2 * (128 / group) tokens of one run: two tiles of 128 rows (token, query head
+// of the KV head) that share every K / V block.  A work item is (window, KV head, range of
+// 128-key blocks).  Per block j, tile t:
+//   S_t = Q_t K_j^T      kind::f16, A, B in shared memory, fp32 in TMEM columns [128 t, +128)
+//   softmax              one thread per row; P overwrites S_t in TMEM; O_t is rescaled only when a
+//                        weight would pass 2^20
+//   O_t += P_t V_j       kind::tf32, A = P_t from TMEM, B = V_j^T in shared memory
+// in the order S_0(j+1), O_1(j), S_1(j+1), O_0(j+1): each softmax has two products' time.
+// The codes are widened by three producer warps on their way into shared memory: 16 codes per
+// 16-byte load, K rows to 128-byte swizzled fp16 lines, V transposed (lane = key) to lines of 32
+// keys in fp32, 64 keys at a time; loads run one half-block ahead in registers.
+//
+// Scheduling.  Every CTA lists the launch's windows (a scan over its tokens), and cuts a window's
+// blocks into equal parts of at most max(4, all blocks / CTAs): a lone long prompt would otherwise
+// leave most SMs waiting for the last window.  Parts are taken from a counter, cut windows first,
+// then whole ones by length.  Cut windows leave fp32 states in the workspace, joined by
+// q8_merge_kernel.
+//
+// Warps: 0 MMA issuer, 1-3 producers, 4-7 softmax of tile 0, 8-11 of tile 1 (TMEM lane quadrant =
+// warp % 4).  setmaxnreg: 384 x 168 = 64,512 at launch = 128 x 88 + 256 x 208.
+#include <cuda_bf16.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include "exp2.cuh"
+#include "ptx.cuh"
+#include "q8.cuh"
+#include "q8_widen.cuh"
+
+namespace ss {
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kLaunchRegs = 168, kRegsProducer = 88, kRegsSoftmax = 208;
+static_assert(128 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs,
+              "setmaxnreg split exceeds the launch register pool");
+constexpr int kRows = 128;         // rows of a tile
+constexpr int kNB = 128;           // keys of a block
+constexpr int kPages = kNB / kPage;
+constexpr int kMaxTokP = 8192;     // tokens per launch
+constexpr int kMaxWin = kMaxTokP / kQ8MinRun;  // windows per launch
+constexpr int kBins = 256;
+constexpr int kMinPart = 4;        // blocks: smallest cut
+constexpr float kSlackP = 20.f;
+constexpr int kPolyEvery = 3;      // one exponential pair in 3 on the FMA pipe
+constexpr int kSched = 16;         // workspace words: next part, CTAs done, cut windows
+
+template <int D>
+struct Lay {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kQ = kHalves * kRows * 128;   // Q tile, fp16
+  static constexpr int kK = kHalves * kNB * 128;     // K block, fp16
+  static constexpr int kV = 2 * D * 128;             // V^T of 64 keys, fp32: 2 atoms of 32 keys
+  static constexpr int kOffK = 2 * kQ;
+  static constexpr int kOffV = kOffK + 2 * kK;
+  static constexpr int kOffCtl = kOffV + 2 * kV;
+};
+
+enum : int { kBarQ = 0, kBarS = 2, kBarPH = 4, kBarP = 6, kBarPV = 8, kBarKF = 10, kBarKE = 12,
+             kBarVF = 14, kBarVE = 16, kBarEnd = 18, kNumBars = 19 };
+
+struct CtlQ {
+  unsigned long long bar[kNumBars];
+  float4 sc[4][kPages];   // per block (mod 4) and page: K scale, log2 and reciprocal of V's
+  uint32_t tmem;
+  int item[2];
+  int abort;
+  int nwin, total;        // windows; parts * KV heads
+  int red[2][12];
+  unsigned short first[kMaxWin], count[kMaxWin], parts[kMaxWin], order[kMaxWin];
+  int cum[kMaxWin + 1];   // work items before each rank
+  int keys[kMaxWin];
+  int hist[kBins];
+};
+
+struct PrefillParams {
+  Q8AttnArgs g;
+  int t0, tn;
+  int tpt;            // tokens per tile
+  unsigned* sched;    // workspace words kSched ..
+  float* part;        // states of cut windows
+  int4* cuts;         // {first token, tokens, parts, first slot} of each cut window
+};
+
+template <int D>
+struct State {  // a cut window's state: O as [D / 4][256 rows] float4, then r and l of 256 rows
+  static constexpr int kFloats = 256 * D + 512;
+};
+
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ void tc_mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+constexpr uint32_t idesc_of(int fmt, int N) {  // fp32 accumulators, M = 128, both K-major
+  return (1u << 4) | (static_cast<uint32_t>(fmt) << 7) | (static_cast<uint32_t>(fmt) << 10) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (128u >> 4 << 24);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t a) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
+}
+
+// Sum and (exclusive) maximum scans over the CTA.
+__device__ __forceinline__ int scan_sum(int v, int* red, int warp, int lane, int& total) {
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += red[w];
+    total += red[w];
+  }
+  return before + inc - v;
+}
+__device__ __forceinline__ int scan_max(int v, int* red, int warp, int lane) {
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc = max(inc, x);
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  int before = -1;
+  for (int w = 0; w < warp; ++w) before = max(before, red[w]);
+  const int up = __shfl_up_sync(0xffffffffu, inc, 1);
+  return lane == 0 ? before : max(before, up);
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kThreads, 1)
+    q8_prefill_kernel(const __grid_constant__ PrefillParams P) {
+  using L = Lay<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sb = smem_u32(smem);
+  CtlQ* ctl = reinterpret_cast<CtlQ*>(smem + L::kOffCtl);
+  const uint32_t bars = smem_u32(ctl->bar);
+  auto bar = [&](int i) { return bars + 8 * i; };
+  const AttnArgs& a = P.g.a;
+  const Q8Pool& pool = P.g.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tw = 2 * P.tpt;  // tokens of a window
+
+  if (tid == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar(kBarQ + t), 128);
+      mbar_init(bar(kBarS + t), 1);
+      mbar_init(bar(kBarPH + t), 128);
+      mbar_init(bar(kBarP + t), 128);
+      mbar_init(bar(kBarPV + t), 1);
+      mbar_init(bar(kBarKF + t), 3);
+      mbar_init(bar(kBarKE + t), 1);
+      mbar_init(bar(kBarVF + t), 3);
+      mbar_init(bar(kBarVE + t), 1);
+    }
+    mbar_init(bar(kBarEnd), 1);
+    fence_mbar_init();
+    ctl->abort = 0;
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&ctl->tmem), 512);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  const int first_item = tid == 0 ? static_cast<int>(atomicAdd(P.sched, 1u)) : 0;
+
+  // ---- the windows of this launch ----------------------------------------------------------
+  for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) ctl->hist[i] = 0;
+  {
+    const int per = (P.tn + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
+    auto seq_of = [&](int i) { return ld_index(a.seq, a.seq64, P.t0 + i); };
+    auto in_run = [&](int i) { return token_in_long_run(a, kQ8MinRun, P.t0 + i, seq_of(i)); };
+    auto starts = [&](int i) { return i == 0 || seq_of(i - 1) != seq_of(i); };
+    int start = -1;  // last run start at or before a token
+    for (int i = b0; i < b1; ++i)
+      if (starts(i)) start = i;
+    const int before = scan_max(start, ctl->red[0], warp, lane);
+    start = before;
+    int n = 0;
+    for (int i = b0; i < b1; ++i) {
+      if (starts(i)) start = i;
+      if ((i - start) % tw == 0 && in_run(i)) ++n;
+    }
+    int nwin;
+    int idx = scan_sum(n, ctl->red[1], warp, lane, nwin) - 1;
+    start = before;
+    for (int i = b0; i < b1; ++i) {
+      if (starts(i)) start = i;
+      if (!in_run(i)) continue;
+      const int at = (i - start) % tw;
+      if (at == 0) ctl->first[++idx] = static_cast<unsigned short>(i);
+      if (at == tw - 1 || i + 1 == P.tn || starts(i + 1))
+        ctl->count[idx] = static_cast<unsigned short>(at + 1);
+      const TokInfo ti = q8_token_info(a, P.t0 + i, blockIdx.x == 0);
+      atomicMax(&ctl->keys[idx], ti.L);
+    }
+    __syncthreads();
+    // Blocks of every window; the largest part, and the order in which parts are taken.
+    int sum = 0;
+    for (int w = tid; w < nwin; w += kThreads) sum += (ctl->keys[w] + kNB - 1) / kNB;
+    int all;
+    scan_sum(sum, ctl->red[0], warp, lane, all);
+    const long long each = (static_cast<long long>(all) * a.KVH + gridDim.x - 1) / gridDim.x;
+    const int most = static_cast<int>(max(each, static_cast<long long>(kMinPart)));
+    auto bin_of = [&](int w) {  // 0 first: cut windows, then whole ones from long to short
+      const int nb = (ctl->keys[w] + kNB - 1) / kNB;
+      return nb > most ? 0 : kBins - 1 - min(nb, kBins - 2);
+    };
+    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&ctl->hist[bin_of(w)], 1);
+    __syncthreads();
+    if (warp == 0) {
+      int local = 0;
+#pragma unroll
+      for (int i = 0; i < kBins / 32; ++i) local += ctl->hist[lane * (kBins / 32) + i];
+      int inc = local;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      int run = inc - local;
+#pragma unroll
+      for (int i = 0; i < kBins / 32; ++i) {
+        const int b = lane * (kBins / 32) + i, h = ctl->hist[b];
+        ctl->hist[b] = run;
+        run += h;
+      }
+      __syncwarp();
+      for (int base = 0; base < nwin; base += 32) {  // stable: every CTA builds the same order
+        const int w = base + lane;
+        const int b = w < nwin ? bin_of(w) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, b);
+        if (w < nwin) ctl->order[ctl->hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
+        __syncwarp();
+        if (w < nwin && lane == __ffs(same) - 1) ctl->hist[b] += __popc(same);
+        __syncwarp();
+      }
+      // Work items before each rank; parts are equal shares of at most `most` blocks.
+      int carry = 0, cuts = 0;
+      for (int base = 0; base < nwin; base += 32) {
+        const int r = base + lane;
+        int parts = 0, w = 0;
+        if (r < nwin) {
+          w = ctl->order[r];
+          const int nb = (ctl->keys[w] + kNB - 1) / kNB;
+          parts = nb > most ? (nb + most - 1) / most : 1;
+          ctl->parts[w] = static_cast<unsigned short>(parts);
+        }
+        int inc2 = parts * a.KVH;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, inc2, o);
+          if (lane >= o) inc2 += x;
+        }
+        if (r < nwin) ctl->cum[r] = carry + inc2 - parts * a.KVH;
+        if (blockIdx.x == 0 && parts > 1)
+          P.cuts[r] = make_int4(P.t0 + ctl->first[w], ctl->count[w], parts, carry + inc2 - parts * a.KVH);
+        cuts += __popc(__ballot_sync(0xffffffffu, parts > 1));
+        carry += __shfl_sync(0xffffffffu, inc2, 31);
+      }
+      if (lane == 0) {
+        ctl->cum[nwin] = carry;
+        ctl->nwin = nwin;
+        ctl->total = carry;
+        if (blockIdx.x == 0) P.sched[2] = static_cast<unsigned>(cuts);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  const int nwin = ctl->nwin, total = ctl->total;
+
+  int jg = 0;      // blocks processed so far by this CTA (phases of the K and V barriers)
+  // Phases of a tile's own barriers: tile 1 sits out windows that fill one tile only.
+  int jt[2] = {0, 0}, qt[2] = {0, 0};  // blocks and windows of each tile so far
+  bool ok = true;
+  int iter = 0;
+  struct Item {
+    bool live;
+    int first, count, kvh, j0, j1, keys, slot;  // slot < 0: the window is whole
+    long long seq;
+  };
+  auto next_item = [&]() -> Item {
+    if (tid == 0) ctl->item[iter & 1] = iter == 0 ? first_item : static_cast<int>(atomicAdd(P.sched, 1u));
+    named_bar_sync(1, kThreads);
+    const int w = ctl->item[iter & 1];
+    ++iter;
+    Item it;
+    it.live = w < total && !ctl->abort;
+    if (!it.live) return it;
+    int lo = 0, hi = nwin;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (ctl->cum[mid] <= w) lo = mid; else hi = mid;
+    }
+    const int win = ctl->order[lo], rest = w - ctl->cum[lo], parts = ctl->parts[win];
+    it.first = ctl->first[win];
+    it.count = ctl->count[win];
+    it.keys = ctl->keys[win];
+    it.kvh = rest / parts;
+    const int p = rest - it.kvh * parts, nb = (it.keys + kNB - 1) / kNB;
+    it.j0 = static_cast<int>(static_cast<long long>(nb) * p / parts);
+    it.j1 = static_cast<int>(static_cast<long long>(nb) * (p + 1) / parts);
+    it.slot = parts > 1 ? w : -1;
+    it.seq = ld_index(a.seq, a.seq64, P.t0 + it.first);
+    return it;
+  };
+  auto timed_out = [&]() {
+    if (lane == 0) {
+      atomicOr(a.err, SS_DEVERR_TIMEOUT);
+      ctl->abort = 1;
+    }
+  };
+
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsProducer>();
+    if (warp == 0) {
+      // ================================= MMA issuer ====================================
+      constexpr uint32_t id_qk = idesc_of(0, kNB), id_pv = idesc_of(2, D);
+      const bool leader = elect_one();
+      for (;;) {
+        const Item it = next_item();
+        if (!it.live) break;
+        const int nblk = it.j1 - it.j0;
+        const bool two = it.count > P.tpt;  // both tiles hold tokens
+        auto qk = [&](int t, int st) {
+          if (leader) {
+            const uint64_t qd = smem_desc_sw128(sb + t * L::kQ, 16, 1024);
+            const uint64_t kd = smem_desc_sw128(sb + L::kOffK + st * L::kK, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
+              tc_mma_f16(tmem + t * kNB, qd + off, kd + off, id_qk, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(bar(kBarS + t));
+          }
+          __syncwarp();
+        };
+        auto pv = [&](int t, int j, bool release) -> bool {  // block j of this item
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait_warp(bar(kBarVF + half), (jg + j) & 1)) return false;
+            if (!wait_warp(bar((half ? kBarP : kBarPH) + t), (jt[t] + j) & 1)) return false;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t vd = smem_desc_sw128(sb + L::kOffV + half * L::kV, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                tc_mma_tf32_ts(tmem + 256 + t * 128, tmem + t * kNB + half * 64 + kk * 8,
+                               vd + (((kk >> 2) * (D * 128) + (kk & 3) * 32) >> 4), id_pv,
+                               (j > 0 || half > 0 || kk > 0) ? 1u : 0u);
+              if (release) tc_commit(bar(kBarVE + half));
+            }
+            __syncwarp();
+          }
+          if (leader) tc_commit(bar(kBarPV + t));
+          __syncwarp();
+          return true;
+        };
+        if (nblk > 0) {
+          ok = wait_warp(bar(kBarQ), qt[0] & 1);
+          if (ok && two) ok = wait_warp(bar(kBarQ + 1), qt[1] & 1);
+          for (int j = 0; j < nblk && ok; ++j) {
+            const int jb = jg + j, st = jb & 1;
+            ok = wait_warp(bar(kBarKF + st), (jb >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            qk(0, st);
+            if (two) {
+              if (j > 0 && !(ok = pv(1, j - 1, true))) break;
+              qk(1, st);
+            }
+            if (leader) tc_commit(bar(kBarKE + st));
+            __syncwarp();
+            ok = pv(0, j, !two);
+          }
+          if (ok && two) ok = pv(1, nblk - 1, true);
+          if (!ok) timed_out();
+          jg += nblk;
+          jt[0] += nblk;
+          ++qt[0];
+          if (two) {
+            jt[1] += nblk;
+            ++qt[1];
+          }
+        }
+        tc_fence_before();
+      }
+      if (leader) tc_commit(bar(kBarEnd));  // every product issued has completed before TMEM is freed
+      __syncwarp();
+      if (!wait_warp(bar(kBarEnd), 0)) timed_out();
+    } else {
+      // ================================== producers ====================================
+      const int pw = warp - 1;
+      for (;;) {
+        const Item it = next_item();
+        if (!it.live) break;
+        const int nblk = it.j1 - it.j0;
+        if (nblk <= 0) continue;
+        const uint8_t* kbase = pool.k + static_cast<long long>(it.kvh) * pool.k_sh;
+        const uint8_t* vbase = pool.v + static_cast<long long>(it.kvh) * pool.v_sh;
+        const float* sbase = pool.scales + static_cast<long long>(it.kvh) * pool.s_sh;
+        // Page ids and scales of a block: lanes 0-7.  id -1: past the keys or outside the pool.
+        auto load_id = [&](int j) -> int {
+          const int pi = (it.j0 + j) * kPages + lane;
+          if (j >= nblk || lane >= kPages || pi * kPage >= it.keys) return -1;
+          const long long id = ld_index(a.bt, a.bt64, it.seq * a.bt_sb + pi * a.bt_sn);
+          if (id >= 0 && id < pool.N) return static_cast<int>(id);
+          atomicOr(a.err, SS_DEVERR_PAGE);
+          return -1;
+        };
+        auto load_scale = [&](int id) -> float2 {
+          if (id < 0) return make_float2(0.f, 1.f);
+          const float* s = sbase + id * pool.s_sn;
+          return make_float2(__ldg(s), __ldg(s + pool.s_sw));
+        };
+        constexpr int kIts = 8 * L::kHalves;       // 16-byte loads of a half-block per lane group
+        constexpr int kMine = (kIts + 2) / 3;
+        uint4 buf[kMine];
+        // K: iteration i covers 8 keys x 64 values (lane = chunk * 8 + key).
+        // V: iteration i covers 32 keys x 16 values (lane = key; the upper lanes take the
+        // neighbouring chunk, so that both halves of a sector are read together).
+        auto load_one = [&](int n, bool is_v, int j, int half, int ids, float vscale) -> uint4 {
+          const int i = pw + 3 * n;
+          int key, d;  // key inside the half-block
+          if (is_v) {
+            key = (i & 1) * 32 + lane;
+            d = 16 * ((i >> 1) ^ (lane >> 4));
+          } else {
+            key = (i & 7) * 8 + (lane & 7);
+            d = 64 * (i >> 3) + 16 * (lane >> 3);
+          }
+          const int in_block = half * 64 + key;
+          const int id = __shfl_sync(0xffffffffu, ids, in_block / kPage);
+          const float vs = __shfl_sync(0xffffffffu, vscale, in_block / kPage);
+          if (i >= kIts || id < 0 || (it.j0 + j) * kNB + in_block >= it.keys || (is_v && !(vs >= kMinVs)))
+            return make_uint4(0, 0, 0, 0);
+          const uint8_t* p = is_v ? vbase + id * pool.v_sn + (key % kPage) * pool.v_ss + d
+                                  : kbase + id * pool.k_sn + (key % kPage) * pool.k_ss + d;
+          return __ldg(reinterpret_cast<const uint4*>(p));
+        };
+        auto emit_one = [&](int n, bool is_v, int half, int st, const uint4& v) {
+          const int i = pw + 3 * n;
+          if (i >= kIts) return;
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          if (is_v) {
+            const int key = lane, d0 = 16 * ((i >> 1) ^ (lane >> 4));
+            const uint32_t base = sb + L::kOffV + half * L::kV + (i & 1) * (D * 128) + d0 * 128 + (key & 3) * 4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t f[4];
+              widen_f32<FMT>(w[q], f);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)  // d0 is a multiple of 16: the line's phase is (4 q + e) % 8
+                st_shared4(base + (4 * q + e) * 128 + (((key >> 2) ^ ((4 * q + e) & 7)) << 4), f[e]);
+            }
+          } else {
+            const int key = half * 64 + (i & 7) * 8 + (lane & 7), c = 2 * (lane >> 3);
+            const uint32_t line = sb + L::kOffK + st * L::kK + (i >> 3) * (kNB * 128) + key * 128;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t h[4];
+              widen<FMT>(w[2 * q], h[0], h[1]);
+              widen<FMT>(w[2 * q + 1], h[2], h[3]);
+              st_shared16(line + (((c + q) ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
+            }
+          }
+        };
+        // Order: K(0), then K(j + 1), V(j) for every block j, each in two halves.
+        int id_v = -1, id_k = load_id(0), id_n = load_id(1);
+        float2 sc_v = make_float2(0.f, 1.f), sc_k = load_scale(id_k);
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) buf[n] = load_one(n, false, 0, 0, id_k, sc_k.y);
+        for (int j = -1; j < nblk && ok; ++j) {
+          // On entry buf holds the first half of K(j + 1), or of V(j) for the last block.
+          const int jk = jg + j + 1, stk = jk & 1;
+          const int id_n2 = load_id(j + 3);
+          const float2 sc_n = load_scale(id_n);
+#pragma unroll 1
+          for (int u = (j + 1 < nblk) ? 0 : 2; u < (j >= 0 ? 4 : 2) && ok; ++u) {
+            const bool is_v = u >= 2;
+            const int half = u & 1;
+            // The next half-block, loaded into the registers as this one leaves them.
+            bool nv, more = true;
+            int nj, nh, nid;
+            float nvs;
+            if (u == 0) { nv = false; nj = j + 1; nh = 1; nid = id_k; nvs = sc_k.y; }
+            else if (u == 1 && j >= 0) { nv = true; nj = j; nh = 0; nid = id_v; nvs = sc_v.y; }
+            else if (u == 2) { nv = true; nj = j; nh = 1; nid = id_v; nvs = sc_v.y; }
+            else if (j + 2 < nblk) { nv = false; nj = j + 2; nh = 0; nid = id_n; nvs = sc_n.y; }
+            else { nv = true; nj = j + 1; nh = 0; nid = id_k; nvs = sc_k.y; more = j + 1 < nblk; }
+            if (is_v) {
+              ok = wait_warp(bar(kBarVE + half), ((jg + j) & 1) ^ 1);
+            } else if (half == 0) {
+              ok = wait_warp(bar(kBarKE + stk), ((jk >> 1) & 1) ^ 1);
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) {
+              emit_one(n, is_v, half, stk, buf[n]);
+              if (more) buf[n] = load_one(n, nv, nj, nh, nid, nvs);
+            }
+            if (!is_v && half == 0 && pw == 0 && lane < kPages) {
+              const float vs = fmaxf(sc_k.y, kMinVs);
+              ctl->sc[jk & 3][lane] = make_float4(sc_k.x, lg2(vs), __frcp_rn(vs), 0.f);
+            }
+            if (is_v || half == 1) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(is_v ? kBarVF + half : kBarKF + stk));
+            }
+          }
+          id_v = id_k; sc_v = sc_k;
+          id_k = id_n; sc_k = sc_n;
+          id_n = id_n2;
+        }
+        if (!ok) timed_out();
+        jg += nblk;
+      }
+    }
+  } else {
+    setmaxnreg_inc<kRegsSoftmax>();
+    const int tt = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + tt * kNB + lane_off, tO = tmem + 256 + tt * 128 + lane_off;
+    const int rt = row / a.group, rh = row - rt * a.group;  // token inside the tile, head
+    for (;;) {
+      const Item it = next_item();
+      if (!it.live) break;
+      const int nblk = it.j1 - it.j0;
+      const int wt = tt * P.tpt + rt;  // token inside the window
+      const bool mine = rt < P.tpt && wt < it.count;
+      const long long t = P.t0 + it.first + wt;
+      __nv_bfloat16* op = a.out + t * a.o_st + static_cast<long long>(it.kvh * a.group + rh) * a.o_sh;
+      if (nblk == 0) {  // no row of the window has keys
+        if (mine)
+          for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      const bool active = tt == 0 || it.count > P.tpt;
+      if (active) {
+        const int lim = mine ? q8_token_info(a, t, false).L : INT_MAX;  // others compute unmasked
+        // ---- this row of Q, as fp16 with its power of two taken out ----------------------
+        float f_row;
+        {
+          uint32_t raw[D / 2];
+          const __nv_bfloat16* qp = a.q + t * a.q_st + static_cast<long long>(it.kvh * a.group + rh) * a.q_sh;
+          float amax = 0.f;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (mine) v = __ldg(reinterpret_cast<const uint4*>(qp) + c);
+            raw[4 * c] = v.x; raw[4 * c + 1] = v.y; raw[4 * c + 2] = v.z; raw[4 * c + 3] = v.w;
+          }
+#pragma unroll
+          for (int c = 0; c < D / 2; ++c)
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[c] << 16)),
+                                     fabsf(__uint_as_float(raw[c] & 0xffff0000u))));
+          const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
+          // A negative sm_scale changes q's sign, so that the factor of the scores is >= 0.
+          const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), a.scale_log2);
+          f_row = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(a.scale_log2);
+          const uint32_t line = sb + tt * L::kQ + row * 128;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              h[k] = pack_f16(__uint_as_float(raw[4 * c + k] << 16) * down,
+                              __uint_as_float(raw[4 * c + k] & 0xffff0000u) * down);
+            st_shared16(line + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(bar(kBarQ + tt));
+        }
+        float ref = -CUDART_INF_F, lsum = 0.f;
+        for (int j = 0; j < nblk; ++j) {
+          const int jb = jt[0] + j;  // this tile's blocks so far
+          ok = wait_warp(bar(kBarS + tt), jb & 1);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t sr[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
+          // Page constants.  The factor is kept above 0 so that a masked score stays -inf under
+          // a zero scale.
+          const float4* sc = ctl->sc[(jg + j) & 3];
+          auto factor = [&](const float4& c) { return fmaxf(c.x * f_row, 1e-37f); };
+          tmem_wait_ld();
+          const int nv = lim - (it.j0 + j) * kNB;
+          if (!__all_sync(0xffffffffu, nv >= kNB)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i >= nv) sr[c][i] = __float_as_uint(-CUDART_INF_F);
+          }
+          float top = -CUDART_INF_F;
+#pragma unroll
+          for (int p = 0; p < kPages; ++p) {
+            const uint32_t* s = &sr[p >> 1][(p & 1) * 16];
+            float m = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+#pragma unroll
+            for (int i = 2; i < 16; i += 2) m = max3(m, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            const float4 pc = sc[p];
+            top = fmaxf(top, fmaf(m, factor(pc), pc.y));
+          }
+          const bool raise = top > ref + kSlackP;
+          const float ref_new = raise ? top : ref;
+          const float alpha = raise ? ex2(ref - ref_new) : 1.f;
+          if (j > 0 && __any_sync(0xffffffffu, raise)) {
+            ok = wait_warp(bar(kBarPV + tt), (jb - 1) & 1);  // complete: S_t(j) was issued after it
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
+          ref = ref_new;
+          const float base = ref == -CUDART_INF_F ? 0.f : ref;
+          float part = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int p = 2 * c + h;
+              const float4 pc = sc[p];
+              const float f = factor(pc), b = pc.y - base;
+              const uint64_t f2 = f2pack(f, f), b2 = f2pack(b, b);
+              uint64_t acc[2] = {0, 0};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                uint32_t& s0 = sr[c][h * 16 + 2 * i];
+                uint32_t& s1 = sr[c][h * 16 + 2 * i + 1];
+                const uint64_t x2 = fma2(f2pack(__uint_as_float(s0), __uint_as_float(s1)), f2, b2);
+                uint64_t w2;
+                if ((p * 8 + i) % kPolyEvery == kPolyEvery - 1) {
+                  w2 = exp2_poly2(x2);
+                } else {
+                  float x0, x1;
+                  f2unpack(x2, x0, x1);
+                  w2 = f2pack(ex2(x0), ex2(x1));
+                }
+                acc[i & 1] = add2(acc[i & 1], w2);
+                s0 = static_cast<uint32_t>(w2);
+                s1 = static_cast<uint32_t>(w2 >> 32);
+              }
+              float a0, a1;
+              f2unpack(add2(acc[0], acc[1]), a0, a1);
+              part = fmaf(a0 + a1, pc.z, part);
+            }
+            tmem_st32(tS + c * 32, sr[c]);
+            if (c & 1) {
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(bar((c == 1 ? kBarPH : kBarP) + tt));
+            }
+          }
+          lsum = lsum * alpha + part;
+        }
+        // ---- O_t / l, or the state of a cut window ----------------------------------------
+        if (ok) ok = wait_warp(bar(kBarPV + tt), (jt[0] + nblk - 1) & 1);
+        if (ok) {
+          tc_fence_after();
+          // A row whose keys are all masked never got a reference (and its weights are not sums of
+          // exact zeros where the polynomial made them).
+          if (ref == -CUDART_INF_F) lsum = 0.f;
+          const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+          float4* st = reinterpret_cast<float4*>(P.part + static_cast<long long>(it.slot) * State<D>::kFloats) + tt * kRows + row;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+            if (it.slot >= 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                __stcg(st + (c * 8 + i) * 256,
+                       make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+            } else if (mine) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint4 v;
+                v.x = pack_bf16(__uint_as_float(o[q * 8 + 0]) * inv, __uint_as_float(o[q * 8 + 1]) * inv);
+                v.y = pack_bf16(__uint_as_float(o[q * 8 + 2]) * inv, __uint_as_float(o[q * 8 + 3]) * inv);
+                v.z = pack_bf16(__uint_as_float(o[q * 8 + 4]) * inv, __uint_as_float(o[q * 8 + 5]) * inv);
+                v.w = pack_bf16(__uint_as_float(o[q * 8 + 6]) * inv, __uint_as_float(o[q * 8 + 7]) * inv);
+                *reinterpret_cast<uint4*>(op + c * 32 + q * 8) = v;
+              }
+            }
+          }
+          if (it.slot >= 0) {
+            float* rl = P.part + static_cast<long long>(it.slot) * State<D>::kFloats + 256 * D + tt * kRows + row;
+            __stcg(rl, ref);
+            __stcg(rl + 256, lsum);
+          }
+        }
+        if (!ok) timed_out();
+        tc_fence_before();
+        jt[0] += nblk;
+      }
+      jg += nblk;
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0) {  // the last CTA out returns the counters to zero
+    __threadfence();
+    if (atomicAdd(P.sched + 1, 1u) == gridDim.x - 1) {
+      P.sched[0] = 0;
+      P.sched[1] = 0;
+    }
+  }
+}
+
+// Joins the states of cut windows: one thread per (row, 16 values).
+template <int D>
+__global__ void __launch_bounds__(256) q8_merge_kernel(const PrefillParams P) {
+  griddep_wait();
+  const AttnArgs& a = P.g.a;
+  const int cuts = static_cast<int>(P.sched[2]);
+  const int per_win = a.KVH * (D / 16);  // blocks of 256 rows
+  for (int b = blockIdx.x; b < cuts * per_win; b += gridDim.x) {
+    const int4 cut = P.cuts[b / per_win];
+    const int rest = b % per_win, h = rest / (D / 16), c = rest % (D / 16);
+    const int row = threadIdx.x, tile = row / kRows, r = row % kRows;
+    const int rt = r / a.group, rh = r - rt * a.group, wt = tile * P.tpt + rt;
+    if (rt >= P.tpt || wt >= cut.y) continue;
+    const float* s0 = P.part + (static_cast<long long>(cut.w) + h * cut.z) * State<D>::kFloats;
+    float ref = -CUDART_INF_F, l = 0.f;
+    for (int p = 0; p < cut.z; ++p) ref = fmaxf(ref, __ldcg(s0 + p * static_cast<long long>(State<D>::kFloats) + 256 * D + row));
+    const float base = ref == -CUDART_INF_F ? 0.f : ref;
+    float4 o[4] = {};
+    for (int p = 0; p < cut.z; ++p) {
+      const float* s = s0 + p * static_cast<long long>(State<D>::kFloats);
+      const float w = ex2(__ldcg(s + 256 * D + row) - base);
+      l += w * __ldcg(s + 256 * D + 256 + row);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(s) + (c * 4 + k) * 256 + row);
+        o[k].x += w * v.x; o[k].y += w * v.y; o[k].z += w * v.z; o[k].w += w * v.w;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<long long>(cut.x + wt) * a.o_st +
+                                          static_cast<long long>(h * a.group + rh) * a.o_sh + c * 16);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      dst[k] = make_uint4(pack_bf16(o[2 * k].x * inv, o[2 * k].y * inv), pack_bf16(o[2 * k].z * inv, o[2 * k].w * inv),
+                          pack_bf16(o[2 * k + 1].x * inv, o[2 * k + 1].y * inv), pack_bf16(o[2 * k + 1].z * inv, o[2 * k + 1].w * inv));
+  }
+}
+
+int prefill_sms(int device) {
+  static std::mutex mu;
+  static int cache[64] = {0};
+  if (device < 0 || device >= 64) return 148;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache[device] == 0 &&
+      cudaDeviceGetAttribute(&cache[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    cache[device] = 148;
+  return cache[device];
+}
+
+template <int D>
+constexpr size_t prefill_smem() {
+  return Lay<D>::kOffCtl + sizeof(CtlQ) + 1024;
+}
+static_assert(prefill_smem<128>() <= 227 * 1024, "shared memory");
+
+template <int D, int FMT>
+bool prepare_one(int device) {
+  static std::once_flag once[64];
+  static bool fine[64];
+  std::call_once(once[device], [&] {
+    cudaFuncAttributes fa;
+    fine[device] = cudaFuncSetAttribute(q8_prefill_kernel<D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(prefill_smem<D>())) == cudaSuccess &&
+                   cudaFuncGetAttributes(&fa, q8_prefill_kernel<D, FMT>) == cudaSuccess &&
+                   fa.numRegs == kLaunchRegs;  // the setmaxnreg split counts on it
+  });
+  return fine[device];
+}
+
+template <typename... Args>
+cudaError_t launch_chained(void (*kernel)(Args...), int grid, int threads, size_t smem,
+                           cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace
+
+// The states: windows are cut into parts of at least 1 / CTAs of all blocks, and a cut window has
+// less than one part more than its share, so at most 2 * CTAs parts need a state.
+size_t q8_prefill_workspace(int device) {
+  return 2 * static_cast<size_t>(prefill_sms(device)) * State<128>::kFloats * sizeof(float) +
+         sizeof(int4) * kMaxWin;
+}
+
+bool q8_prefill_supported(const Q8AttnArgs& g, int device) {
+  if (device < 0 || device >= 64 || !q8_decode_supported(g)) return false;
+  const bool i8 = g.p.fmt == SS_CODE_INT8;
+  return g.p.D == 128 ? (i8 ? prepare_one<128, SS_CODE_INT8>(device) : prepare_one<128, SS_CODE_E4M3>(device))
+                      : (i8 ? prepare_one<64, SS_CODE_INT8>(device) : prepare_one<64, SS_CODE_E4M3>(device));
+}
+
+cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
+                              void* workspace, void* states, cudaStream_t stream) {
+  PrefillParams p;
+  p.g = g;
+  p.t0 = static_cast<int>(t0);
+  p.tn = static_cast<int>(tn);
+  p.tpt = kRows / g.a.group;
+  p.sched = static_cast<unsigned*>(workspace) + kSched;
+  p.cuts = static_cast<int4*>(states);
+  p.part = reinterpret_cast<float*>(p.cuts + kMaxWin);
+  const int grid = prefill_sms(device);
+  const bool i8 = g.p.fmt == SS_CODE_INT8;
+  if (g.p.D == 128)
+    return i8 ? launch_chained(q8_prefill_kernel<128, SS_CODE_INT8>, grid, kThreads, prefill_smem<128>(), stream, p)
+              : launch_chained(q8_prefill_kernel<128, SS_CODE_E4M3>, grid, kThreads, prefill_smem<128>(), stream, p);
+  return i8 ? launch_chained(q8_prefill_kernel<64, SS_CODE_INT8>, grid, kThreads, prefill_smem<64>(), stream, p)
+            : launch_chained(q8_prefill_kernel<64, SS_CODE_E4M3>, grid, kThreads, prefill_smem<64>(), stream, p);
+}
+
+cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* workspace, void* states,
+                            cudaStream_t stream) {
+  PrefillParams p;
+  p.g = g;
+  p.t0 = p.tn = 0;
+  p.tpt = kRows / g.a.group;
+  p.sched = static_cast<unsigned*>(workspace) + kSched;
+  p.cuts = static_cast<int4*>(states);
+  p.part = reinterpret_cast<float*>(p.cuts + kMaxWin);
+  const int grid = 4 * prefill_sms(device);
+  return g.p.D == 128 ? launch_chained(q8_merge_kernel<128>, grid, 256, 0, stream, p)
+                      : launch_chained(q8_merge_kernel<64>, grid, 256, 0, stream, p);
+}
+
+int q8_prefill_window() { return kMaxTokP; }
+
+}  // namespace ss
