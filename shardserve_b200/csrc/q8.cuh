@@ -108,19 +108,60 @@ __device__ __forceinline__ TokInfo q8_token_info(const AttnArgs& a, long long t,
   return token_info_from(a, seq, ld_index(a.pos, a.pos64, t), report);
 }
 
+// Tokens t0 .. t0 + tn - 1 into shared memory: seq[i] (32 bits of the id; kQ8MinRun - 1 neighbours
+// on either side too) and len[i] (keys).  Both attention kernels tell runs from these.
+constexpr int kQ8MinRun = 8;   // tokens of shorter runs belong to the split-K kernel
+constexpr int kQ8Pad = kQ8MinRun - 1;
+__device__ __forceinline__ void stage_tokens(const AttnArgs& a, long long t0, int tn, int* seq,
+                                             int* len, bool report) {
+  constexpr int U = 8;  // loads in flight: every one is a round trip to L2 or beyond
+  for (int i0 = threadIdx.x; i0 < tn; i0 += U * blockDim.x) {
+    long long s[U], p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * static_cast<int>(blockDim.x), tn - 1);
+      s[u] = ld_index(a.seq, a.seq64, t0 + i);
+      p[u] = ld_index(a.pos, a.pos64, t0 + i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * static_cast<int>(blockDim.x);
+      if (i >= tn) break;
+      seq[i] = static_cast<int>(s[u]);
+      len[i] = s[u] == -1 ? 0 : token_info_from(a, s[u], p[u], report).L;
+    }
+  }
+  for (int k = threadIdx.x; k < 2 * kQ8Pad; k += blockDim.x) {
+    const int i = k < kQ8Pad ? -1 - k : tn + k - kQ8Pad;
+    const long long t = t0 + i;
+    // Past the batch's ends: anything but the id of the token at the end.
+    seq[i] = t >= 0 && t < a.T ? static_cast<int>(ld_index(a.seq, a.seq64, t))
+                               : ~static_cast<int>(ld_index(a.seq, a.seq64, t < 0 ? 0 : a.T - 1));
+  }
+}
+// Token i of staged ids lies in a run of at least kQ8MinRun tokens of one sequence.
+__device__ __forceinline__ bool in_staged_run(const int* seq, int i) {
+  const int s = seq[i];
+  int n = 1;
+#pragma unroll
+  for (int k = 1, on = 1; k <= kQ8Pad; ++k) n += (on = on && seq[i - k] == s);
+#pragma unroll
+  for (int k = 1, on = 1; k <= kQ8Pad; ++k) n += (on = on && seq[i + k] == s);
+  return n >= kQ8MinRun;
+}
+
 cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_generic(const Q8AttnArgs& a, cudaStream_t stream);
 // Split-K kernel (q8_decode.cu): workspace bytes, the layouts it addresses, and the launch
-// (*launches: kernels enqueued).  Tokens of runs of at least min_run tokens are left out (0: none).
+// (*launches: kernels enqueued).  skip_runs: tokens of runs belong to the tiles.
 size_t q8_decode_workspace(int device);
 bool q8_decode_supported(const Q8AttnArgs& g);
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, int min_run, int device, void* workspace,
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, int device, void* workspace,
                              cudaStream_t stream, int* launches);
 // tcgen05 tiles of prompt chunks (q8_prefill.cu), for runs of at least kQ8MinRun tokens: workspace
 // bytes of the cut windows' states, the layouts it takes, tokens per launch, and the launches of
 // the tiles and of the join of the cut windows.
-constexpr int kQ8MinRun = 4;
 size_t q8_prefill_workspace(int device);
 bool q8_prefill_supported(const Q8AttnArgs& g, int device);
 int q8_prefill_window();

@@ -185,7 +185,7 @@ int ss_ragged_paged_attention_q8(
       ss::count_launches(2);
     }
     int launches = 0;
-    e = ss::launch_q8_decode(g, tiles ? ss::kQ8MinRun : 0, device, workspace, s, &launches);
+    e = ss::launch_q8_decode(g, tiles, device, workspace, s, &launches);
     ss::count_launches(static_cast<unsigned>(launches));
     if (e != cudaSuccess) return cuda_failed(e, "q8 split-K attention launch");
     ss::set_last_path(tiles ? 7 : 5);

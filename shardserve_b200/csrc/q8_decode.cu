@@ -109,7 +109,7 @@ __device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
 struct DecParams {
   Q8AttnArgs g;
   int t0, tn;          // tokens of this launch
-  int min_run;         // tokens of runs at least this long belong to the tile kernel (0: none)
+  int skip_runs;       // tokens of runs belong to the tile kernel
   int min_chunk;       // fewest units of a CTA
   unsigned* counter;   // [kMaxCtas], zero between calls
   float* part;         // [2 * grid] partial states
@@ -162,7 +162,7 @@ struct DecSmem {
   alignas(16) float state[Tr::kWarps][2][Tr::kState];
   Piece piece[Tr::kWarps][2];
   int pre[kMaxTok + 1];  // units before each token
-  int seq[kMaxTok];
+  int seq[kMaxTok + 2 * kQ8Pad];
   int len[kMaxTok];
   int scan[Tr::kWarps];
   int arrived;
@@ -182,18 +182,18 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   griddep_launch_dependents();
 
   // ---- units before every token ----------------------------------------------------------
+  int* const seq = sm.seq + kQ8Pad;
+  stage_tokens(a, P.t0, P.tn, seq, sm.len, blockIdx.x == 0);
+  __syncthreads();
   const int per = (P.tn + NT - 1) / NT;
   const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
   int sum = 0;
   for (int i = b0; i < b1; ++i) {
-    const long long t = P.t0 + i;
-    const TokInfo ti = q8_token_info(a, t, blockIdx.x == 0);
-    const bool mine = !token_in_long_run(a, P.min_run, t, ti.seq);
-    const int np = mine ? ti.npages : 0;
-    sm.seq[i] = static_cast<int>(ti.seq);
-    sm.len[i] = mine ? ti.L : -1;
     sm.pre[i] = sum;  // within this thread's run
-    sum += np * a.KVH;
+    if (P.skip_runs && in_staged_run(seq, i))
+      sm.len[i] = -1;
+    else
+      sum += (sm.len[i] + kPage - 1) / kPage * a.KVH;
   }
   int inc = sum;
 #pragma unroll
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     const int rem = u - sm.pre[tok];
     const int h = rem / np, p0 = rem - h * np;
     const int cnt = min(np - p0, u1 - u);  // pages of this segment
-    const long long btrow = static_cast<long long>(sm.seq[tok]) * a.bt_sb;
+    const long long btrow = static_cast<long long>(seq[tok]) * a.bt_sb;
     const long long t = P.t0 + tok;
 
     // Page ids, 32 at a time (lane i: page p0 + base + i).
@@ -678,11 +678,11 @@ bool q8_decode_supported(const Q8AttnArgs& g) {
          rows16(a.out, a.o_st, a.o_sh, a.o_sd);
 }
 
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, int min_run, int device, void* workspace,
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, int device, void* workspace,
                              cudaStream_t stream, int* launches) {
   DecParams p;
   p.g = g;
-  p.min_run = min_run;
+  p.skip_runs = skip_runs;
   p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
   const int sms = decode_sms(device);

@@ -18,9 +18,11 @@
 //                        weight would pass 2^20
 //   O_t += P_t V_j       kind::tf32, A = P_t from TMEM, B = V_j^T in shared memory
 // in the order S_0(j+1), O_1(j), S_1(j+1), O_0(j+1): each softmax has two products' time.
-// The codes are widened by three producer warps on their way into shared memory: 16 codes per
-// 16-byte load, K rows to 128-byte swizzled fp16 lines, V transposed (lane = key) to lines of 32
-// keys in fp32, 64 keys at a time; loads run one half-block ahead in registers.
+// The codes are widened by four producer warps on their way into shared memory, one page of 16 keys
+// each at a time: K rows to 128-byte swizzled fp16 lines, V transposed (lane = key) to lines of 32
+// keys in fp32.  Addresses are lane constants plus immediates: with one producer warp per scheduler
+// it is the length of its instruction stream that counts (three warps that took 8 keys of every
+// page needed 2.5 times the instructions, and the prompt case 190 us).
 //
 // Scheduling.  Every CTA lists the launch's windows (a scan over its tokens), and cuts a window's
 // blocks into equal parts of at most max(4, all blocks / CTAs): a lone long prompt would otherwise
@@ -28,8 +30,9 @@
 // then whole ones by length.  Cut windows leave fp32 states in the workspace, joined by
 // q8_merge_kernel.
 //
-// Warps: 0 MMA issuer, 1-3 producers, 4-7 softmax of tile 0, 8-11 of tile 1 (TMEM lane quadrant =
-// warp % 4).  setmaxnreg: 384 x 168 = 64,512 at launch = 128 x 88 + 256 x 208.
+// Warps: 0-3 producers, 4-7 softmax of tile 0, 8-11 of tile 1 (TMEM lane quadrant = warp % 4), 12
+// MMA issuer, 13-15 only list windows.  setmaxnreg: 512 x 128 = 65,536 registers at launch =
+// 128 x 104 + 256 x 160 + 128 x 88.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -46,9 +49,10 @@ namespace ss {
 
 namespace {
 
-constexpr int kThreads = 384;
-constexpr int kLaunchRegs = 168, kRegsProducer = 88, kRegsSoftmax = 208;
-static_assert(128 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs,
+constexpr int kThreads = 512;
+constexpr int kWorkers = 416;      // threads of the warps that take work items
+constexpr int kLaunchRegs = 128, kRegsProducer = 104, kRegsSoftmax = 160, kRegsIssuer = 88;
+static_assert(128 * kRegsProducer + 256 * kRegsSoftmax + 128 * kRegsIssuer <= kThreads * kLaunchRegs,
               "setmaxnreg split exceeds the launch register pool");
 constexpr int kRows = 128;         // rows of a tile
 constexpr int kNB = 128;           // keys of a block
@@ -69,7 +73,9 @@ struct Lay {
   static constexpr int kV = 2 * D * 128;             // V^T of 64 keys, fp32: 2 atoms of 32 keys
   static constexpr int kOffK = 2 * kQ;
   static constexpr int kOffV = kOffK + 2 * kK;
-  static constexpr int kOffCtl = kOffV + 2 * kV;
+  static constexpr int kOffSlots = kOffV + 2 * kV;   // codes on their way: 2 half-blocks
+  static constexpr int kSlots = 2 * 2 * kHalves * 128 * 16;
+  static constexpr int kOffCtl = kOffSlots + kSlots;
 };
 
 enum : int { kBarQ = 0, kBarS = 2, kBarPH = 4, kBarP = 6, kBarPV = 8, kBarKF = 10, kBarKE = 12,
@@ -82,11 +88,10 @@ struct CtlQ {
   int item[2];
   int abort;
   int nwin, total;        // windows; parts * KV heads
-  int red[2][12];
-  unsigned short first[kMaxWin], count[kMaxWin], parts[kMaxWin], order[kMaxWin];
+  int red[2][kThreads / 32];
+  unsigned short first[kMaxWin], count[kMaxWin], order[kMaxWin];
   int cum[kMaxWin + 1];   // work items before each rank
   int keys[kMaxWin];
-  int hist[kBins];
 };
 
 struct PrefillParams {
@@ -124,6 +129,22 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 }
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t a) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// 16 bytes from global to shared memory, or 16 zeros (bytes = 0).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Sum and (exclusive) maximum scans over the CTA.
@@ -185,9 +206,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(kBarPH + t), 128);
       mbar_init(bar(kBarP + t), 128);
       mbar_init(bar(kBarPV + t), 1);
-      mbar_init(bar(kBarKF + t), 3);
+      mbar_init(bar(kBarKF + t), 4);
       mbar_init(bar(kBarKE + t), 1);
-      mbar_init(bar(kBarVF + t), 3);
+      mbar_init(bar(kBarVF + t), 4);
       mbar_init(bar(kBarVE + t), 1);
     }
     mbar_init(bar(kBarEnd), 1);
@@ -202,15 +223,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_launch_dependents();
   const int first_item = tid == 0 ? static_cast<int>(atomicAdd(P.sched, 1u)) : 0;
 
+  int* const hist = reinterpret_cast<int*>(smem + L::kOffSlots);
   // ---- the windows of this launch ----------------------------------------------------------
   for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
-  for (int i = tid; i < kBins; i += kThreads) ctl->hist[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   {
+    // The operand buffers are idle: the staged ids and lengths stand there.
+    int* const seq = reinterpret_cast<int*>(smem) + kQ8Pad;
+    int* const len = seq + kMaxTokP + kQ8Pad;
+    stage_tokens(a, P.t0, P.tn, seq, len, blockIdx.x == 0);
+    __syncthreads();
     const int per = (P.tn + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
-    auto seq_of = [&](int i) { return ld_index(a.seq, a.seq64, P.t0 + i); };
-    auto in_run = [&](int i) { return token_in_long_run(a, kQ8MinRun, P.t0 + i, seq_of(i)); };
-    auto starts = [&](int i) { return i == 0 || seq_of(i - 1) != seq_of(i); };
+    auto in_run = [&](int i) { return in_staged_run(seq, i); };
+    auto starts = [&](int i) { return i == 0 || seq[i - 1] != seq[i]; };
     int start = -1;  // last run start at or before a token
     for (int i = b0; i < b1; ++i)
       if (starts(i)) start = i;
@@ -224,15 +250,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     int nwin;
     int idx = scan_sum(n, ctl->red[1], warp, lane, nwin) - 1;
     start = before;
+    int most_keys = 0;  // of this thread's tokens of window idx
     for (int i = b0; i < b1; ++i) {
       if (starts(i)) start = i;
       if (!in_run(i)) continue;
       const int at = (i - start) % tw;
-      if (at == 0) ctl->first[++idx] = static_cast<unsigned short>(i);
-      if (at == tw - 1 || i + 1 == P.tn || starts(i + 1))
-        ctl->count[idx] = static_cast<unsigned short>(at + 1);
-      const TokInfo ti = q8_token_info(a, P.t0 + i, blockIdx.x == 0);
-      atomicMax(&ctl->keys[idx], ti.L);
+      if (at == 0) {
+        ctl->first[++idx] = static_cast<unsigned short>(i);
+        most_keys = 0;
+      }
+      most_keys = max(most_keys, len[i]);
+      const bool ends = at == tw - 1 || i + 1 == P.tn || starts(i + 1);
+      if (ends) ctl->count[idx] = static_cast<unsigned short>(at + 1);
+      if (ends || i + 1 == b1) atomicMax(&ctl->keys[idx], most_keys);
     }
     __syncthreads();
     // Blocks of every window; the largest part, and the order in which parts are taken.
@@ -246,12 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nb = (ctl->keys[w] + kNB - 1) / kNB;
       return nb > most ? 0 : kBins - 1 - min(nb, kBins - 2);
     };
-    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&ctl->hist[bin_of(w)], 1);
+    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&hist[bin_of(w)], 1);
     __syncthreads();
     if (warp == 0) {
       int local = 0;
 #pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) local += ctl->hist[lane * (kBins / 32) + i];
+      for (int i = 0; i < kBins / 32; ++i) local += hist[lane * (kBins / 32) + i];
       int inc = local;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -261,8 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int run = inc - local;
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
-        const int b = lane * (kBins / 32) + i, h = ctl->hist[b];
-        ctl->hist[b] = run;
+        const int b = lane * (kBins / 32) + i, h = hist[b];
+        hist[b] = run;
         run += h;
       }
       __syncwarp();
@@ -270,9 +300,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = base + lane;
         const int b = w < nwin ? bin_of(w) : -1;
         const unsigned same = __match_any_sync(0xffffffffu, b);
-        if (w < nwin) ctl->order[ctl->hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
+        if (w < nwin) ctl->order[hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
         __syncwarp();
-        if (w < nwin && lane == __ffs(same) - 1) ctl->hist[b] += __popc(same);
+        if (w < nwin && lane == __ffs(same) - 1) hist[b] += __popc(same);
         __syncwarp();
       }
       // Work items before each rank; parts are equal shares of at most `most` blocks.
@@ -284,7 +314,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           w = ctl->order[r];
           const int nb = (ctl->keys[w] + kNB - 1) / kNB;
           parts = nb > most ? (nb + most - 1) / most : 1;
-          ctl->parts[w] = static_cast<unsigned short>(parts);
         }
         int inc2 = parts * a.KVH;
 #pragma unroll
@@ -324,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto next_item = [&]() -> Item {
     if (tid == 0) ctl->item[iter & 1] = iter == 0 ? first_item : static_cast<int>(atomicAdd(P.sched, 1u));
-    named_bar_sync(1, kThreads);
+    named_bar_sync(1, kWorkers);
     const int w = ctl->item[iter & 1];
     ++iter;
     Item it;
@@ -335,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int mid = (lo + hi) >> 1;
       if (ctl->cum[mid] <= w) lo = mid; else hi = mid;
     }
-    const int win = ctl->order[lo], rest = w - ctl->cum[lo], parts = ctl->parts[win];
+    const int win = ctl->order[lo], rest = w - ctl->cum[lo], parts = (ctl->cum[lo + 1] - ctl->cum[lo]) / a.KVH;
     it.first = ctl->first[win];
     it.count = ctl->count[win];
     it.keys = ctl->keys[win];
@@ -354,9 +383,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  if (warp < 4) {
-    setmaxnreg_dec<kRegsProducer>();
-    if (warp == 0) {
+  if (warp >= 12) {
+    setmaxnreg_dec<kRegsIssuer>();
+    if (warp == 12) {
       // ================================= MMA issuer ====================================
       constexpr uint32_t id_qk = idesc_of(0, kNB), id_pv = idesc_of(2, D);
       const bool leader = elect_one();
@@ -431,9 +460,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader) tc_commit(bar(kBarEnd));  // every product issued has completed before TMEM is freed
       __syncwarp();
       if (!wait_warp(bar(kBarEnd), 0)) timed_out();
-    } else {
+    }
+  } else if (warp < 4) {
+    setmaxnreg_dec<kRegsProducer>();
+    {
       // ================================== producers ====================================
-      const int pw = warp - 1;
+      // A producer warp widens page `warp` of each half-block (64 keys).
+      // K: load i covers 8 keys (8 (i & 1) + lane % 8) x 64 values (64 (i >> 1) + 16 (lane / 8)).
+      // V: load i covers 16 keys (lane % 16) x 32 values (32 i + 16 (lane / 16)).
+      constexpr int kLoads = 2 * L::kHalves;
+      // A lane's 16 bytes go to a slot of its own and come back to it: the slots stand in for
+      // registers, two half-blocks deep.
+      const uint32_t slots = sb + L::kOffSlots + (warp * 32 + lane) * 16;
+      const int k_key = lane & 7, v_key = lane & 15, hi = lane >> 4;
+      const long long k_off = k_key * pool.k_ss + 16 * (lane >> 3), v_off = v_key * pool.v_ss + 16 * hi;
+      // K lines: 16-byte chunk 2 (lane / 8) + q of a 64-value line, swizzled by the key.
+      uint32_t k_at[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        k_at[q] = sb + L::kOffK + (warp * 16 + k_key) * 128 + (((2 * (lane >> 3) + q) ^ k_key) << 4);
+      // V lines: value 16 hi + k (k = 0 .. 15) of this lane's key.  The upper lanes take their values
+      // in the order k ^ 4, which puts the two half-warps' stores into different banks.
+      uint32_t v_at[8];
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+        v_at[m] = sb + L::kOffV + (warp >> 1) * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
+                  (((((warp & 1) * 4 + (v_key >> 2)) ^ (4 * hi)) ^ m) << 4) + (v_key & 3) * 4;
       for (;;) {
         const Item it = next_item();
         if (!it.live) break;
@@ -456,106 +508,111 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float* s = sbase + id * pool.s_sn;
           return make_float2(__ldg(s), __ldg(s + pool.s_sw));
         };
-        constexpr int kIts = 8 * L::kHalves;       // 16-byte loads of a half-block per lane group
-        constexpr int kMine = (kIts + 2) / 3;
-        uint4 buf[kMine];
-        // K: iteration i covers 8 keys x 64 values (lane = chunk * 8 + key).
-        // V: iteration i covers 32 keys x 16 values (lane = key; the upper lanes take the
-        // neighbouring chunk, so that both halves of a sector are read together).
-        auto load_one = [&](int n, bool is_v, int j, int half, int ids, float vscale) -> uint4 {
-          const int i = pw + 3 * n;
-          int key, d;  // key inside the half-block
-          if (is_v) {
-            key = (i & 1) * 32 + lane;
-            d = 16 * ((i >> 1) ^ (lane >> 4));
-          } else {
-            key = (i & 7) * 8 + (lane & 7);
-            d = 64 * (i >> 3) + 16 * (lane >> 3);
-          }
-          const int in_block = half * 64 + key;
-          const int id = __shfl_sync(0xffffffffu, ids, in_block / kPage);
-          const float vs = __shfl_sync(0xffffffffu, vscale, in_block / kPage);
-          if (i >= kIts || id < 0 || (it.j0 + j) * kNB + in_block >= it.keys || (is_v && !(vs >= kMinVs)))
-            return make_uint4(0, 0, 0, 0);
-          const uint8_t* p = is_v ? vbase + id * pool.v_sn + (key % kPage) * pool.v_ss + d
-                                  : kbase + id * pool.k_sn + (key % kPage) * pool.k_ss + d;
-          return __ldg(reinterpret_cast<const uint4*>(p));
+        // Half-blocks in the order K(0), then K(j + 1), V(j) for every block j.
+        const int units = 4 * nblk;
+        auto unit = [&](int n, bool& is_v, int& j, int& half) {
+          const int m = n - 2;
+          half = n & 1;
+          is_v = n >= 2 && ((m & 2) || m / 4 == nblk - 1);
+          j = n < 2 ? 0 : m / 4 + (is_v ? 0 : 1);
         };
-        auto emit_one = [&](int n, bool is_v, int half, int st, const uint4& v) {
-          const int i = pw + 3 * n;
-          if (i >= kIts) return;
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          if (is_v) {
-            const int key = lane, d0 = 16 * ((i >> 1) ^ (lane >> 4));
-            const uint32_t base = sb + L::kOffV + half * L::kV + (i & 1) * (D * 128) + d0 * 128 + (key & 3) * 4;
+        int id_v = -1, id_k = -1, id_n = load_id(0), next_id = 1;
+        float2 sc_v = make_float2(0.f, 1.f), sc_k = sc_v, sc_n = load_scale(id_n);
+        int id_n2 = load_id(1);
+        auto issue = [&](int n) {
+          if (n < units) {
+            bool is_v;
+            int j, half;
+            unit(n, is_v, j, half);
+            if (!is_v && half == 0) {  // on to the next block
+              id_v = id_k; sc_v = sc_k;
+              id_k = id_n; sc_k = sc_n;
+              id_n = id_n2; sc_n = load_scale(id_n);
+              id_n2 = load_id(++next_id);
+              if (warp == 0 && lane < kPages) {
+                const float vs = fmaxf(sc_k.y, kMinVs);
+                ctl->sc[(jg + j) & 3][lane] = make_float4(sc_k.x, lg2(vs), __frcp_rn(vs), 0.f);
+              }
+            } else if (is_v && half == 0 && j == nblk - 1) {  // the last block has no K after it
+              id_v = id_k; sc_v = sc_k;
+            }
+            const int page = half * 4 + warp;
+            const int id = __shfl_sync(0xffffffffu, is_v ? id_v : id_k, page);
+            const float vs = __shfl_sync(0xffffffffu, sc_v.y, page);
+            const int left = id >= 0 && (!is_v || vs >= kMinVs) ? it.keys - (it.j0 + j) * kNB - page * kPage : 0;
+            const uint32_t dst = slots + (n & 1) * (kLoads * 128 * 16);
+            if (is_v) {
+              const uint8_t* p = vbase + max(id, 0) * pool.v_sn + v_off;
+              const int bytes = v_key < left ? 16 : 0;
+#pragma unroll
+              for (int i = 0; i < kLoads; ++i) cp_async16(dst + i * (128 * 16), bytes ? p + 32 * i : vbase, bytes);
+            } else {
+              const uint8_t* p = kbase + max(id, 0) * pool.k_sn + k_off;
+#pragma unroll
+              for (int i = 0; i < kLoads; ++i) {
+                const int bytes = k_key + 8 * (i & 1) < left ? 16 : 0;
+                cp_async16(dst + i * (128 * 16), bytes ? p + 8 * (i & 1) * pool.k_ss + 64 * (i >> 1) : kbase, bytes);
+              }
+            }
+          }
+          cp_async_commit();
+        };
+        auto emit_k = [&](uint32_t src, uint32_t stage) {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const uint4 v = ld_shared16(src + i * (128 * 16));
+            uint32_t h[8];
+            widen<FMT>(v.x, h[0], h[1]);
+            widen<FMT>(v.y, h[2], h[3]);
+            widen<FMT>(v.z, h[4], h[5]);
+            widen<FMT>(v.w, h[6], h[7]);
+            const uint32_t off = stage + (i >> 1) * (kNB * 128) + (i & 1) * (8 * 128);
+            st_shared16(k_at[0] + off, h[0], h[1], h[2], h[3]);
+            st_shared16(k_at[1] + off, h[4], h[5], h[6], h[7]);
+          }
+        };
+        auto emit_v = [&](uint32_t src, uint32_t stage) {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const uint4 v = ld_shared16(src + i * (128 * 16));
+            const uint32_t w[4] = {hi ? v.y : v.x, hi ? v.x : v.y, hi ? v.w : v.z, hi ? v.z : v.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               uint32_t f[4];
               widen_f32<FMT>(w[q], f);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)  // d0 is a multiple of 16: the line's phase is (4 q + e) % 8
-                st_shared4(base + (4 * q + e) * 128 + (((key >> 2) ^ ((4 * q + e) & 7)) << 4), f[e]);
-            }
-          } else {
-            const int key = half * 64 + (i & 7) * 8 + (lane & 7), c = 2 * (lane >> 3);
-            const uint32_t line = sb + L::kOffK + st * L::kK + (i >> 3) * (kNB * 128) + key * 128;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t h[4];
-              widen<FMT>(w[2 * q], h[0], h[1]);
-              widen<FMT>(w[2 * q + 1], h[2], h[3]);
-              st_shared16(line + (((c + q) ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
+              for (int e = 0; e < 4; ++e)
+                st_shared4(v_at[(4 * q + e) & 7] + stage + i * (32 * 128) + (4 * q + e) * 128, f[e]);
             }
           }
         };
-        // Order: K(0), then K(j + 1), V(j) for every block j, each in two halves.
-        int id_v = -1, id_k = load_id(0), id_n = load_id(1);
-        float2 sc_v = make_float2(0.f, 1.f), sc_k = load_scale(id_k);
-#pragma unroll
-        for (int n = 0; n < kMine; ++n) buf[n] = load_one(n, false, 0, 0, id_k, sc_k.y);
-        for (int j = -1; j < nblk && ok; ++j) {
-          // On entry buf holds the first half of K(j + 1), or of V(j) for the last block.
-          const int jk = jg + j + 1, stk = jk & 1;
-          const int id_n2 = load_id(j + 3);
-          const float2 sc_n = load_scale(id_n);
+        issue(0);
+        issue(1);
 #pragma unroll 1
-          for (int u = (j + 1 < nblk) ? 0 : 2; u < (j >= 0 ? 4 : 2) && ok; ++u) {
-            const bool is_v = u >= 2;
-            const int half = u & 1;
-            // The next half-block, loaded into the registers as this one leaves them.
-            bool nv, more = true;
-            int nj, nh, nid;
-            float nvs;
-            if (u == 0) { nv = false; nj = j + 1; nh = 1; nid = id_k; nvs = sc_k.y; }
-            else if (u == 1 && j >= 0) { nv = true; nj = j; nh = 0; nid = id_v; nvs = sc_v.y; }
-            else if (u == 2) { nv = true; nj = j; nh = 1; nid = id_v; nvs = sc_v.y; }
-            else if (j + 2 < nblk) { nv = false; nj = j + 2; nh = 0; nid = id_n; nvs = sc_n.y; }
-            else { nv = true; nj = j + 1; nh = 0; nid = id_k; nvs = sc_k.y; more = j + 1 < nblk; }
-            if (is_v) {
-              ok = wait_warp(bar(kBarVE + half), ((jg + j) & 1) ^ 1);
-            } else if (half == 0) {
-              ok = wait_warp(bar(kBarKE + stk), ((jk >> 1) & 1) ^ 1);
-            }
-            if (!ok) break;
-#pragma unroll
-            for (int n = 0; n < kMine; ++n) {
-              emit_one(n, is_v, half, stk, buf[n]);
-              if (more) buf[n] = load_one(n, nv, nj, nh, nid, nvs);
-            }
-            if (!is_v && half == 0 && pw == 0 && lane < kPages) {
-              const float vs = fmaxf(sc_k.y, kMinVs);
-              ctl->sc[jk & 3][lane] = make_float4(sc_k.x, lg2(vs), __frcp_rn(vs), 0.f);
-            }
-            if (is_v || half == 1) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(is_v ? kBarVF + half : kBarKF + stk));
-            }
+        for (int n = 0; n < units && ok; ++n) {
+          bool is_v;
+          int j, half;
+          unit(n, is_v, j, half);
+          const int jb = jg + j, st = jb & 1;
+          cp_async_wait<1>();
+          if (is_v)
+            ok = wait_warp(bar(kBarVE + half), (jb & 1) ^ 1);
+          else if (half == 0)
+            ok = wait_warp(bar(kBarKE + st), ((jb >> 1) & 1) ^ 1);
+          if (!ok) break;
+          const uint32_t src = slots + (n & 1) * (kLoads * 128 * 16);
+          if (is_v)
+            emit_v(src, half * L::kV);
+          else
+            emit_k(src, st * L::kK + half * (64 * 128));
+          issue(n + 2);
+          if (is_v || half == 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(is_v ? kBarVF + half : kBarKF + st));
           }
-          id_v = id_k; sc_v = sc_k;
-          id_k = id_n; sc_k = sc_n;
-          id_n = id_n2;
         }
+        cp_async_wait<0>();
         if (!ok) timed_out();
         jg += nblk;
       }
@@ -621,32 +678,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait_warp(bar(kBarS + tt), jb & 1);
           if (!ok) break;
           tc_fence_after();
-          uint32_t sr[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
-          // Page constants.  The factor is kept above 0 so that a masked score stays -inf under
-          // a zero scale.
-          const float4* sc = ctl->sc[(jg + j) & 3];
-          auto factor = [&](const float4& c) { return fmaxf(c.x * f_row, 1e-37f); };
-          tmem_wait_ld();
+          // Keys 64-127 are read once for the row's maximum and again for the weights, so that no
+          // more than 64 scores are held at a time.
+          uint32_t lo[32], up[32];
           const int nv = lim - (it.j0 + j) * kNB;
-          if (!__all_sync(0xffffffffu, nv >= kNB)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
+          const bool partial = !__all_sync(0xffffffffu, nv >= kNB);
+          const float4* sc = ctl->sc[(jg + j) & 3];
+          // The factor is kept above 0 so that a masked score stays -inf under a zero scale.
+          auto factor = [&](const float4& c) { return fmaxf(c.x * f_row, 1e-37f); };
+          auto mask = [&](uint32_t (&x)[32], int c) {
+            if (partial) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (c * 32 + i >= nv) sr[c][i] = __float_as_uint(-CUDART_INF_F);
-          }
+                if (c * 32 + i >= nv) x[i] = __float_as_uint(-CUDART_INF_F);
+            }
+          };
           float top = -CUDART_INF_F;
+          auto maximum = [&](const uint32_t (&x)[32], int c) {
 #pragma unroll
-          for (int p = 0; p < kPages; ++p) {
-            const uint32_t* s = &sr[p >> 1][(p & 1) * 16];
-            float m = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+            for (int h = 0; h < 2; ++h) {
+              float m = fmaxf(__uint_as_float(x[16 * h]), __uint_as_float(x[16 * h + 1]));
 #pragma unroll
-            for (int i = 2; i < 16; i += 2) m = max3(m, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-            const float4 pc = sc[p];
-            top = fmaxf(top, fmaf(m, factor(pc), pc.y));
-          }
+              for (int i = 2; i < 16; i += 2)
+                m = max3(m, __uint_as_float(x[16 * h + i]), __uint_as_float(x[16 * h + i + 1]));
+              const float4 pc = sc[2 * c + h];
+              top = fmaxf(top, fmaf(m, factor(pc), pc.y));
+            }
+          };
+          tmem_ld32(tS + 64, lo);
+          tmem_ld32(tS + 96, up);
+          tmem_wait_ld();
+          mask(lo, 2);
+          mask(up, 3);
+          maximum(lo, 2);
+          maximum(up, 3);
+          tmem_ld32(tS, lo);
+          tmem_ld32(tS + 32, up);
+          tmem_wait_ld();
+          mask(lo, 0);
+          mask(up, 1);
+          maximum(lo, 0);
+          maximum(up, 1);
           const bool raise = top > ref + kSlackP;
           const float ref_new = raise ? top : ref;
           const float alpha = raise ? ex2(ref - ref_new) : 1.f;
@@ -667,22 +739,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           ref = ref_new;
           const float base = ref == -CUDART_INF_F ? 0.f : ref;
           float part = 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          auto weights = [&](uint32_t (&x)[32], int c) {  // scores of 32 keys into weights, stored
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int p = 2 * c + h;
-              const float4 pc = sc[p];
+              const float4 pc = sc[2 * c + h];
               const float f = factor(pc), b = pc.y - base;
               const uint64_t f2 = f2pack(f, f), b2 = f2pack(b, b);
               uint64_t acc[2] = {0, 0};
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                uint32_t& s0 = sr[c][h * 16 + 2 * i];
-                uint32_t& s1 = sr[c][h * 16 + 2 * i + 1];
+                uint32_t& s0 = x[h * 16 + 2 * i];
+                uint32_t& s1 = x[h * 16 + 2 * i + 1];
                 const uint64_t x2 = fma2(f2pack(__uint_as_float(s0), __uint_as_float(s1)), f2, b2);
                 uint64_t w2;
-                if ((p * 8 + i) % kPolyEvery == kPolyEvery - 1) {
+                if ((h * 8 + i) % kPolyEvery == kPolyEvery - 1) {
                   w2 = exp2_poly2(x2);
                 } else {
                   float x0, x1;
@@ -697,13 +767,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               f2unpack(add2(acc[0], acc[1]), a0, a1);
               part = fmaf(a0 + a1, pc.z, part);
             }
-            tmem_st32(tS + c * 32, sr[c]);
-            if (c & 1) {
-              tmem_wait_st();
-              tc_fence_before();
-              mbar_arrive(bar((c == 1 ? kBarPH : kBarP) + tt));
-            }
-          }
+            tmem_st32(tS + c * 32, x);
+          };
+          weights(lo, 0);
+          tmem_ld32(tS + 64, lo);
+          weights(up, 1);
+          tmem_ld32(tS + 96, up);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(kBarPH + tt));
+          tmem_wait_ld();
+          mask(lo, 2);
+          mask(up, 3);
+          weights(lo, 2);
+          weights(up, 3);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(kBarP + tt));
           lsum = lsum * alpha + part;
         }
         // ---- O_t / l, or the state of a cut window ----------------------------------------
