@@ -18,11 +18,13 @@
 //                        weight would pass 2^20
 //   O_t += P_t V_j       kind::tf32, A = P_t from TMEM, B = V_j^T in shared memory
 // in the order S_0(j+1), O_1(j), S_1(j+1), O_0(j+1): each softmax has two products' time.
-// The codes are widened by four producer warps on their way into shared memory, one page of 16 keys
-// each at a time: K rows to 128-byte swizzled fp16 lines, V transposed (lane = key) to lines of 32
-// keys in fp32.  Addresses are lane constants plus immediates: with one producer warp per scheduler
-// it is the length of its instruction stream that counts (three warps that took 8 keys of every
-// page needed 2.5 times the instructions, and the prompt case 190 us).
+// The codes are widened on their way into shared memory: K rows to 128-byte swizzled fp16 lines by
+// three warps, V transposed (lane = key) to lines of 32 keys in fp32 by four, a page's
+// registers being loaded for the next block as soon as it is stored.
+//
+// The roles' loops are kept rolled and small: with everything unrolled each warp ran at about one
+// instruction in five cycles, the rate at which instructions came from the cache, a key block took
+// 10,000 cycles whatever was taken out of it, and the prompt case 123 us.
 //
 // Scheduling.  Every CTA lists the launch's windows (a scan over its tokens), and cuts a window's
 // blocks into equal parts of at most max(4, all blocks / CTAs): a lone long prompt would otherwise
@@ -30,9 +32,9 @@
 // then whole ones by length.  Cut windows leave fp32 states in the workspace, joined by
 // q8_merge_kernel.
 //
-// Warps: 0-3 producers, 4-7 softmax of tile 0, 8-11 of tile 1 (TMEM lane quadrant = warp % 4), 12
-// MMA issuer, 13-15 only list windows.  setmaxnreg: 512 x 128 = 65,536 registers at launch =
-// 128 x 104 + 256 x 160 + 128 x 88.
+// Warps: 0 MMA issuer, 1-3 K, 4-7 V, 8-11 softmax of tile 0, 12-15 of tile 1
+// (TMEM lane quadrant = warp % 4).  setmaxnreg: 512 x 128 = 65,536 registers at launch =
+// 256 x 112 + 256 x 144.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -50,9 +52,9 @@ namespace ss {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kWorkers = 416;      // threads of the warps that take work items
-constexpr int kLaunchRegs = 128, kRegsProducer = 104, kRegsSoftmax = 160, kRegsIssuer = 88;
-static_assert(128 * kRegsProducer + 256 * kRegsSoftmax + 128 * kRegsIssuer <= kThreads * kLaunchRegs,
+constexpr int kSoftmaxWarp = 8;    // first softmax warp
+constexpr int kLaunchRegs = 128, kRegsProducer = 112, kRegsSoftmax = 144;
+static_assert(256 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs,
               "setmaxnreg split exceeds the launch register pool");
 constexpr int kRows = 128;         // rows of a tile
 constexpr int kNB = 128;           // keys of a block
@@ -73,9 +75,7 @@ struct Lay {
   static constexpr int kV = 2 * D * 128;             // V^T of 64 keys, fp32: 2 atoms of 32 keys
   static constexpr int kOffK = 2 * kQ;
   static constexpr int kOffV = kOffK + 2 * kK;
-  static constexpr int kOffSlots = kOffV + 2 * kV;   // codes on their way: 2 half-blocks
-  static constexpr int kSlots = 2 * 2 * kHalves * 128 * 16;
-  static constexpr int kOffCtl = kOffSlots + kSlots;
+  static constexpr int kOffCtl = kOffV + 2 * kV;
 };
 
 enum : int { kBarQ = 0, kBarS = 2, kBarPH = 4, kBarP = 6, kBarPV = 8, kBarKF = 10, kBarKE = 12,
@@ -92,6 +92,7 @@ struct CtlQ {
   unsigned short first[kMaxWin], count[kMaxWin], order[kMaxWin];
   int cum[kMaxWin + 1];   // work items before each rank
   int keys[kMaxWin];
+  int hist[kBins];
 };
 
 struct PrefillParams {
@@ -129,22 +130,6 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 }
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t a) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
-}
-
-__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-// 16 bytes from global to shared memory, or 16 zeros (bytes = 0).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Sum and (exclusive) maximum scans over the CTA.
@@ -206,9 +191,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(kBarPH + t), 128);
       mbar_init(bar(kBarP + t), 128);
       mbar_init(bar(kBarPV + t), 1);
-      mbar_init(bar(kBarKF + t), 4);
+      mbar_init(bar(kBarKF + t), 3);
       mbar_init(bar(kBarKE + t), 1);
-      mbar_init(bar(kBarVF + t), 4);
+      mbar_init(bar(kBarVF + t), 2);
       mbar_init(bar(kBarVE + t), 1);
     }
     mbar_init(bar(kBarEnd), 1);
@@ -223,10 +208,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_launch_dependents();
   const int first_item = tid == 0 ? static_cast<int>(atomicAdd(P.sched, 1u)) : 0;
 
-  int* const hist = reinterpret_cast<int*>(smem + L::kOffSlots);
   // ---- the windows of this launch ----------------------------------------------------------
   for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
-  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) ctl->hist[i] = 0;
   {
     // The operand buffers are idle: the staged ids and lengths stand there.
     int* const seq = reinterpret_cast<int*>(smem) + kQ8Pad;
@@ -276,12 +260,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nb = (ctl->keys[w] + kNB - 1) / kNB;
       return nb > most ? 0 : kBins - 1 - min(nb, kBins - 2);
     };
-    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&hist[bin_of(w)], 1);
+    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&ctl->hist[bin_of(w)], 1);
     __syncthreads();
     if (warp == 0) {
       int local = 0;
 #pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) local += hist[lane * (kBins / 32) + i];
+      for (int i = 0; i < kBins / 32; ++i) local += ctl->hist[lane * (kBins / 32) + i];
       int inc = local;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -291,8 +275,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int run = inc - local;
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
-        const int b = lane * (kBins / 32) + i, h = hist[b];
-        hist[b] = run;
+        const int b = lane * (kBins / 32) + i, h = ctl->hist[b];
+        ctl->hist[b] = run;
         run += h;
       }
       __syncwarp();
@@ -300,9 +284,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = base + lane;
         const int b = w < nwin ? bin_of(w) : -1;
         const unsigned same = __match_any_sync(0xffffffffu, b);
-        if (w < nwin) ctl->order[hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
+        if (w < nwin) ctl->order[ctl->hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
         __syncwarp();
-        if (w < nwin && lane == __ffs(same) - 1) hist[b] += __popc(same);
+        if (w < nwin && lane == __ffs(same) - 1) ctl->hist[b] += __popc(same);
         __syncwarp();
       }
       // Work items before each rank; parts are equal shares of at most `most` blocks.
@@ -353,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto next_item = [&]() -> Item {
     if (tid == 0) ctl->item[iter & 1] = iter == 0 ? first_item : static_cast<int>(atomicAdd(P.sched, 1u));
-    named_bar_sync(1, kWorkers);
+    named_bar_sync(1, kThreads);
     const int w = ctl->item[iter & 1];
     ++iter;
     Item it;
@@ -383,9 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  if (warp >= 12) {
-    setmaxnreg_dec<kRegsIssuer>();
-    if (warp == 12) {
+  if (warp < kSoftmaxWarp) {
+    setmaxnreg_dec<kRegsProducer>();
+    if (warp == 0) {
       // ================================= MMA issuer ====================================
       constexpr uint32_t id_qk = idesc_of(0, kNB), id_pv = idesc_of(2, D);
       const bool leader = elect_one();
@@ -396,30 +380,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool two = it.count > P.tpt;  // both tiles hold tokens
         auto qk = [&](int t, int st) {
           if (leader) {
-            const uint64_t qd = smem_desc_sw128(sb + t * L::kQ, 16, 1024);
-            const uint64_t kd = smem_desc_sw128(sb + L::kOffK + st * L::kK, 16, 1024);
+            uint64_t qd = smem_desc_sw128(sb + t * L::kQ, 16, 1024);
+            uint64_t kd = smem_desc_sw128(sb + L::kOffK + st * L::kK, 16, 1024);
+#pragma unroll 1
+            for (int i = 0; i < L::kHalves; ++i) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
-              tc_mma_f16(tmem + t * kNB, qd + off, kd + off, id_qk, kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                tc_mma_f16(tmem + t * kNB, qd + kk * 2, kd + kk * 2, id_qk, (i | kk) ? 1u : 0u);
+              qd += kRows * 128 / 16;
+              kd += kNB * 128 / 16;
             }
             tc_commit(bar(kBarS + t));
           }
           __syncwarp();
         };
         auto pv = [&](int t, int j, bool release) -> bool {  // block j of this item
-#pragma unroll
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
             if (!wait_warp(bar(kBarVF + half), (jg + j) & 1)) return false;
             if (!wait_warp(bar((half ? kBarP : kBarPH) + t), (jt[t] + j) & 1)) return false;
             tc_fence_after();
             if (leader) {
-              const uint64_t vd = smem_desc_sw128(sb + L::kOffV + half * L::kV, 16, 1024);
+              uint64_t vd = smem_desc_sw128(sb + L::kOffV + half * L::kV, 16, 1024);
+              uint32_t pa = tmem + t * kNB + half * 64;
+#pragma unroll 1
+              for (int i = 0; i < 2; ++i) {  // 32 keys each
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)
-                tc_mma_tf32_ts(tmem + 256 + t * 128, tmem + t * kNB + half * 64 + kk * 8,
-                               vd + (((kk >> 2) * (D * 128) + (kk & 3) * 32) >> 4), id_pv,
-                               (j > 0 || half > 0 || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < 4; ++kk)
+                  tc_mma_tf32_ts(tmem + 256 + t * 128, pa + kk * 8, vd + kk * 2, id_pv,
+                                 (j | half | i | kk) ? 1u : 0u);
+                vd += D * 128 / 16;
+                pa += 32;
+              }
               if (release) tc_commit(bar(kBarVE + half));
             }
             __syncwarp();
@@ -460,41 +452,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader) tc_commit(bar(kBarEnd));  // every product issued has completed before TMEM is freed
       __syncwarp();
       if (!wait_warp(bar(kBarEnd), 0)) timed_out();
-    }
-  } else if (warp < 4) {
-    setmaxnreg_dec<kRegsProducer>();
-    {
+    } else {
       // ================================== producers ====================================
-      // A producer warp widens page `warp` of each half-block (64 keys).
-      // K: load i covers 8 keys (8 (i & 1) + lane % 8) x 64 values (64 (i >> 1) + 16 (lane / 8)).
-      // V: load i covers 16 keys (lane % 16) x 32 values (32 i + 16 (lane / 16)).
-      constexpr int kLoads = 2 * L::kHalves;
-      // A lane's 16 bytes go to a slot of its own and come back to it: the slots stand in for
-      // registers, two half-blocks deep.
-      const uint32_t slots = sb + L::kOffSlots + (warp * 32 + lane) * 16;
-      const int k_key = lane & 7, v_key = lane & 15, hi = lane >> 4;
-      const long long k_off = k_key * pool.k_ss + 16 * (lane >> 3), v_off = v_key * pool.v_ss + 16 * hi;
-      // K lines: 16-byte chunk 2 (lane / 8) + q of a 64-value line, swizzled by the key.
-      uint32_t k_at[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        k_at[q] = sb + L::kOffK + (warp * 16 + k_key) * 128 + (((2 * (lane >> 3) + q) ^ k_key) << 4);
-      // V lines: value 16 hi + k (k = 0 .. 15) of this lane's key.  The upper lanes take their values
-      // in the order k ^ 4, which puts the two half-warps' stores into different banks.
-      uint32_t v_at[8];
-#pragma unroll
-      for (int m = 0; m < 8; ++m)
-        v_at[m] = sb + L::kOffV + (warp >> 1) * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
-                  (((((warp & 1) * 4 + (v_key >> 2)) ^ (4 * hi)) ^ m) << 4) + (v_key & 3) * 4;
+      const bool is_v = warp >= 4;
+      // Page ids and scales of a block's 8 pages: lanes 0-7.  id -1: past the keys or outside the
+      // pool.
       for (;;) {
         const Item it = next_item();
         if (!it.live) break;
         const int nblk = it.j1 - it.j0;
         if (nblk <= 0) continue;
-        const uint8_t* kbase = pool.k + static_cast<long long>(it.kvh) * pool.k_sh;
-        const uint8_t* vbase = pool.v + static_cast<long long>(it.kvh) * pool.v_sh;
         const float* sbase = pool.scales + static_cast<long long>(it.kvh) * pool.s_sh;
-        // Page ids and scales of a block: lanes 0-7.  id -1: past the keys or outside the pool.
         auto load_id = [&](int j) -> int {
           const int pi = (it.j0 + j) * kPages + lane;
           if (j >= nblk || lane >= kPages || pi * kPage >= it.keys) return -1;
@@ -508,118 +476,132 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float* s = sbase + id * pool.s_sn;
           return make_float2(__ldg(s), __ldg(s + pool.s_sw));
         };
-        // Half-blocks in the order K(0), then K(j + 1), V(j) for every block j.
-        const int units = 4 * nblk;
-        auto unit = [&](int n, bool& is_v, int& j, int& half) {
-          const int m = n - 2;
-          half = n & 1;
-          is_v = n >= 2 && ((m & 2) || m / 4 == nblk - 1);
-          j = n < 2 ? 0 : m / 4 + (is_v ? 0 : 1);
-        };
-        int id_v = -1, id_k = -1, id_n = load_id(0), next_id = 1;
-        float2 sc_v = make_float2(0.f, 1.f), sc_k = sc_v, sc_n = load_scale(id_n);
-        int id_n2 = load_id(1);
-        auto issue = [&](int n) {
-          if (n < units) {
-            bool is_v;
-            int j, half;
-            unit(n, is_v, j, half);
-            if (!is_v && half == 0) {  // on to the next block
-              id_v = id_k; sc_v = sc_k;
-              id_k = id_n; sc_k = sc_n;
-              id_n = id_n2; sc_n = load_scale(id_n);
-              id_n2 = load_id(++next_id);
-              if (warp == 0 && lane < kPages) {
-                const float vs = fmaxf(sc_k.y, kMinVs);
-                ctl->sc[(jg + j) & 3][lane] = make_float4(sc_k.x, lg2(vs), __frcp_rn(vs), 0.f);
+        int id = load_id(0), id_next = load_id(1);
+        float2 scl = load_scale(id);
+        if (!is_v) {
+          // Warp 1 + r widens pages r, r + 3, r + 6.  Load (i, k) of a page: 8 keys (8 k + lane % 8) x
+          // 64 values (64 i + 16 (lane / 8)).
+          const int r = warp - 1, key = lane & 7;
+          const uint8_t* base = pool.k + static_cast<long long>(it.kvh) * pool.k_sh + key * pool.k_ss + 16 * (lane >> 3);
+          // 16-byte chunk 2 (lane / 8) + q of a line of 64 values, swizzled by the key.
+          uint32_t at[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            at[q] = sb + L::kOffK + key * 128 + (((2 * (lane >> 3) + q) ^ key) << 4);
+          auto load = [&](int j, int p, uint4 (&v)[L::kHalves][2]) {
+            const int pid = __shfl_sync(0xffffffffu, id, p & 31);
+            const int left = pid < 0 || p >= kPages ? 0 : it.keys - ((it.j0 + j) * kPages + p) * kPage;
+            const uint8_t* src = base + static_cast<long long>(max(pid, 0)) * pool.k_sn;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int i = 0; i < L::kHalves; ++i) {
+                v[i][k] = make_uint4(0, 0, 0, 0);
+                if (key + 8 * k < left) v[i][k] = __ldg(reinterpret_cast<const uint4*>(src + 8 * k * pool.k_ss + 64 * i));
               }
-            } else if (is_v && half == 0 && j == nblk - 1) {  // the last block has no K after it
-              id_v = id_k; sc_v = sc_k;
-            }
-            const int page = half * 4 + warp;
-            const int id = __shfl_sync(0xffffffffu, is_v ? id_v : id_k, page);
-            const float vs = __shfl_sync(0xffffffffu, sc_v.y, page);
-            const int left = id >= 0 && (!is_v || vs >= kMinVs) ? it.keys - (it.j0 + j) * kNB - page * kPage : 0;
-            const uint32_t dst = slots + (n & 1) * (kLoads * 128 * 16);
-            if (is_v) {
-              const uint8_t* p = vbase + max(id, 0) * pool.v_sn + v_off;
-              const int bytes = v_key < left ? 16 : 0;
+          };
+          uint4 buf[3][L::kHalves][2];
 #pragma unroll
-              for (int i = 0; i < kLoads; ++i) cp_async16(dst + i * (128 * 16), bytes ? p + 32 * i : vbase, bytes);
-            } else {
-              const uint8_t* p = kbase + max(id, 0) * pool.k_sn + k_off;
-#pragma unroll
-              for (int i = 0; i < kLoads; ++i) {
-                const int bytes = k_key + 8 * (i & 1) < left ? 16 : 0;
-                cp_async16(dst + i * (128 * 16), bytes ? p + 8 * (i & 1) * pool.k_ss + 64 * (i >> 1) : kbase, bytes);
-              }
-            }
-          }
-          cp_async_commit();
-        };
-        auto emit_k = [&](uint32_t src, uint32_t stage) {
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            const uint4 v = ld_shared16(src + i * (128 * 16));
-            uint32_t h[8];
-            widen<FMT>(v.x, h[0], h[1]);
-            widen<FMT>(v.y, h[2], h[3]);
-            widen<FMT>(v.z, h[4], h[5]);
-            widen<FMT>(v.w, h[6], h[7]);
-            const uint32_t off = stage + (i >> 1) * (kNB * 128) + (i & 1) * (8 * 128);
-            st_shared16(k_at[0] + off, h[0], h[1], h[2], h[3]);
-            st_shared16(k_at[1] + off, h[4], h[5], h[6], h[7]);
-          }
-        };
-        auto emit_v = [&](uint32_t src, uint32_t stage) {
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            const uint4 v = ld_shared16(src + i * (128 * 16));
-            const uint32_t w[4] = {hi ? v.y : v.x, hi ? v.x : v.y, hi ? v.w : v.z, hi ? v.z : v.w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t f[4];
-              widen_f32<FMT>(w[q], f);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                st_shared4(v_at[(4 * q + e) & 7] + stage + i * (32 * 128) + (4 * q + e) * 128, f[e]);
-            }
-          }
-        };
-        issue(0);
-        issue(1);
-#pragma unroll 1
-        for (int n = 0; n < units && ok; ++n) {
-          bool is_v;
-          int j, half;
-          unit(n, is_v, j, half);
-          const int jb = jg + j, st = jb & 1;
-          cp_async_wait<1>();
-          if (is_v)
-            ok = wait_warp(bar(kBarVE + half), (jb & 1) ^ 1);
-          else if (half == 0)
+          for (int n = 0; n < 3; ++n) load(0, r + 3 * n, buf[n]);
+          for (int j = 0; j < nblk; ++j) {
+            const int jb = jg + j, st = jb & 1;
+            const float2 now = scl;
+            id = id_next;
+            id_next = load_id(j + 2);
+            scl = load_scale(id);
             ok = wait_warp(bar(kBarKE + st), ((jb >> 1) & 1) ^ 1);
-          if (!ok) break;
-          const uint32_t src = slots + (n & 1) * (kLoads * 128 * 16);
-          if (is_v)
-            emit_v(src, half * L::kV);
-          else
-            emit_k(src, st * L::kK + half * (64 * 128));
-          issue(n + 2);
-          if (is_v || half == 1) {
+            if (!ok) break;
+            if (r == 0 && lane < kPages) {
+              const float vs = fmaxf(now.y, kMinVs);
+              ctl->sc[jb & 3][lane] = make_float4(now.x, lg2(vs), __frcp_rn(vs), 0.f);
+            }
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+              if (r + 3 * n < kPages) {
+                const uint32_t off = st * L::kK + (r + 3 * n) * (16 * 128);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int i = 0; i < L::kHalves; ++i) {
+                    const uint4 v = buf[n][i][k];
+                    uint32_t w[8];
+                    widen<FMT>(v.x, w[0], w[1]);
+                    widen<FMT>(v.y, w[2], w[3]);
+                    widen<FMT>(v.z, w[4], w[5]);
+                    widen<FMT>(v.w, w[6], w[7]);
+                    st_shared16(at[0] + off + i * (kNB * 128) + 8 * k * 128, w[0], w[1], w[2], w[3]);
+                    st_shared16(at[1] + off + i * (kNB * 128) + 8 * k * 128, w[4], w[5], w[6], w[7]);
+                  }
+              }
+              load(j + 1, r + 3 * n, buf[n]);  // in flight until the next block
+            }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(is_v ? kBarVF + half : kBarKF + st));
+            if (lane == 0) mbar_arrive(bar(kBarKF + st));
+          }
+        } else {
+          // Warp 4 + 2 h + u widens pages 4 h + 2 u and the one after.  Load (p, i): 16 keys (lane %
+          // 16) of page p x 32 values (32 i + 16 (lane / 16)).
+          const int h = (warp - 4) >> 1, u = warp & 1, key = lane & 15, hi = lane >> 4;
+          const uint8_t* base = pool.v + static_cast<long long>(it.kvh) * pool.v_sh + key * pool.v_ss + 16 * hi;
+          // Line of value 16 hi + k (k = 0 .. 15), this lane's key.  The upper lanes take their values
+          // in the order k ^ 4, which puts the two half-warps' stores into different banks.
+          uint32_t at[8];
+#pragma unroll
+          for (int m = 0; m < 8; ++m)
+            at[m] = sb + L::kOffV + h * L::kV + u * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
+                    ((((key >> 2) ^ (4 * hi)) ^ m) << 4) + (key & 3) * 4;
+          auto load = [&](int j, int p, uint4 (&v)[D / 32]) {
+            const int pg = 4 * h + 2 * u + p;
+            const int pid = __shfl_sync(0xffffffffu, id, pg);
+            const float vs = __shfl_sync(0xffffffffu, scl.y, pg);
+            const int left = pid < 0 || !(vs >= kMinVs) ? 0 : it.keys - ((it.j0 + j) * kPages + pg) * kPage;
+            const uint8_t* src = base + static_cast<long long>(max(pid, 0)) * pool.v_sn;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              v[i] = make_uint4(0, 0, 0, 0);
+              if (key < left) v[i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
+            }
+          };
+          uint4 buf[2][D / 32];
+          load(0, 0, buf[0]);
+          load(0, 1, buf[1]);
+          for (int j = 0; j < nblk; ++j) {
+            const int jb = jg + j;
+            id = id_next;
+            id_next = load_id(j + 2);
+            scl = load_scale(id);
+            ok = wait_warp(bar(kBarVE + h), (jb & 1) ^ 1);
+            if (!ok) break;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                const uint4 v = buf[p][i];
+                const uint32_t w[4] = {hi ? v.y : v.x, hi ? v.x : v.y, hi ? v.w : v.z, hi ? v.z : v.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t f[4];
+                  widen_f32<FMT>(w[q], f);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)  // page 1: the other half of the line
+                    st_shared4((at[(4 * q + e) & 7] ^ (64 * p)) + i * (32 * 128) + (4 * q + e) * 128, f[e]);
+                }
+              }
+              load(j + 1, p, buf[p]);  // in flight until the next block
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kBarVF + h));
           }
         }
-        cp_async_wait<0>();
         if (!ok) timed_out();
         jg += nblk;
       }
     }
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
-    const int tt = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const int tt = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + tt * kNB + lane_off, tO = tmem + 256 + tt * 128 + lane_off;
     const int rt = row / a.group, rh = row - rt * a.group;  // token inside the tile, head
@@ -678,15 +660,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait_warp(bar(kBarS + tt), jb & 1);
           if (!ok) break;
           tc_fence_after();
-          // Keys 64-127 are read once for the row's maximum and again for the weights, so that no
-          // more than 64 scores are held at a time.
-          uint32_t lo[32], up[32];
+          // The scores are read twice, 32 at a time, for the row's maximum and for the weights: the
+          // loops stay rolled.  (Straight-line code for 128 scores runs at the rate at which the
+          // instruction cache refills, about one instruction in five cycles.)
           const int nv = lim - (it.j0 + j) * kNB;
           const bool partial = !__all_sync(0xffffffffu, nv >= kNB);
           const float4* sc = ctl->sc[(jg + j) & 3];
           // The factor is kept above 0 so that a masked score stays -inf under a zero scale.
           auto factor = [&](const float4& c) { return fmaxf(c.x * f_row, 1e-37f); };
-          auto mask = [&](uint32_t (&x)[32], int c) {
+          uint32_t x[32];
+          auto read = [&](int c) {
+            tmem_ld32(tS + c * 32, x);
+            tmem_wait_ld();
             if (partial) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -694,7 +679,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           };
           float top = -CUDART_INF_F;
-          auto maximum = [&](const uint32_t (&x)[32], int c) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            read(c);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float m = fmaxf(__uint_as_float(x[16 * h]), __uint_as_float(x[16 * h + 1]));
@@ -704,21 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float4 pc = sc[2 * c + h];
               top = fmaxf(top, fmaf(m, factor(pc), pc.y));
             }
-          };
-          tmem_ld32(tS + 64, lo);
-          tmem_ld32(tS + 96, up);
-          tmem_wait_ld();
-          mask(lo, 2);
-          mask(up, 3);
-          maximum(lo, 2);
-          maximum(up, 3);
-          tmem_ld32(tS, lo);
-          tmem_ld32(tS + 32, up);
-          tmem_wait_ld();
-          mask(lo, 0);
-          mask(up, 1);
-          maximum(lo, 0);
-          maximum(up, 1);
+          }
           const bool raise = top > ref + kSlackP;
           const float ref_new = raise ? top : ref;
           const float alpha = raise ? ex2(ref - ref_new) : 1.f;
@@ -726,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = wait_warp(bar(kBarPV + tt), (jb - 1) & 1);  // complete: S_t(j) was issued after it
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(tO + c * 32, o);
@@ -739,7 +712,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ref = ref_new;
           const float base = ref == -CUDART_INF_F ? 0.f : ref;
           float part = 0.f;
-          auto weights = [&](uint32_t (&x)[32], int c) {  // scores of 32 keys into weights, stored
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            read(c);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float4 pc = sc[2 * c + h];
@@ -768,22 +743,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               part = fmaf(a0 + a1, pc.z, part);
             }
             tmem_st32(tS + c * 32, x);
-          };
-          weights(lo, 0);
-          tmem_ld32(tS + 64, lo);
-          weights(up, 1);
-          tmem_ld32(tS + 96, up);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(bar(kBarPH + tt));
-          tmem_wait_ld();
-          mask(lo, 2);
-          mask(up, 3);
-          weights(lo, 2);
-          weights(up, 3);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(bar(kBarP + tt));
+            if (c & 1) {
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(bar((c == 1 ? kBarPH : kBarP) + tt));
+            }
+          }
           lsum = lsum * alpha + part;
         }
         // ---- O_t / l, or the state of a cut window ----------------------------------------
@@ -795,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ref == -CUDART_INF_F) lsum = 0.f;
           const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
           float4* st = reinterpret_cast<float4*>(P.part + static_cast<long long>(it.slot) * State<D>::kFloats) + tt * kRows + row;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             tmem_ld32(tO + c * 32, o);
