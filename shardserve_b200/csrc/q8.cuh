@@ -114,6 +114,16 @@ constexpr int kQ8MinRun = 8;   // tokens of shorter runs belong to the split-K k
 constexpr int kQ8Pad = kQ8MinRun - 1;
 __device__ __forceinline__ void stage_tokens(const AttnArgs& a, long long t0, int tn, int* seq,
                                              int* len, bool report) {
+  // The neighbours first: their loads are in flight with the others.  Past the batch's ends stands
+  // anything but the id of the token at the end.
+  int at = 0, neighbour = 0;
+  if (threadIdx.x < 2 * kQ8Pad) {
+    const int k = threadIdx.x;
+    at = k < kQ8Pad ? -1 - k : tn + k - kQ8Pad;
+    const long long t = t0 + at, in = t < 0 ? 0 : min(t, a.T - 1);
+    const int id = static_cast<int>(ld_index(a.seq, a.seq64, in));
+    neighbour = in == t ? id : ~id;
+  }
   constexpr int U = 8;  // loads in flight: every one is a round trip to L2 or beyond
   for (int i0 = threadIdx.x; i0 < tn; i0 += U * blockDim.x) {
     long long s[U], p[U];
@@ -131,13 +141,7 @@ __device__ __forceinline__ void stage_tokens(const AttnArgs& a, long long t0, in
       len[i] = s[u] == -1 ? 0 : token_info_from(a, s[u], p[u], report).L;
     }
   }
-  for (int k = threadIdx.x; k < 2 * kQ8Pad; k += blockDim.x) {
-    const int i = k < kQ8Pad ? -1 - k : tn + k - kQ8Pad;
-    const long long t = t0 + i;
-    // Past the batch's ends: anything but the id of the token at the end.
-    seq[i] = t >= 0 && t < a.T ? static_cast<int>(ld_index(a.seq, a.seq64, t))
-                               : ~static_cast<int>(ld_index(a.seq, a.seq64, t < 0 ? 0 : a.T - 1));
-  }
+  if (threadIdx.x < 2 * kQ8Pad) seq[at] = neighbour;
 }
 // Token i of staged ids lies in a run of at least kQ8MinRun tokens of one sequence.
 __device__ __forceinline__ bool in_staged_run(const int* seq, int i) {
@@ -154,11 +158,12 @@ cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_generic(const Q8AttnArgs& a, cudaStream_t stream);
 // Split-K kernel (q8_decode.cu): workspace bytes, the layouts it addresses, and the launch
-// (*launches: kernels enqueued).  skip_runs: tokens of runs belong to the tiles.
+// (*launches: kernels enqueued).  skip_runs: tokens of runs belong to the tiles; beside: the launch
+// before is the tiles', which this kernel does not wait for until its end.
 size_t q8_decode_workspace(int device);
 bool q8_decode_supported(const Q8AttnArgs& g);
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, int device, void* workspace,
-                             cudaStream_t stream, int* launches);
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, int device,
+                             void* workspace, cudaStream_t stream, int* launches);
 // tcgen05 tiles of prompt chunks (q8_prefill.cu), for runs of at least kQ8MinRun tokens: workspace
 // bytes of the cut windows' states, the layouts it takes, tokens per launch, and the launches of
 // the tiles and of the join of the cut windows.
@@ -166,9 +171,8 @@ size_t q8_prefill_workspace(int device);
 bool q8_prefill_supported(const Q8AttnArgs& g, int device);
 int q8_prefill_window();
 cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
-                              void* workspace, void* states, cudaStream_t stream);
-cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* workspace, void* states,
-                            cudaStream_t stream);
+                              void* states, cudaStream_t stream);
+cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* states, cudaStream_t stream);
 cudaError_t launch_block_tables(const BlockTablesArgs& a, cudaStream_t stream);
 int block_tables_max_rows();
 

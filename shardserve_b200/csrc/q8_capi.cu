@@ -172,22 +172,31 @@ int ss_ragged_paged_attention_q8(
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.err = static_cast<unsigned*>(workspace);
   if (ss::q8_decode_supported(g)) {
-    // A batch with more tokens than rows holds a prompt chunk.  (Block counts of the tiles fit
-    // 31 bits for tables of up to 2^20 columns.)
-    const bool tiles = tokens > bt_rows && bt_cols <= (1 << 20) && ss::q8_prefill_supported(g, device);
+    // A batch with more tokens than rows holds a prompt chunk.  (The tiles count units of at most
+    // 1024 windows in 31 bits.)
+    const bool tiles = tokens > bt_rows && bt_cols * kv_heads < (1LL << 24) &&
+                       ss::q8_prefill_supported(g, device);
     void* states = static_cast<uint8_t*>(workspace) + ss::q8_decode_workspace(device);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    for (int64_t t0 = 0; tiles && t0 < tokens; t0 += ss::q8_prefill_window()) {
-      const int64_t tn = tokens - t0 < ss::q8_prefill_window() ? tokens - t0 : ss::q8_prefill_window();
-      e = ss::launch_q8_prefill(g, t0, tn, device, workspace, states, s);
-      if (e == cudaSuccess) e = ss::launch_q8_merge(g, device, workspace, states, s);
+    // Tiles first: the split-K kernel then takes the SMs as they leave them, and the join of cut
+    // windows comes last.  A batch of several tile launches joins each before the next.
+    const int64_t per = ss::q8_prefill_window();
+    const bool one = tokens <= per;
+    for (int64_t t0 = 0; tiles && t0 < tokens; t0 += per) {
+      e = ss::launch_q8_prefill(g, t0, tokens - t0 < per ? tokens - t0 : per, device, states, s);
+      if (e == cudaSuccess && !one) e = ss::launch_q8_merge(g, device, states, s);
       if (e != cudaSuccess) return cuda_failed(e, "q8 tile attention launch");
-      ss::count_launches(2);
+      ss::count_launches(one ? 1 : 2);
     }
     int launches = 0;
-    e = ss::launch_q8_decode(g, tiles, device, workspace, s, &launches);
+    e = ss::launch_q8_decode(g, tiles, tiles && one, device, workspace, s, &launches);
     ss::count_launches(static_cast<unsigned>(launches));
     if (e != cudaSuccess) return cuda_failed(e, "q8 split-K attention launch");
+    if (tiles && one) {
+      e = ss::launch_q8_merge(g, device, states, s);
+      if (e != cudaSuccess) return cuda_failed(e, "q8 merge launch");
+      ss::count_launches(1);
+    }
     ss::set_last_path(tiles ? 7 : 5);
     return SS_OK;
   }

@@ -110,6 +110,7 @@ struct DecParams {
   Q8AttnArgs g;
   int t0, tn;          // tokens of this launch
   int skip_runs;       // tokens of runs belong to the tile kernel
+  int beside;          // the kernel before is that tile kernel: start beside it, end after it
   int min_chunk;       // fewest units of a CTA
   unsigned* counter;   // [kMaxCtas], zero between calls
   float* part;         // [2 * grid] partial states
@@ -178,7 +179,9 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   const AttnArgs& a = P.g.a;
   const Q8Pool& pool = P.g.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  griddep_wait();
+  // The tile kernel let this one start after its own wait for what came before the call, and
+  // neither reads what the other writes.
+  if (!P.beside) griddep_wait();
   griddep_launch_dependents();
 
   // ---- units before every token ----------------------------------------------------------
@@ -222,7 +225,10 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   }
   const int chunk = max((U + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), P.min_chunk);
   const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
-  if (c0 >= U) return;
+  if (c0 >= U) {
+    if (P.beside) griddep_wait();
+    return;
+  }
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
   // Warps 0 .. nwa - 1 hold at least one unit each.
   const int nwa = min(NW, n_cta), wq = n_cta / nwa, wr = n_cta % nwa;
@@ -615,6 +621,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       }
     }
   }
+  if (P.beside) griddep_wait();
 }
 
 int decode_sms(int device) {
@@ -678,11 +685,12 @@ bool q8_decode_supported(const Q8AttnArgs& g) {
          rows16(a.out, a.o_st, a.o_sh, a.o_sd);
 }
 
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, int device, void* workspace,
-                             cudaStream_t stream, int* launches) {
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, int device,
+                             void* workspace, cudaStream_t stream, int* launches) {
   DecParams p;
   p.g = g;
   p.skip_runs = skip_runs;
+  p.beside = beside;
   p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
   const int sms = decode_sms(device);
@@ -710,6 +718,7 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, int device, vo
 #undef SS_Q8_DECODE
     if (e != cudaSuccess) return e;
     ++*launches;
+    p.beside = 0;  // a second launch waits for the first
   }
   return cudaSuccess;
 }

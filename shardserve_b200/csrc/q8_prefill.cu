@@ -19,22 +19,23 @@
 //   O_t += P_t V_j       kind::tf32, A = P_t from TMEM, B = V_j^T in shared memory
 // in the order S_0(j+1), O_1(j), S_1(j+1), O_0(j+1): each softmax has two products' time.
 // The codes are widened on their way into shared memory: K rows to 128-byte swizzled fp16 lines by
-// three warps, V transposed (lane = key) to lines of 32 keys in fp32 by four, a page's
-// registers being loaded for the next block as soon as it is stored.
+// three warps, V transposed (lane = key) to lines of 32 keys in fp32 by eight (a page
+// of a block each); a page's registers are loaded for the next block as soon as it is stored.
 //
 // The roles' loops are kept rolled and small: with everything unrolled each warp ran at about one
 // instruction in five cycles, the rate at which instructions came from the cache, a key block took
 // 10,000 cycles whatever was taken out of it, and the prompt case 123 us.
 //
-// Scheduling.  Every CTA lists the launch's windows (a scan over its tokens), and cuts a window's
-// blocks into equal parts of at most max(4, all blocks / CTAs): a lone long prompt would otherwise
-// leave most SMs waiting for the last window.  Parts are taken from a counter, cut windows first,
-// then whole ones by length.  Cut windows leave fp32 states in the workspace, joined by
-// q8_merge_kernel.
+// Scheduling.  Every CTA lists the launch's windows (a scan over its tokens) and takes an equal run
+// of the units (window, KV head, block; beginning a window counts as
+// two blocks), so that all finish together; a window that a run's end
+// cuts leaves fp32 states in the workspace, joined by q8_merge_kernel.  (Whole windows taken from
+// a counter, long ones first and the longest cut in two, left 12 to 19 blocks per CTA in the
+// prompt case.)  The roles walk the CTA's run on their own: a producer is in the next window while
+// the softmax warps finish the last.
 //
-// Warps: 0 MMA issuer, 1-3 K, 4-7 V, 8-11 softmax of tile 0, 12-15 of tile 1
-// (TMEM lane quadrant = warp % 4).  setmaxnreg: 512 x 128 = 65,536 registers at launch =
-// 256 x 112 + 256 x 144.
+// Warps: 0 MMA issuer, 1-3 K, 4-11 V, 12-15 softmax of tile 0, 16-19 of tile 1 (TMEM lane quadrant =
+// warp % 4), up to 96 registers a thread.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -51,21 +52,17 @@ namespace ss {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kSoftmaxWarp = 8;    // first softmax warp
-constexpr int kLaunchRegs = 128, kRegsProducer = 112, kRegsSoftmax = 144;
-static_assert(256 * kRegsProducer + 256 * kRegsSoftmax <= kThreads * kLaunchRegs,
-              "setmaxnreg split exceeds the launch register pool");
+constexpr int kThreads = 640;
+constexpr int kVWarp = 4, kSoftmaxWarp = 12;  // first V and softmax warps
 constexpr int kRows = 128;         // rows of a tile
 constexpr int kNB = 128;           // keys of a block
 constexpr int kPages = kNB / kPage;
 constexpr int kMaxTokP = 8192;     // tokens per launch
 constexpr int kMaxWin = kMaxTokP / kQ8MinRun;  // windows per launch
-constexpr int kBins = 256;
-constexpr int kMinPart = 4;        // blocks: smallest cut
+constexpr int kMinPart = 4;        // units: smallest share of a CTA
+constexpr int kHead = 2;           // units that beginning a window costs (Q, first and last waits)
 constexpr float kSlackP = 20.f;
 constexpr int kPolyEvery = 3;      // one exponential pair in 3 on the FMA pipe
-constexpr int kSched = 16;         // workspace words: next part, CTAs done, cut windows
 
 template <int D>
 struct Lay {
@@ -85,23 +82,21 @@ struct CtlQ {
   unsigned long long bar[kNumBars];
   float4 sc[4][kPages];   // per block (mod 4) and page: K scale, log2 and reciprocal of V's
   uint32_t tmem;
-  int item[2];
-  int abort;
-  int nwin, total;        // windows; parts * KV heads
-  int red[2][kThreads / 32];
-  unsigned short first[kMaxWin], count[kMaxWin], order[kMaxWin];
-  int cum[kMaxWin + 1];   // work items before each rank
-  int keys[kMaxWin];
-  int hist[kBins];
+  int red[kThreads / 32];
+  unsigned short first[kMaxWin], count[kMaxWin];
+  int keys[kMaxWin], seq[kMaxWin];
+  int pre[kMaxWin + 1];   // units before each window
 };
 
 struct PrefillParams {
   Q8AttnArgs g;
   int t0, tn;
   int tpt;            // tokens per tile
-  unsigned* sched;    // workspace words kSched ..
-  float* part;        // states of cut windows
-  int4* cuts;         // {first token, tokens, parts, first slot} of each cut window
+  unsigned magic;     // ceil(2^32 / window): x / window = (x * magic) >> 32 for x < 2^13
+  unsigned magic_group;  // the same for the group (0: of one head)
+  float* part;        // [2 * grid] states: of the window begun before the CTA's run, and in it
+  int4* cuts;         // [grid] {first token, tokens, KV head, parts} of the window that the CTA
+                      // begins and leaves unfinished (parts 0: none)
 };
 
 template <int D>
@@ -131,6 +126,18 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t a) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
 }
+
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// 16 bytes from global to shared memory, or 16 zeros (bytes = 0).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Sum and (exclusive) maximum scans over the CTA.
 __device__ __forceinline__ int scan_sum(int v, int* red, int warp, int lane, int& total) {
@@ -193,12 +200,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(kBarPV + t), 1);
       mbar_init(bar(kBarKF + t), 3);
       mbar_init(bar(kBarKE + t), 1);
-      mbar_init(bar(kBarVF + t), 2);
+      mbar_init(bar(kBarVF + t), 4);
       mbar_init(bar(kBarVE + t), 1);
     }
     mbar_init(bar(kBarEnd), 1);
     fence_mbar_init();
-    ctl->abort = 0;
   }
   if (warp == 0) {
     tmem_alloc(smem_u32(&ctl->tmem), 512);
@@ -206,41 +212,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   griddep_wait();
   griddep_launch_dependents();
-  const int first_item = tid == 0 ? static_cast<int>(atomicAdd(P.sched, 1u)) : 0;
 
   // ---- the windows of this launch ----------------------------------------------------------
-  for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
-  for (int i = tid; i < kBins; i += kThreads) ctl->hist[i] = 0;
+  int nwin, units;
   {
     // The operand buffers are idle: the staged ids and lengths stand there.
     int* const seq = reinterpret_cast<int*>(smem) + kQ8Pad;
     int* const len = seq + kMaxTokP + kQ8Pad;
+    for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
     stage_tokens(a, P.t0, P.tn, seq, len, blockIdx.x == 0);
     __syncthreads();
     const int per = (P.tn + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
-    auto in_run = [&](int i) { return in_staged_run(seq, i); };
     auto starts = [&](int i) { return i == 0 || seq[i - 1] != seq[i]; };
+    // Token i of the run that starts at `start` (as far as this launch sees).
+    auto in_run = [&](int i, int start) { return i - start >= kQ8Pad || in_staged_run(seq, i); };
+    auto place = [&](int x) { return x - tw * static_cast<int>(__umulhi(static_cast<unsigned>(x), P.magic)); };
     int start = -1;  // last run start at or before a token
     for (int i = b0; i < b1; ++i)
       if (starts(i)) start = i;
-    const int before = scan_max(start, ctl->red[0], warp, lane);
+    const int before = scan_max(start, ctl->red, warp, lane);
     start = before;
     int n = 0;
     for (int i = b0; i < b1; ++i) {
       if (starts(i)) start = i;
-      if ((i - start) % tw == 0 && in_run(i)) ++n;
+      if (place(i - start) == 0 && in_run(i, start)) ++n;
     }
-    int nwin;
-    int idx = scan_sum(n, ctl->red[1], warp, lane, nwin) - 1;
+    int idx = scan_sum(n, ctl->red, warp, lane, nwin) - 1;
     start = before;
     int most_keys = 0;  // of this thread's tokens of window idx
     for (int i = b0; i < b1; ++i) {
       if (starts(i)) start = i;
-      if (!in_run(i)) continue;
-      const int at = (i - start) % tw;
+      if (!in_run(i, start)) continue;
+      const int at = place(i - start);
       if (at == 0) {
         ctl->first[++idx] = static_cast<unsigned short>(i);
+        ctl->seq[idx] = seq[i];
         most_keys = 0;
       }
       most_keys = max(most_keys, len[i]);
@@ -249,134 +256,80 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ends || i + 1 == b1) atomicMax(&ctl->keys[idx], most_keys);
     }
     __syncthreads();
-    // Blocks of every window; the largest part, and the order in which parts are taken.
-    int sum = 0;
-    for (int w = tid; w < nwin; w += kThreads) sum += (ctl->keys[w] + kNB - 1) / kNB;
-    int all;
-    scan_sum(sum, ctl->red[0], warp, lane, all);
-    const long long each = (static_cast<long long>(all) * a.KVH + gridDim.x - 1) / gridDim.x;
-    const int most = static_cast<int>(max(each, static_cast<long long>(kMinPart)));
-    auto bin_of = [&](int w) {  // 0 first: cut windows, then whole ones from long to short
-      const int nb = (ctl->keys[w] + kNB - 1) / kNB;
-      return nb > most ? 0 : kBins - 1 - min(nb, kBins - 2);
-    };
-    for (int w = tid; w < nwin; w += kThreads) atomicAdd(&ctl->hist[bin_of(w)], 1);
-    __syncthreads();
-    if (warp == 0) {
-      int local = 0;
+    auto units_of = [](int keys) { return keys > 0 ? (keys + kNB - 1) / kNB + kHead : 0; };
+    constexpr int kPer = (kMaxWin + kThreads - 1) / kThreads;
+    int blocks = 0;
 #pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) local += ctl->hist[lane * (kBins / 32) + i];
-      int inc = local;
+    for (int k = 0; k < kPer; ++k) {
+      const int w = tid * kPer + k;
+      if (w < nwin) blocks += units_of(ctl->keys[w]);
+    }
+    int run = scan_sum(blocks * a.KVH, ctl->red, warp, lane, units);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      int run = inc - local;
-#pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) {
-        const int b = lane * (kBins / 32) + i, h = ctl->hist[b];
-        ctl->hist[b] = run;
-        run += h;
-      }
-      __syncwarp();
-      for (int base = 0; base < nwin; base += 32) {  // stable: every CTA builds the same order
-        const int w = base + lane;
-        const int b = w < nwin ? bin_of(w) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, b);
-        if (w < nwin) ctl->order[ctl->hist[b] + __popc(same & ((1u << lane) - 1u))] = static_cast<unsigned short>(w);
-        __syncwarp();
-        if (w < nwin && lane == __ffs(same) - 1) ctl->hist[b] += __popc(same);
-        __syncwarp();
-      }
-      // Work items before each rank; parts are equal shares of at most `most` blocks.
-      int carry = 0, cuts = 0;
-      for (int base = 0; base < nwin; base += 32) {
-        const int r = base + lane;
-        int parts = 0, w = 0;
-        if (r < nwin) {
-          w = ctl->order[r];
-          const int nb = (ctl->keys[w] + kNB - 1) / kNB;
-          parts = nb > most ? (nb + most - 1) / most : 1;
-        }
-        int inc2 = parts * a.KVH;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc2, o);
-          if (lane >= o) inc2 += x;
-        }
-        if (r < nwin) ctl->cum[r] = carry + inc2 - parts * a.KVH;
-        if (blockIdx.x == 0 && parts > 1)
-          P.cuts[r] = make_int4(P.t0 + ctl->first[w], ctl->count[w], parts, carry + inc2 - parts * a.KVH);
-        cuts += __popc(__ballot_sync(0xffffffffu, parts > 1));
-        carry += __shfl_sync(0xffffffffu, inc2, 31);
-      }
-      if (lane == 0) {
-        ctl->cum[nwin] = carry;
-        ctl->nwin = nwin;
-        ctl->total = carry;
-        if (blockIdx.x == 0) P.sched[2] = static_cast<unsigned>(cuts);
+    for (int k = 0; k < kPer; ++k) {
+      const int w = tid * kPer + k;
+      if (w < nwin) {
+        ctl->pre[w] = run;
+        run += units_of(ctl->keys[w]) * a.KVH;
       }
     }
+    if (tid == 0) ctl->pre[nwin] = units;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const int nwin = ctl->nwin, total = ctl->total;
+  const int share = max((units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinPart);
+  const int u0 = min(static_cast<long long>(blockIdx.x) * share, static_cast<long long>(units));
+  const int u1 = min(u0 + static_cast<long long>(share), static_cast<long long>(units));
 
   int jg = 0;      // blocks processed so far by this CTA (phases of the K and V barriers)
   // Phases of a tile's own barriers: tile 1 sits out windows that fill one tile only.
   int jt[2] = {0, 0}, qt[2] = {0, 0};  // blocks and windows of each tile so far
   bool ok = true;
-  int iter = 0;
   struct Item {
-    bool live;
-    int first, count, kvh, j0, j1, keys, slot;  // slot < 0: the window is whole
-    long long seq;
+    int win, first, count, kvh, j0, j1, keys, nb, len;
   };
-  auto next_item = [&]() -> Item {
-    if (tid == 0) ctl->item[iter & 1] = iter == 0 ? first_item : static_cast<int>(atomicAdd(P.sched, 1u));
-    named_bar_sync(1, kThreads);
-    const int w = ctl->item[iter & 1];
-    ++iter;
+  // The part of a window and KV head that unit u stands in, as far as this CTA's run goes.
+  auto item_at = [&](int u, int win) -> Item {
     Item it;
-    it.live = w < total && !ctl->abort;
-    if (!it.live) return it;
-    int lo = 0, hi = nwin;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (ctl->cum[mid] <= w) lo = mid; else hi = mid;
-    }
-    const int win = ctl->order[lo], rest = w - ctl->cum[lo], parts = (ctl->cum[lo + 1] - ctl->cum[lo]) / a.KVH;
+    while (ctl->pre[win + 1] <= u) ++win;
+    it.win = win;
     it.first = ctl->first[win];
     it.count = ctl->count[win];
     it.keys = ctl->keys[win];
-    it.kvh = rest / parts;
-    const int p = rest - it.kvh * parts, nb = (it.keys + kNB - 1) / kNB;
-    it.j0 = static_cast<int>(static_cast<long long>(nb) * p / parts);
-    it.j1 = static_cast<int>(static_cast<long long>(nb) * (p + 1) / parts);
-    it.slot = parts > 1 ? w : -1;
-    it.seq = ld_index(a.seq, a.seq64, P.t0 + it.first);
+    it.nb = (it.keys + kNB - 1) / kNB;
+    const int n = it.nb + kHead, rest = u - ctl->pre[win];
+    it.kvh = rest / n;
+    const int x0 = rest - it.kvh * n, x1 = min(n, x0 + u1 - u);
+    it.len = x1 - x0;
+    it.j0 = max(x0 - kHead, 0);
+    it.j1 = max(x1 - kHead, 0);
     return it;
   };
-  auto timed_out = [&]() {
-    if (lane == 0) {
-      atomicOr(a.err, SS_DEVERR_TIMEOUT);
-      ctl->abort = 1;
+  int win0 = 0;  // window of the run's first unit
+  if (u0 < u1) {
+    int hi = nwin;
+    while (hi - win0 > 1) {
+      const int mid = (win0 + hi) >> 1;
+      if (ctl->pre[mid] <= u0) win0 = mid; else hi = mid;
     }
+  }
+  auto timed_out = [&]() {
+    if (lane == 0) atomicOr(a.err, SS_DEVERR_TIMEOUT);
   };
 
   if (warp < kSoftmaxWarp) {
-    setmaxnreg_dec<kRegsProducer>();
     if (warp == 0) {
       // ================================= MMA issuer ====================================
       constexpr uint32_t id_qk = idesc_of(0, kNB), id_pv = idesc_of(2, D);
       const bool leader = elect_one();
-      for (;;) {
-        const Item it = next_item();
-        if (!it.live) break;
+      for (int u = u0, win = win0; u < u1 && ok;) {
+        const Item it = item_at(u, win);
         const int nblk = it.j1 - it.j0;
+        u += it.len;
+        win = it.win;
+        if (nblk == 0) continue;
         const bool two = it.count > P.tpt;  // both tiles hold tokens
         auto qk = [&](int t, int st) {
           if (leader) {
@@ -420,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           return true;
         };
-        if (nblk > 0) {
+        {
           ok = wait_warp(bar(kBarQ), qt[0] & 1);
           if (ok && two) ok = wait_warp(bar(kBarQ + 1), qt[1] & 1);
           for (int j = 0; j < nblk && ok; ++j) {
@@ -454,19 +407,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait_warp(bar(kBarEnd), 0)) timed_out();
     } else {
       // ================================== producers ====================================
-      const bool is_v = warp >= 4;
+      const bool is_v = warp >= kVWarp;
       // Page ids and scales of a block's 8 pages: lanes 0-7.  id -1: past the keys or outside the
       // pool.
-      for (;;) {
-        const Item it = next_item();
-        if (!it.live) break;
+      for (int u = u0, win = win0; u < u1 && ok;) {
+        const Item it = item_at(u, win);
         const int nblk = it.j1 - it.j0;
-        if (nblk <= 0) continue;
+        u += it.len;
+        win = it.win;
+        if (nblk == 0) continue;
+        const long long bt_row = static_cast<long long>(ctl->seq[it.win]) * a.bt_sb;
         const float* sbase = pool.scales + static_cast<long long>(it.kvh) * pool.s_sh;
         auto load_id = [&](int j) -> int {
           const int pi = (it.j0 + j) * kPages + lane;
           if (j >= nblk || lane >= kPages || pi * kPage >= it.keys) return -1;
-          const long long id = ld_index(a.bt, a.bt64, it.seq * a.bt_sb + pi * a.bt_sn);
+          const long long id = ld_index(a.bt, a.bt64, bt_row + pi * a.bt_sn);
           if (id >= 0 && id < pool.N) return static_cast<int>(id);
           atomicOr(a.err, SS_DEVERR_PAGE);
           return -1;
@@ -540,32 +495,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(bar(kBarKF + st));
           }
         } else {
-          // Warp 4 + 2 h + u widens pages 4 h + 2 u and the one after.  Load (p, i): 16 keys (lane %
-          // 16) of page p x 32 values (32 i + 16 (lane / 16)).
-          const int h = (warp - 4) >> 1, u = warp & 1, key = lane & 15, hi = lane >> 4;
+          // Warp 4 + 4 h + u widens page u of half h of every block.  Load i: 16 keys (lane % 16) x
+          // 32 values (32 i + 16 (lane / 16)).
+          const int h = (warp - kVWarp) >> 2, u = warp & 3, key = lane & 15, hi = lane >> 4;
           const uint8_t* base = pool.v + static_cast<long long>(it.kvh) * pool.v_sh + key * pool.v_ss + 16 * hi;
           // Line of value 16 hi + k (k = 0 .. 15), this lane's key.  The upper lanes take their values
           // in the order k ^ 4, which puts the two half-warps' stores into different banks.
           uint32_t at[8];
 #pragma unroll
           for (int m = 0; m < 8; ++m)
-            at[m] = sb + L::kOffV + h * L::kV + u * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
-                    ((((key >> 2) ^ (4 * hi)) ^ m) << 4) + (key & 3) * 4;
-          auto load = [&](int j, int p, uint4 (&v)[D / 32]) {
-            const int pg = 4 * h + 2 * u + p;
-            const int pid = __shfl_sync(0xffffffffu, id, pg);
-            const float vs = __shfl_sync(0xffffffffu, scl.y, pg);
-            const int left = pid < 0 || !(vs >= kMinVs) ? 0 : it.keys - ((it.j0 + j) * kPages + pg) * kPage;
+            at[m] = sb + L::kOffV + h * L::kV + (u >> 1) * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
+                    ((((u & 1) * 4 + (key >> 2)) ^ (4 * hi) ^ m) << 4) + (key & 3) * 4;
+          uint4 buf[D / 32];
+          auto load = [&](int j) {
+            const int pid = __shfl_sync(0xffffffffu, id, 4 * h + u);
+            const float vs = __shfl_sync(0xffffffffu, scl.y, 4 * h + u);
+            const int left = pid < 0 || !(vs >= kMinVs) ? 0 : it.keys - ((it.j0 + j) * kPages + 4 * h + u) * kPage;
             const uint8_t* src = base + static_cast<long long>(max(pid, 0)) * pool.v_sn;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-              v[i] = make_uint4(0, 0, 0, 0);
-              if (key < left) v[i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
+              buf[i] = make_uint4(0, 0, 0, 0);
+              if (key < left) buf[i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
             }
           };
-          uint4 buf[2][D / 32];
-          load(0, 0, buf[0]);
-          load(0, 1, buf[1]);
+          load(0);
           for (int j = 0; j < nblk; ++j) {
             const int jb = jg + j;
             id = id_next;
@@ -574,25 +527,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = wait_warp(bar(kBarVE + h), (jb & 1) ^ 1);
             if (!ok) break;
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
+            for (int i = 0; i < D / 32; ++i) {
+              const uint4 v = buf[i];
+              const uint32_t w[4] = {hi ? v.y : v.x, hi ? v.x : v.y, hi ? v.w : v.z, hi ? v.z : v.w};
 #pragma unroll
-              for (int i = 0; i < D / 32; ++i) {
-                const uint4 v = buf[p][i];
-                const uint32_t w[4] = {hi ? v.y : v.x, hi ? v.x : v.y, hi ? v.w : v.z, hi ? v.z : v.w};
+              for (int q = 0; q < 4; ++q) {
+                uint32_t f[4];
+                widen_f32<FMT>(w[q], f);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  uint32_t f[4];
-                  widen_f32<FMT>(w[q], f);
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)  // page 1: the other half of the line
-                    st_shared4((at[(4 * q + e) & 7] ^ (64 * p)) + i * (32 * 128) + (4 * q + e) * 128, f[e]);
-                }
+                for (int e = 0; e < 4; ++e)
+                  st_shared4(at[(4 * q + e) & 7] + i * (32 * 128) + (4 * q + e) * 128, f[e]);
               }
-              load(j + 1, p, buf[p]);  // in flight until the next block
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kBarVF + h));
+            load(j + 1);  // in flight until the next block
           }
         }
         if (!ok) timed_out();
@@ -600,61 +550,158 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    setmaxnreg_inc<kRegsSoftmax>();
     const int tt = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + tt * kNB + lane_off, tO = tmem + 256 + tt * 128 + lane_off;
     const int rt = row / a.group, rh = row - rt * a.group;  // token inside the tile, head
-    for (;;) {
-      const Item it = next_item();
-      if (!it.live) break;
-      const int nblk = it.j1 - it.j0;
-      const int wt = tt * P.tpt + rt;  // token inside the window
-      const bool mine = rt < P.tpt && wt < it.count;
-      const long long t = P.t0 + it.first + wt;
-      __nv_bfloat16* op = a.out + t * a.o_st + static_cast<long long>(it.kvh * a.group + rh) * a.o_sh;
-      if (nblk == 0) {  // no row of the window has keys
-        if (mine)
-          for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
-        continue;
+    // Windows without keys: zero rows.
+    for (int w = blockIdx.x; w < nwin; w += gridDim.x) {
+      if (ctl->keys[w] != 0) continue;
+      for (int e = tid - 32 * kSoftmaxWarp; e < ctl->count[w] * a.H * (D / 8); e += 256) {
+        const int d = e % (D / 8) * 8, h = e / (D / 8) % a.H, i = e / (D / 8) / a.H;
+        *reinterpret_cast<uint4*>(a.out + (P.t0 + ctl->first[w] + i) * a.o_st + h * a.o_sh + d) = make_uint4(0, 0, 0, 0);
       }
-      const bool active = tt == 0 || it.count > P.tpt;
-      if (active) {
-        const int lim = mine ? q8_token_info(a, t, false).L : INT_MAX;  // others compute unmasked
-        // ---- this row of Q, as fp16 with its power of two taken out ----------------------
-        float f_row;
-        {
-          uint32_t raw[D / 2];
-          const __nv_bfloat16* qp = a.q + t * a.q_st + static_cast<long long>(it.kvh * a.group + rh) * a.q_sh;
-          float amax = 0.f;
+    }
+    if (warp == kSoftmaxWarp && lane == 0) {  // the window that this run begins and does not finish
+      int4 cut = make_int4(0, 0, 0, 0);
+      if (u0 < u1) {
+        int win = win0;
+        while (ctl->pre[win + 1] < u1) ++win;
+        const int n = (ctl->keys[win] + kNB - 1) / kNB + kHead, kvh = (u1 - 1 - ctl->pre[win]) / n;
+        const int begin = ctl->pre[win] + kvh * n + kHead, end = begin + n - kHead;  // its blocks
+        if (begin >= u0 && begin < u1 && end > u1)
+          cut = make_int4(P.t0 + ctl->first[win], ctl->count[win], kvh, (end - 1) / share - static_cast<int>(blockIdx.x) + 1);
+      }
+      P.cuts[blockIdx.x] = cut;
+    }
+    // An item's Q is loaded before the epilogue of the one before it: the product of its first block
+    // then runs beside that epilogue.
+    Item it, cur;
+    bool have = false;  // cur's blocks are done, its epilogue is not
+    float ref = 0.f, lsum = 0.f, f_row = 0.f;
+    auto takes = [&](const Item& i) { return tt == 0 || i.count > P.tpt; };  // this tile holds tokens
+    auto is_mine = [&](const Item& i) { return rt < P.tpt && tt * P.tpt + rt < i.count; };
+    for (int u = u0, win = win0; ok;) {
+      bool more = false;
+      while (u < u1 && !more) {
+        it = item_at(u, win);
+        u += it.len;
+        win = it.win;
+        more = it.j1 > it.j0;
+      }
+      long long my_seq = 0, my_pos = 0;
+      float f_next = 0.f;
+      if (more && takes(it)) {
+        const long long tc = P.t0 + it.first + (is_mine(it) ? tt * P.tpt + rt : 0);
+        my_seq = ld_index(a.seq, a.seq64, tc);
+        my_pos = ld_index(a.pos, a.pos64, tc);
+        // ---- 32 rows of Q per warp, D / 8 lanes each 16 bytes of a row: copied to their place, then
+        // turned there into fp16 with the row's power of two taken out.
+        constexpr int LR = D / 8, RP = 32 / LR;  // lanes of a row, rows of a step
+        const int c = lane % LR, r0 = (warp & 3) * 32 + lane / LR;
+        const __nv_bfloat16* qb = a.q + (P.t0 + it.first + tt * P.tpt) * a.q_st +
+                                  static_cast<long long>(it.kvh * a.group) * a.q_sh + 8 * c;
+        const int left = min(it.count - tt * P.tpt, P.tpt);  // tokens of this tile
+        const uint32_t dst = sb + tt * L::kQ + (c >> 3) * (kRows * 128);
+        auto at = [&](int r) { return dst + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+#pragma unroll 1
+        for (int r = r0; r < r0 + 32; r += RP) {
+          const int tok = a.group == 1 ? r : static_cast<int>(__umulhi(static_cast<unsigned>(r), P.magic_group));
+          const int hd = r - tok * a.group;
+          cp_async16(at(r), tok < left ? qb + tok * a.q_st + hd * a.q_sh : a.q, tok < left ? 16 : 0);
+        }
+        cp_async_wait_all();
+#pragma unroll 1
+        for (int n0 = 0; n0 < 32 / RP; n0 += 4) {
+          uint4 v[4];
+          float amax[4];
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine) v = __ldg(reinterpret_cast<const uint4*>(qp) + c);
-            raw[4 * c] = v.x; raw[4 * c + 1] = v.y; raw[4 * c + 2] = v.z; raw[4 * c + 3] = v.w;
+          for (int n = 0; n < 4; ++n) {
+            v[n] = ld_shared16(at(r0 + (n0 + n) * RP));
+            const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+            amax[n] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              amax[n] = fmaxf(amax[n], fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
           }
 #pragma unroll
-          for (int c = 0; c < D / 2; ++c)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[c] << 16)),
-                                     fabsf(__uint_as_float(raw[c] & 0xffff0000u))));
-          const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
-          // A negative sm_scale changes q's sign, so that the factor of the scores is >= 0.
-          const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), a.scale_log2);
-          f_row = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(a.scale_log2);
-          const uint32_t line = sb + tt * L::kQ + row * 128;
+          for (int o = 1; o < LR; o <<= 1)
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
+            for (int n = 0; n < 4; ++n) amax[n] = fmaxf(amax[n], __shfl_xor_sync(0xffffffffu, amax[n], o));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+            const int e = min(max(static_cast<int>(__float_as_uint(amax[n]) >> 23) - 127, -126), 126);
+            // A negative sm_scale changes q's sign, so that the factor of the scores is >= 0.
+            const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), a.scale_log2);
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              h[k] = pack_f16(__uint_as_float(raw[4 * c + k] << 16) * down,
-                              __uint_as_float(raw[4 * c + k] & 0xffff0000u) * down);
-            st_shared16(line + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+              h[k] = pack_f16(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down);
+            st_shared16(at(r0 + (n0 + n) * RP), h[0], h[1], h[2], h[3]);
+            const float f = __shfl_sync(0xffffffffu, __uint_as_float(static_cast<uint32_t>(127 + e) << 23), (lane % RP) * LR);
+            if (lane / RP == n0 + n) f_next = f * fabsf(a.scale_log2);  // the row this lane computes
           }
-          fence_proxy_async_smem();
-          mbar_arrive(bar(kBarQ + tt));
         }
-        float ref = -CUDART_INF_F, lsum = 0.f;
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kBarQ + tt));
+      }
+      if (have) {
+        // ---- O_t / l of the item before, or the state of a cut window ---------------------
+        const bool whole = cur.j1 - cur.j0 == cur.nb, mine = is_mine(cur);
+        float* const state = P.part + (2ll * blockIdx.x + (cur.j0 == 0 ? 1 : 0)) * State<D>::kFloats;
+        __nv_bfloat16* op = a.out + (P.t0 + cur.first + tt * P.tpt + rt) * a.o_st +
+                            static_cast<long long>(cur.kvh * a.group + rh) * a.o_sh;
+        ok = wait_warp(bar(kBarPV + tt), (jt[0] - 1) & 1);
+        if (ok) {
+          tc_fence_after();
+          // A row whose keys are all masked never got a reference (and its weights are not sums of
+          // exact zeros where the polynomial made them).
+          if (ref == -CUDART_INF_F) lsum = 0.f;
+          const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+          float4* st = reinterpret_cast<float4*>(state) + tt * kRows + row;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+            if (!whole) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                __stcg(st + (c * 8 + i) * 256,
+                       make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+            } else if (mine) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint4 v;
+                v.x = pack_bf16(__uint_as_float(o[q * 8 + 0]) * inv, __uint_as_float(o[q * 8 + 1]) * inv);
+                v.y = pack_bf16(__uint_as_float(o[q * 8 + 2]) * inv, __uint_as_float(o[q * 8 + 3]) * inv);
+                v.z = pack_bf16(__uint_as_float(o[q * 8 + 4]) * inv, __uint_as_float(o[q * 8 + 5]) * inv);
+                v.w = pack_bf16(__uint_as_float(o[q * 8 + 6]) * inv, __uint_as_float(o[q * 8 + 7]) * inv);
+                *reinterpret_cast<uint4*>(op + c * 32 + q * 8) = v;
+              }
+            }
+          }
+          if (!whole) {
+            float* rl = state + 256 * D + tt * kRows + row;
+            __stcg(rl, ref);
+            __stcg(rl + 256, lsum);
+          }
+        }
+        if (!ok) break;
+        tc_fence_before();
+      }
+      if (!more) break;
+      cur = it;
+      have = takes(it);
+      const int nblk = it.j1 - it.j0;
+      if (have) {
+        // Rows past the window compute unmasked.
+        const int lim = !is_mine(it) ? INT_MAX : my_seq == -1 ? 0 : token_info_from(a, my_seq, my_pos, false).L;
+        f_row = f_next;
+        ref = -CUDART_INF_F;
+        lsum = 0.f;
         for (int j = 0; j < nblk; ++j) {
           const int jb = jt[0] + j;  // this tile's blocks so far
           ok = wait_warp(bar(kBarS + tt), jb & 1);
@@ -751,62 +798,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           lsum = lsum * alpha + part;
         }
-        // ---- O_t / l, or the state of a cut window ----------------------------------------
-        if (ok) ok = wait_warp(bar(kBarPV + tt), (jt[0] + nblk - 1) & 1);
-        if (ok) {
-          tc_fence_after();
-          // A row whose keys are all masked never got a reference (and its weights are not sums of
-          // exact zeros where the polynomial made them).
-          if (ref == -CUDART_INF_F) lsum = 0.f;
-          const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-          float4* st = reinterpret_cast<float4*>(P.part + static_cast<long long>(it.slot) * State<D>::kFloats) + tt * kRows + row;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
-            tmem_wait_ld();
-            if (it.slot >= 0) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                __stcg(st + (c * 8 + i) * 256,
-                       make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
-            } else if (mine) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint4 v;
-                v.x = pack_bf16(__uint_as_float(o[q * 8 + 0]) * inv, __uint_as_float(o[q * 8 + 1]) * inv);
-                v.y = pack_bf16(__uint_as_float(o[q * 8 + 2]) * inv, __uint_as_float(o[q * 8 + 3]) * inv);
-                v.z = pack_bf16(__uint_as_float(o[q * 8 + 4]) * inv, __uint_as_float(o[q * 8 + 5]) * inv);
-                v.w = pack_bf16(__uint_as_float(o[q * 8 + 6]) * inv, __uint_as_float(o[q * 8 + 7]) * inv);
-                *reinterpret_cast<uint4*>(op + c * 32 + q * 8) = v;
-              }
-            }
-          }
-          if (it.slot >= 0) {
-            float* rl = P.part + static_cast<long long>(it.slot) * State<D>::kFloats + 256 * D + tt * kRows + row;
-            __stcg(rl, ref);
-            __stcg(rl + 256, lsum);
-          }
-        }
-        if (!ok) timed_out();
-        tc_fence_before();
         jt[0] += nblk;
       }
       jg += nblk;
     }
+    if (!ok) timed_out();
   }
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
-  }
-  if (tid == 0) {  // the last CTA out returns the counters to zero
-    __threadfence();
-    if (atomicAdd(P.sched + 1, 1u) == gridDim.x - 1) {
-      P.sched[0] = 0;
-      P.sched[1] = 0;
-    }
   }
 }
 
@@ -815,21 +816,23 @@ template <int D>
 __global__ void __launch_bounds__(256) q8_merge_kernel(const PrefillParams P) {
   griddep_wait();
   const AttnArgs& a = P.g.a;
-  const int cuts = static_cast<int>(P.sched[2]);
-  const int per_win = a.KVH * (D / 16);  // blocks of 256 rows
-  for (int b = blockIdx.x; b < cuts * per_win; b += gridDim.x) {
-    const int4 cut = P.cuts[b / per_win];
-    const int rest = b % per_win, h = rest / (D / 16), c = rest % (D / 16);
+  const int cta = blockIdx.x / (D / 16), c = blockIdx.x % (D / 16);
+  const int4 cut = P.cuts[cta];
+  {
+    const int parts = cut.w;
+    if (parts == 0) return;
     const int row = threadIdx.x, tile = row / kRows, r = row % kRows;
     const int rt = r / a.group, rh = r - rt * a.group, wt = tile * P.tpt + rt;
-    if (rt >= P.tpt || wt >= cut.y) continue;
-    const float* s0 = P.part + (static_cast<long long>(cut.w) + h * cut.z) * State<D>::kFloats;
+    if (rt >= P.tpt || wt >= cut.y) return;
+    // Part 0 is the state of the window that the CTA begins, the others those that the following
+    // CTAs found begun.
+    auto state = [&](int p) { return P.part + (2ll * (cta + p) + (p == 0 ? 1 : 0)) * State<D>::kFloats; };
     float ref = -CUDART_INF_F, l = 0.f;
-    for (int p = 0; p < cut.z; ++p) ref = fmaxf(ref, __ldcg(s0 + p * static_cast<long long>(State<D>::kFloats) + 256 * D + row));
+    for (int p = 0; p < parts; ++p) ref = fmaxf(ref, __ldcg(state(p) + 256 * D + row));
     const float base = ref == -CUDART_INF_F ? 0.f : ref;
     float4 o[4] = {};
-    for (int p = 0; p < cut.z; ++p) {
-      const float* s = s0 + p * static_cast<long long>(State<D>::kFloats);
+    for (int p = 0; p < parts; ++p) {
+      const float* s = state(p);
       const float w = ex2(__ldcg(s + 256 * D + row) - base);
       l += w * __ldcg(s + 256 * D + 256 + row);
 #pragma unroll
@@ -840,7 +843,7 @@ __global__ void __launch_bounds__(256) q8_merge_kernel(const PrefillParams P) {
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<long long>(cut.x + wt) * a.o_st +
-                                          static_cast<long long>(h * a.group + rh) * a.o_sh + c * 16);
+                                          static_cast<long long>(cut.z * a.group + rh) * a.o_sh + c * 16);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       dst[k] = make_uint4(pack_bf16(o[2 * k].x * inv, o[2 * k].y * inv), pack_bf16(o[2 * k].z * inv, o[2 * k].w * inv),
@@ -870,11 +873,8 @@ bool prepare_one(int device) {
   static std::once_flag once[64];
   static bool fine[64];
   std::call_once(once[device], [&] {
-    cudaFuncAttributes fa;
     fine[device] = cudaFuncSetAttribute(q8_prefill_kernel<D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(prefill_smem<D>())) == cudaSuccess &&
-                   cudaFuncGetAttributes(&fa, q8_prefill_kernel<D, FMT>) == cudaSuccess &&
-                   fa.numRegs == kLaunchRegs;  // the setmaxnreg split counts on it
+                                        static_cast<int>(prefill_smem<D>())) == cudaSuccess;
   });
   return fine[device];
 }
@@ -897,11 +897,8 @@ cudaError_t launch_chained(void (*kernel)(Args...), int grid, int threads, size_
 
 }  // namespace
 
-// The states: windows are cut into parts of at least 1 / CTAs of all blocks, and a cut window has
-// less than one part more than its share, so at most 2 * CTAs parts need a state.
 size_t q8_prefill_workspace(int device) {
-  return 2 * static_cast<size_t>(prefill_sms(device)) * State<128>::kFloats * sizeof(float) +
-         sizeof(int4) * kMaxWin;
+  return static_cast<size_t>(prefill_sms(device)) * (2 * State<128>::kFloats * sizeof(float) + sizeof(int4));
 }
 
 bool q8_prefill_supported(const Q8AttnArgs& g, int device) {
@@ -912,16 +909,17 @@ bool q8_prefill_supported(const Q8AttnArgs& g, int device) {
 }
 
 cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
-                              void* workspace, void* states, cudaStream_t stream) {
+                              void* states, cudaStream_t stream) {
   PrefillParams p;
   p.g = g;
   p.t0 = static_cast<int>(t0);
   p.tn = static_cast<int>(tn);
   p.tpt = kRows / g.a.group;
-  p.sched = static_cast<unsigned*>(workspace) + kSched;
-  p.cuts = static_cast<int4*>(states);
-  p.part = reinterpret_cast<float*>(p.cuts + kMaxWin);
   const int grid = prefill_sms(device);
+  p.magic = static_cast<unsigned>(((1ull << 32) + 2 * p.tpt - 1) / (2 * p.tpt));
+  p.magic_group = static_cast<unsigned>(((1ull << 32) + g.a.group - 1) / g.a.group);
+  p.part = static_cast<float*>(states);
+  p.cuts = reinterpret_cast<int4*>(p.part + 2ll * grid * State<128>::kFloats);
   const bool i8 = g.p.fmt == SS_CODE_INT8;
   if (g.p.D == 128)
     return i8 ? launch_chained(q8_prefill_kernel<128, SS_CODE_INT8>, grid, kThreads, prefill_smem<128>(), stream, p)
@@ -930,16 +928,16 @@ cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, i
             : launch_chained(q8_prefill_kernel<64, SS_CODE_E4M3>, grid, kThreads, prefill_smem<64>(), stream, p);
 }
 
-cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* workspace, void* states,
+cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* states,
                             cudaStream_t stream) {
   PrefillParams p;
   p.g = g;
   p.t0 = p.tn = 0;
   p.tpt = kRows / g.a.group;
-  p.sched = static_cast<unsigned*>(workspace) + kSched;
-  p.cuts = static_cast<int4*>(states);
-  p.part = reinterpret_cast<float*>(p.cuts + kMaxWin);
-  const int grid = 4 * prefill_sms(device);
+  p.magic = p.magic_group = 0;
+  const int ctas = prefill_sms(device), grid = ctas * (g.p.D / 16);
+  p.part = static_cast<float*>(states);
+  p.cuts = reinterpret_cast<int4*>(p.part + 2ll * ctas * State<128>::kFloats);
   return g.p.D == 128 ? launch_chained(q8_merge_kernel<128>, grid, 256, 0, stream, p)
                       : launch_chained(q8_merge_kernel<64>, grid, 256, 0, stream, p);
 }
