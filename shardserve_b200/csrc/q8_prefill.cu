@@ -58,6 +58,7 @@ constexpr int kRows = 128;         // rows of a tile
 constexpr int kNB = 128;           // keys of a block
 constexpr int kPages = kNB / kPage;
 constexpr int kMaxTokP = 8192;     // tokens per launch
+static_assert((kMaxTokP + kThreads - 1) / kThreads <= 32, "a thread's tokens fit a mask");
 constexpr int kMaxWin = kMaxTokP / kQ8MinRun;  // windows per launch
 constexpr int kMinPart = 4;        // units: smallest share of a CTA
 constexpr int kHead = 2;           // units that beginning a window costs (Q, first and last waits)
@@ -219,7 +220,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The operand buffers are idle: the staged ids and lengths stand there.
     int* const seq = reinterpret_cast<int*>(smem) + kQ8Pad;
     int* const len = seq + kMaxTokP + kQ8Pad;
-    for (int i = tid; i < kMaxWin; i += kThreads) ctl->keys[i] = 0;
     stage_tokens(a, P.t0, P.tn, seq, len, blockIdx.x == 0);
     __syncthreads();
     const int per = (P.tn + kThreads - 1) / kThreads;
@@ -233,27 +233,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (starts(i)) start = i;
     const int before = scan_max(start, ctl->red, warp, lane);
     start = before;
-    int n = 0;
+    unsigned begins = 0;  // tokens of this thread that begin a window (at most 13 tokens a thread)
     for (int i = b0; i < b1; ++i) {
       if (starts(i)) start = i;
-      if (place(i - start) == 0 && in_run(i, start)) ++n;
+      if (place(i - start) == 0 && in_run(i, start)) begins |= 1u << (i - b0);
     }
-    int idx = scan_sum(n, ctl->red, warp, lane, nwin) - 1;
-    start = before;
-    int most_keys = 0;  // of this thread's tokens of window idx
-    for (int i = b0; i < b1; ++i) {
-      if (starts(i)) start = i;
-      if (!in_run(i, start)) continue;
-      const int at = place(i - start);
-      if (at == 0) {
-        ctl->first[++idx] = static_cast<unsigned short>(i);
-        ctl->seq[idx] = seq[i];
-        most_keys = 0;
+    int idx = scan_sum(__popc(begins), ctl->red, warp, lane, nwin);
+    for (; begins; begins &= begins - 1) ctl->first[idx++] = static_cast<unsigned short>(b0 + __ffs(begins) - 1);
+    __syncthreads();
+    // One warp per window: its tokens, and the keys that they attend.
+    for (int w = warp; w < nwin; w += kThreads / 32) {
+      const int f = ctl->first[w], id = seq[f];
+      int count = 0, keys = 0;
+      for (int k = 0; k < tw; k += 32) {
+        const int i = f + k + lane;
+        const bool on = k + lane < tw && i < P.tn && seq[i] == id;
+        const unsigned m = __ballot_sync(0xffffffffu, on);
+        const int n = m == ~0u ? 32 : __ffs(~m) - 1;  // up to the run's end
+        keys = max(keys, lane < n ? len[i] : 0);
+        count += n;
+        if (n < 32) break;
       }
-      most_keys = max(most_keys, len[i]);
-      const bool ends = at == tw - 1 || i + 1 == P.tn || starts(i + 1);
-      if (ends) ctl->count[idx] = static_cast<unsigned short>(at + 1);
-      if (ends || i + 1 == b1) atomicMax(&ctl->keys[idx], most_keys);
+      keys = __reduce_max_sync(0xffffffffu, keys);
+      if (lane == 0) {
+        ctl->count[w] = static_cast<unsigned short>(count);
+        ctl->keys[w] = keys;
+        ctl->seq[w] = id;
+      }
     }
     __syncthreads();
     auto units_of = [](int keys) { return keys > 0 ? (keys + kNB - 1) / kNB + kHead : 0; };
