@@ -169,7 +169,7 @@ struct DecSmem {
   int arrived;
 };
 
-template <int D, int FMT, int NG>
+template <int D, int FMT, int NG, bool PK>
 __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     q8_decode_kernel(const __grid_constant__ DecParams P) {
   using Tr = DecTraits<D, NG>;
@@ -271,57 +271,85 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
 
     uint32_t kr[KT][2][C][4], vr[KT][4][VW];
     float2 sc[KT], sc_next[KT];
-    const uint8_t* kbase = pool.k + static_cast<long long>(h) * pool.k_sh + 16 * t4;
-    const uint8_t* vbase = pool.v + static_cast<long long>(h) * pool.v_sh + (D / 8) * g;
+    // Lane pointers into page 0; the strides are constants where the rows of a head's page are one
+    // run of memory (PK), which makes every load but a page's first an immediate offset.
+    const long long k_ss = PK ? D : pool.k_ss, v_ss = PK ? D : pool.v_ss;
+    const uint8_t* kbase = pool.k + static_cast<long long>(h) * pool.k_sh + 16 * t4 + g * k_ss;
+    const uint8_t* vbase = pool.v + static_cast<long long>(h) * pool.v_sh + (D / 8) * g + 2 * t4 * v_ss;
     const float* sbase = pool.scales + static_cast<long long>(h) * pool.s_sh;
+    const int nfull = min(cnt, L / kPage - p0);  // pages of the segment that are attended whole
     auto page_of = [&](int i) -> int {  // i < cnt + KT, called by the whole warp in order
       return i < cnt ? __shfl_sync(0xffffffffu, ids, i & 31) : -1;
     };
-    int pg[KT];
     auto keys_of = [&](int i) { return i < cnt ? min(kPage, L - (p0 + i) * kPage) : 0; };
+    int pg[KT];
+    bool all[KT];  // the page is attended whole and lies in the pool
+    auto next_pages = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        pg[k] = page_of(i + k);
+        all[k] = i + k < nfull && pg[k] >= 0;
+      }
+    };
     auto load_k = [&](int i) {  // K codes and scales of pages i .. i + KT - 1
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-        const int n = pg[k] < 0 ? 0 : keys_of(i + k);
-        sc_next[k] = make_float2(0.f, 1.f);
-        if (n > 0) {
+        const uint8_t* src = kbase + pg[k] * pool.k_sn;
+        if (all[k]) {
           const float* s = sbase + pg[k] * pool.s_sn;
-          sc_next[k].x = __ldg(s);
-          sc_next[k].y = __ldg(s + pool.s_sw);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (g + 8 * r < n)
-              v = ld_stream16(kbase + pg[k] * pool.k_sn + (g + 8 * r) * pool.k_ss + 64 * c);
-            kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
+          if (PK) {
+            sc_next[k] = __ldg(reinterpret_cast<const float2*>(s));
+          } else {
+            sc_next[k].x = __ldg(s);
+            sc_next[k].y = __ldg(s + pool.s_sw);
           }
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const uint4 v = ld_stream16(src + 8 * r * k_ss + 64 * c);
+              kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
+            }
+        } else {  // the row's last page, a page outside the pool, or past the segment
+          const int n = pg[k] < 0 ? 0 : keys_of(i + k);
+          sc_next[k] = make_float2(0.f, 1.f);
+          if (n > 0) {
+            const float* s = sbase + pg[k] * pool.s_sn;
+            sc_next[k].x = __ldg(s);
+            sc_next[k].y = __ldg(s + pool.s_sw);
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (g + 8 * r < n) v = ld_stream16(src + 8 * r * k_ss + 64 * c);
+              kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
+            }
+        }
       }
     };
     auto load_v = [&](int i) {
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-        const int n = pg[k] < 0 ? 0 : keys_of(i + k);
+        const uint8_t* src = vbase + pg[k] * pool.v_sn;
+        const int n = all[k] ? kPage : pg[k] < 0 ? 0 : keys_of(i + k);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = 2 * t4 + (j & 1) + 8 * (j >> 1);
-          const uint8_t* p = vbase + pg[k] * pool.v_sn + key * pool.v_ss;
+          const int row = (j & 1) + 8 * (j >> 1);  // key 2 t + row
           if constexpr (VW == 4) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (key < n) v = ld_stream16(p);
+            if (all[k] || 2 * t4 + row < n) v = ld_stream16(src + row * v_ss);
             vr[k][j][0] = v.x; vr[k][j][1] = v.y; vr[k][j][VW - 2] = v.z; vr[k][j][VW - 1] = v.w;
           } else {
             uint2 v = make_uint2(0, 0);
-            if (key < n) v = ld_stream8(p);
+            if (all[k] || 2 * t4 + row < n) v = ld_stream8(src + row * v_ss);
             vr[k][j][0] = v.x; vr[k][j][1] = v.y;
           }
         }
       }
     };
-#pragma unroll
-    for (int k = 0; k < KT; ++k) pg[k] = page_of(k);
+    next_pages(0);
     load_k(0);
     load_v(0);
 
@@ -364,14 +392,17 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       qs[n] = up;
     }
 
-    float acc[NG][MT][4], ref[NG], lsum[NG];  // ref, lsum: of head 8 n + g
+    // Of head 8 n + g: the reference (0 before the first score), how far a score may pass it (-inf
+    // before the first one), and the sum of weights.
+    float acc[NG][MT][4], base[NG], limit[NG], lsum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
-      ref[n] = -CUDART_INF_F;
+      base[n] = 0.f;
+      limit[n] = -CUDART_INF_F;
       lsum[n] = 0.f;
     }
 
@@ -396,50 +427,57 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
             }
         }
       }
-      int nk[KT];
-#pragma unroll
-      for (int k = 0; k < KT; ++k) nk[k] = keys_of(i + k);
       // ---- the next pages' K ---------------------------------------------------------------
       if (((i + KT) & 31) == 0) {
         ids = ids_next;
         ids_next = load_ids(i + KT + 32);
       }
-#pragma unroll
-      for (int k = 0; k < KT; ++k) pg[k] = page_of(i + KT + k);
-      load_k(i + KT);
-      // ---- weights --------------------------------------------------------------------------
+      next_pages(i + KT);
+      if (i + KT < cnt) load_k(i + KT);
+      // ---- weights: x becomes its distance from the row's reference -----------------------
       bool raise = false;
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         const float lv = lg2(fmaxf(sc[k].y, kMinVs));
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const float f = sc[k].x * qs[n];
-          float top = -CUDART_INF_F;
+          const float f = sc[k].x * qs[n], b = lv - base[n];
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& v = x[k][r][2 * n + j];
-              v = fmaf(v, f, lv);
-              if (nk[k] < kPage && 8 * r + 2 * t4 + j >= nk[k]) v = -CUDART_INF_F;
-              top = fmaxf(top, v);
-            }
-          raise |= top > ref[n] + kSlack;
+            for (int j = 0; j < 2; ++j) x[k][r][2 * n + j] = fmaf(x[k][r][2 * n + j], f, b);
         }
+        if (i + k >= nfull) {  // keys past the row
+          const int n = keys_of(i + k);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (8 * r + 2 * t4 + j >= n)
+#pragma unroll
+                for (int m = 0; m < NG; ++m) x[k][r][2 * m + j] = -CUDART_INF_F;
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+          raise |= fmaxf(max3(x[k][0][2 * n], x[k][0][2 * n + 1], x[k][1][2 * n]), x[k][1][2 * n + 1]) > limit[n];
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          float m = ref[n];
+          // How far the reference moves: to the largest of these scores, never down.
+          float m = limit[n] == -CUDART_INF_F ? -CUDART_INF_F : 0.f;
 #pragma unroll
           for (int k = 0; k < KT; ++k)
 #pragma unroll
             for (int r = 0; r < 2; ++r) m = max3(m, x[k][r][2 * n], x[k][r][2 * n + 1]);
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          const float f = m == -CUDART_INF_F ? 1.f : ex2(ref[n] - m);
-          ref[n] = m;
+          const bool some = m != -CUDART_INF_F;  // a score has been seen
+          const float up = some ? m : 0.f;
+          // Before the first score there is nothing to scale.
+          const float f = limit[n] == -CUDART_INF_F ? 0.f : ex2(-up);
+          base[n] += up;
+          if (some) limit[n] = kSlack;
           lsum[n] *= f;
           const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
@@ -449,26 +487,35 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
             acc[n][q][2] *= f0;
             acc[n][q][3] *= f1;
           }
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              x[k][r][2 * n] -= up;
+              x[k][r][2 * n + 1] -= up;
+            }
         }
       }
       uint32_t pb[KT][NG][2][2];
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         const float iv = __frcp_rn(fmaxf(sc[k].y, kMinVs));
-        const uint32_t keep = sc[k].y >= kMinVs ? ~0u : 0u;  // a page whose scale is 0 holds zeros
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const float base = ref[n] == -CUDART_INF_F ? 0.f : ref[n];
           float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float w = ex2(x[k][r][2 * n + j] - base);
+              const float w = ex2(x[k][r][2 * n + j]);
               sum += w;
-              pb[k][n][r][j] = to_tf32(w) & keep;
+              pb[k][n][r][j] = to_tf32(w);
             }
           lsum[n] = fmaf(sum, iv, lsum[n]);
+        }
+        if (!(sc[k].y >= kMinVs)) {  // a page whose V scale is 0 holds zeros
+#pragma unroll
+          for (int n = 0; n < NG; ++n) pb[k][n][0][0] = pb[k][n][0][1] = pb[k][n][1][0] = pb[k][n][1][1] = 0u;
         }
       }
       // ---- values ---------------------------------------------------------------------------
@@ -487,7 +534,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
               mma_tf32(acc[n][2 * w + 1], v0[2], v0[3], v1[2], v1[3], pb[k][n][r][0], pb[k][n][r][1]);
             }
           }
-      load_v(i + KT);
+      if (i + KT < cnt) load_v(i + KT);
     }
     // ---- the segment's end ----------------------------------------------------------------
 #pragma unroll
@@ -528,7 +575,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       if (t4 == 0)
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          st[Tr::kRows * D + 8 * n + g] = ref[n];
+          st[Tr::kRows * D + 8 * n + g] = limit[n] == -CUDART_INF_F ? -CUDART_INF_F : base[n];
           st[Tr::kRows * D + Tr::kRows + 8 * n + g] = lsum[n];
         }
       if (lane == 0) sm.piece[warp][slot] = Piece{tok * a.KVH + h, first, last};
@@ -635,7 +682,7 @@ int decode_sms(int device) {
   return std::min(cache[device], kMaxCtas);
 }
 
-template <int D, int FMT, int NG>
+template <int D, int FMT, int NG, bool PK>
 cudaError_t launch_one(const DecParams& p, int grid, cudaStream_t stream) {
   using Tr = DecTraits<D, NG>;
   static std::once_flag once[64];
@@ -645,7 +692,7 @@ cudaError_t launch_one(const DecParams& p, int grid, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&] {
-    err[dev] = cudaFuncSetAttribute(q8_decode_kernel<D, FMT, NG>,
+    err[dev] = cudaFuncSetAttribute(q8_decode_kernel<D, FMT, NG, PK>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(sizeof(DecSmem<D, NG>)));
   });
@@ -660,7 +707,7 @@ cudaError_t launch_one(const DecParams& p, int grid, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q8_decode_kernel<D, FMT, NG>, p);
+  return cudaLaunchKernelEx(&cfg, q8_decode_kernel<D, FMT, NG, PK>, p);
 }
 
 }  // namespace
@@ -694,6 +741,8 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
   p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
   const int sms = decode_sms(device);
+  const bool packed = g.p.k_ss == g.p.D && g.p.v_ss == g.p.D && g.p.s_sw == 1 && g.p.s_sn % 2 == 0 &&
+                      g.p.s_sh % 2 == 0 && (reinterpret_cast<uintptr_t>(g.p.scales) & 7) == 0;
   // Tokens per launch: the row lists' room, and units that fit 31 bits.
   const long long per_token = g.a.W * g.a.KVH;
   const long long most = std::max<long long>(1, std::min<long long>(kMaxTok, 0x7fffffffLL / per_token));
@@ -707,14 +756,20 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
     const long long bound = std::max<long long>(1, (per_token * p.tn + p.min_chunk - 1) / p.min_chunk);
     const int grid = static_cast<int>(std::min<long long>(sms, bound));
     cudaError_t e;
-#define SS_Q8_DECODE(D, NG)                                                    \
-  e = g.p.fmt == SS_CODE_INT8 ? launch_one<D, SS_CODE_INT8, NG>(p, grid, stream) \
-                              : launch_one<D, SS_CODE_E4M3, NG>(p, grid, stream)
+#define SS_Q8_DECODE_PK(D, FMT, NG) \
+  e = packed ? launch_one<D, FMT, NG, true>(p, grid, stream) : launch_one<D, FMT, NG, false>(p, grid, stream)
+#define SS_Q8_DECODE(D, NG)                              \
+  if (g.p.fmt == SS_CODE_INT8) {                         \
+    SS_Q8_DECODE_PK(D, SS_CODE_INT8, NG);                \
+  } else {                                               \
+    SS_Q8_DECODE_PK(D, SS_CODE_E4M3, NG);                \
+  }
     if (g.p.D == 128) {
-      if (wide) SS_Q8_DECODE(128, 2); else SS_Q8_DECODE(128, 1);
+      if (wide) { SS_Q8_DECODE(128, 2) } else { SS_Q8_DECODE(128, 1) }
     } else {
-      if (wide) SS_Q8_DECODE(64, 2); else SS_Q8_DECODE(64, 1);
+      if (wide) { SS_Q8_DECODE(64, 2) } else { SS_Q8_DECODE(64, 1) }
     }
+#undef SS_Q8_DECODE_PK
 #undef SS_Q8_DECODE
     if (e != cudaSuccess) return e;
     ++*launches;
