@@ -15,9 +15,11 @@
 // What bounds it: HBM (2 * head_dim bytes per key and KV head), once the ~300 instructions per
 // 4 KiB page (two thirds of them widen bytes) stay below the issue rate.
 //
-// Layout in registers.  The operands of mma.sync are wider than the codes, so the bytes pass
-// through registers anyway; they are loaded there straight from global memory in fragment order,
-// with no shared memory in between.  The order of head_dim and of the keys inside a product is
+// Data path.  A warp streams its own pages: every lane copies (cp.async) the 16-byte pieces that it
+// will use itself into slots of its own, three pages ahead, and loads them back in fragment order;
+// no other lane reads them, so nothing synchronises but the lane's own copy groups.  (With the next
+// page in registers instead, issued piece by piece as registers came free, about 32 KiB per SM were
+// in flight and a page took a warp 4,400 cycles: 31 us for the 64-row batch.)  The order of head_dim and of the keys inside a product is
 // free as long as both operands agree.  Lane (g, t) = (lane / 4, lane % 4):
 //   S = Q K^T       m16n8k16, M = query heads (of one KV head), N = 8 keys.  The lane loads bytes
 //                   [64 c + 16 t, +16) of keys g and g + 8 (16-byte loads); Q is loaded to match.
@@ -25,8 +27,6 @@
 //                   bytes [D/8 g, +D/8) of keys 2t, 2t+1, 2t+8, 2t+9, which are the keys whose
 //                   weights for head g it already holds: S's accumulators are P^T's operand.
 // A lane's V bytes are consecutive, so its outputs are 32 consecutive bytes of an output row.
-// K's registers are refilled for the next page as soon as the page's scores are done, V's when
-// its product is: 4 KiB in flight per warp, 64 KiB per SM.
 //
 // Work split.  Unit = (row, page), row = (token, KV head).  One CTA per SM takes an equal run of
 // units and every warp an equal run of the CTA's.  A row inside a warp's run goes straight to the
@@ -63,12 +63,16 @@ struct DecTraits {
   static constexpr int VW = D / 32;          // 32-bit words a lane holds of a V row
   static constexpr int kRows = 8 * NG;       // query heads of a row (padded)
   static constexpr int kState = kRows * D + 2 * kRows;  // floats of a partial state: O, r, l
+  static constexpr int kStages = 48 / kWarps;            // steps in flight per warp, 4 KiB each
+  static constexpr int kRing = kStages * 4096;           // bytes of a warp's slots
+  static_assert(kState * 4 <= kRing, "a warp's state fits its idle slots");
 };
 
 struct Piece {  // a warp's part of a row that others share
   int row;      // -1: none
   int first;    // the row's first page is inside
   int last;     // the row's last page is inside
+  int mid;      // its state stands in the workspace (the warp went on to another row), not in its slots
 };
 
 __device__ __forceinline__ uint32_t to_tf32(float x) {
@@ -92,18 +96,38 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Streamed loads: the codes are read once per call.
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
+// Copies into the lane's own slots, and back.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_some(uint32_t dst, const void* src, int bytes) {  // the rest: zeros
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+template <int VW>
+__device__ __forceinline__ void copy_v(uint32_t dst, const void* src) {
+  if constexpr (VW == 4)
+    copy16(dst, src);
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 load_slot16(uint32_t src) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+template <int VW>
+__device__ __forceinline__ void load_v(uint32_t src, uint32_t (&w)[VW]) {
+  if constexpr (VW == 4) {
+    const uint4 v = load_slot16(src);
+    w[0] = v.x; w[1] = v.y; w[VW - 2] = v.z; w[VW - 1] = v.w;
+  } else {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(src) : "memory");
+  }
 }
 
 struct DecParams {
@@ -114,6 +138,7 @@ struct DecParams {
   int min_chunk;       // fewest units of a CTA
   unsigned* counter;   // [kMaxCtas], zero between calls
   float* part;         // [2 * grid] partial states
+  float* mid;          // [grid][warps] states of rows that a warp ends before its run does
 };
 
 // Folds `n` states, state i at `at(i)`, into one; thread `e` of the group handles float4 e.
@@ -160,14 +185,15 @@ __device__ __forceinline__ void fold(At at, int n, int e, float4& o, float& r, f
 template <int D, int NG>
 struct DecSmem {
   using Tr = DecTraits<D, NG>;
-  alignas(16) float state[Tr::kWarps][2][Tr::kState];
+  // Slots of the warps; before the stream, the staged ids and lengths; after it, states.
+  alignas(16) uint8_t ring[Tr::kWarps][Tr::kRing];
+  float2 scale[Tr::kWarps][Tr::kStages][Tr::KT];
   Piece piece[Tr::kWarps][2];
   int pre[kMaxTok + 1];  // units before each token
-  int seq[kMaxTok + 2 * kQ8Pad];
-  int len[kMaxTok];
   int scan[Tr::kWarps];
   int arrived;
 };
+static_assert((2 * kMaxTok + 2 * kQ8Pad) * 4 <= 48 * 4096, "the staged tokens fit the slots");
 
 template <int D, int FMT, int NG, bool PK>
 __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
@@ -185,8 +211,9 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   griddep_launch_dependents();
 
   // ---- units before every token ----------------------------------------------------------
-  int* const seq = sm.seq + kQ8Pad;
-  stage_tokens(a, P.t0, P.tn, seq, sm.len, blockIdx.x == 0);
+  int* const seq = reinterpret_cast<int*>(sm.ring) + kQ8Pad;
+  int* const len = seq + kMaxTok + kQ8Pad;
+  stage_tokens(a, P.t0, P.tn, seq, len, blockIdx.x == 0);
   __syncthreads();
   const int per = (P.tn + NT - 1) / NT;
   const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
@@ -194,9 +221,9 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   for (int i = b0; i < b1; ++i) {
     sm.pre[i] = sum;  // within this thread's run
     if (P.skip_runs && in_staged_run(seq, i))
-      sm.len[i] = -1;
+      len[i] = -1;
     else
-      sum += (sm.len[i] + kPage - 1) / kPage * a.KVH;
+      sum += (len[i] + kPage - 1) / kPage * a.KVH;
   }
   int inc = sum;
 #pragma unroll
@@ -205,7 +232,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     if (lane >= o) inc += x;
   }
   if (lane == 31) sm.scan[warp] = inc;
-  if (tid < 2 * NW) sm.piece[tid >> 1][tid & 1].row = -1;
+  if (tid < 2 * NW) sm.piece[tid >> 1][tid & 1].row = -1;  // (ordered by the barriers below)
   __syncthreads();
   int before = inc - sum, U = 0;
 #pragma unroll
@@ -219,7 +246,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   __syncthreads();
   // Tokens of this launch without keys: zero rows, spread over the CTAs.
   for (int i = blockIdx.x; i < P.tn; i += gridDim.x) {
-    if (sm.len[i] != 0) continue;
+    if (len[i] != 0) continue;
     for (int e = tid; e < a.H * D; e += NT)
       a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
   }
@@ -245,13 +272,31 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     }
     tok = lo;
   }
+  int seq_now = 0, L = 0, tok_now = -1;  // of the token whose row is streamed
+  if (u < u1) {
+    while (sm.pre[tok + 1] <= u) ++tok;
+    tok_now = tok;
+    seq_now = seq[tok];
+    L = len[tok];
+  }
+  __syncthreads();  // the staged tokens have been read: the slots are free
+  const uint32_t slot = smem_u32(sm.ring[warp]) + lane * 16;
+  const uint32_t slot_sc = smem_u32(sm.scale[warp]);
+  const long long k_ss = PK ? D : pool.k_ss, v_ss = PK ? D : pool.v_ss;
+
   while (u < u1) {
     while (sm.pre[tok + 1] <= u) ++tok;
-    const int L = sm.len[tok], np = (L + kPage - 1) / kPage;
+    if (tok != tok_now) {
+      const TokInfo ti = q8_token_info(a, P.t0 + tok, false);
+      tok_now = tok;
+      seq_now = static_cast<int>(ti.seq);
+      L = ti.L;
+    }
+    const int np = (L + kPage - 1) / kPage;
     const int rem = u - sm.pre[tok];
     const int h = rem / np, p0 = rem - h * np;
     const int cnt = min(np - p0, u1 - u);  // pages of this segment
-    const long long btrow = static_cast<long long>(seq[tok]) * a.bt_sb;
+    const long long btrow = static_cast<long long>(seq_now) * a.bt_sb;
     const long long t = P.t0 + tok;
 
     // Page ids, 32 at a time (lane i: page p0 + base + i).
@@ -269,89 +314,77 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     };
     int ids = load_ids(0), ids_next = load_ids(32);
 
-    uint32_t kr[KT][2][C][4], vr[KT][4][VW];
-    float2 sc[KT], sc_next[KT];
     // Lane pointers into page 0; the strides are constants where the rows of a head's page are one
-    // run of memory (PK), which makes every load but a page's first an immediate offset.
-    const long long k_ss = PK ? D : pool.k_ss, v_ss = PK ? D : pool.v_ss;
+    // run of memory (PK), which makes every piece but a page's first an immediate offset.
     const uint8_t* kbase = pool.k + static_cast<long long>(h) * pool.k_sh + 16 * t4 + g * k_ss;
     const uint8_t* vbase = pool.v + static_cast<long long>(h) * pool.v_sh + (D / 8) * g + 2 * t4 * v_ss;
     const float* sbase = pool.scales + static_cast<long long>(h) * pool.s_sh;
     const int nfull = min(cnt, L / kPage - p0);  // pages of the segment that are attended whole
-    auto page_of = [&](int i) -> int {  // i < cnt + KT, called by the whole warp in order
-      return i < cnt ? __shfl_sync(0xffffffffu, ids, i & 31) : -1;
-    };
     auto keys_of = [&](int i) { return i < cnt ? min(kPage, L - (p0 + i) * kPage) : 0; };
-    int pg[KT];
-    bool all[KT];  // the page is attended whole and lies in the pool
-    auto next_pages = [&](int i) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        pg[k] = page_of(i + k);
-        all[k] = i + k < nfull && pg[k] >= 0;
-      }
-    };
-    auto load_k = [&](int i) {  // K codes and scales of pages i .. i + KT - 1
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const uint8_t* src = kbase + pg[k] * pool.k_sn;
-        if (all[k]) {
-          const float* s = sbase + pg[k] * pool.s_sn;
-          if (PK) {
-            sc_next[k] = __ldg(reinterpret_cast<const float2*>(s));
-          } else {
-            sc_next[k].x = __ldg(s);
-            sc_next[k].y = __ldg(s + pool.s_sw);
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const uint4 v = ld_stream16(src + 8 * r * k_ss + 64 * c);
-              kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
-            }
-        } else {  // the row's last page, a page outside the pool, or past the segment
-          const int n = pg[k] < 0 ? 0 : keys_of(i + k);
-          sc_next[k] = make_float2(0.f, 1.f);
-          if (n > 0) {
-            const float* s = sbase + pg[k] * pool.s_sn;
-            sc_next[k].x = __ldg(s);
-            sc_next[k].y = __ldg(s + pool.s_sw);
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (g + 8 * r < n) v = ld_stream16(src + 8 * r * k_ss + 64 * c);
-              kr[k][r][c][0] = v.x; kr[k][r][c][1] = v.y; kr[k][r][c][2] = v.z; kr[k][r][c][3] = v.w;
-            }
+    // Copies pages i .. i + KT - 1 into a stage.  K pieces stand at slots (k, r, c), V's after them.
+    int fetched = 0;
+    auto fetch = [&](int stage) {
+      const int i = fetched;
+      fetched += KT;
+      if (i < cnt) {
+        if (i > 0 && (i & 31) == 0) {
+          ids = ids_next;
+          ids_next = load_ids(i + 32);
         }
-      }
-    };
-    auto load_v = [&](int i) {
+        const uint32_t dst = slot + stage * 4096;
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const uint8_t* src = vbase + pg[k] * pool.v_sn;
-        const int n = all[k] ? kPage : pg[k] < 0 ? 0 : keys_of(i + k);
+        for (int k = 0; k < KT; ++k) {
+          const int pg = i + k < cnt ? __shfl_sync(0xffffffffu, ids, (i + k) & 31) : -1;
+          const uint8_t* ks = kbase + pg * pool.k_sn;
+          const uint8_t* vs = vbase + pg * pool.v_sn;
+          const uint32_t kd = dst + k * (2 * C * 512);
+          const uint32_t vd = dst + 2048 + k * (C * 1024) - (VW == 2 ? lane * 8 : 0);
+          const uint32_t sd = slot_sc + (stage * KT + k) * 8;
+          if (i + k < nfull && pg >= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = (j & 1) + 8 * (j >> 1);  // key 2 t + row
-          if constexpr (VW == 4) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (all[k] || 2 * t4 + row < n) v = ld_stream16(src + row * v_ss);
-            vr[k][j][0] = v.x; vr[k][j][1] = v.y; vr[k][j][VW - 2] = v.z; vr[k][j][VW - 1] = v.w;
-          } else {
-            uint2 v = make_uint2(0, 0);
-            if (all[k] || 2 * t4 + row < n) v = ld_stream8(src + row * v_ss);
-            vr[k][j][0] = v.x; vr[k][j][1] = v.y;
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int c = 0; c < C; ++c) copy16(kd + (r * C + c) * 512, ks + 8 * r * k_ss + 64 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) copy_v<VW>(vd + j * (VW * 128), vs + ((j & 1) + 8 * (j >> 1)) * v_ss);
+            if (lane == 0) {
+              const float* s = sbase + pg * pool.s_sn;
+              if (PK) {
+                copy_some<8>(sd, s, 8);
+              } else {
+                copy_some<4>(sd, s, 4);
+                copy_some<4>(sd + 4, s + pool.s_sw, 4);
+              }
+            }
+          } else {  // the row's last page, a page outside the pool, or past the segment
+            const int n = pg < 0 ? 0 : keys_of(i + k);
+            const uint8_t* none = pool.k;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int c = 0; c < C; ++c) {
+                const bool on = g + 8 * r < n;
+                copy_some<16>(kd + (r * C + c) * 512, on ? ks + 8 * r * k_ss + 64 * c : none, on ? 16 : 0);
+              }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = (j & 1) + 8 * (j >> 1);  // key 2 t + row
+              const bool on = 2 * t4 + row < n;
+              copy_some<4 * VW>(vd + j * (VW * 128), on ? vs + row * v_ss : none, on ? 4 * VW : 0);
+            }
+            if (lane == 0) {
+              const float* s = sbase + pg * pool.s_sn;
+              float2 sc = make_float2(0.f, 1.f);
+              if (n > 0) sc = make_float2(__ldg(s), __ldg(s + pool.s_sw));
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sd), "f"(sc.x), "f"(sc.y) : "memory");
+            }
           }
         }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    next_pages(0);
-    load_k(0);
-    load_v(0);
+#pragma unroll
+    for (int st = 0; st < Tr::kStages; ++st) fetch(st);
 
     // Queries as fp16 with the row's power of two taken out: lane (g, t) holds head g's values
     // [64 c + 16 t, +16), the order of the K bytes.
@@ -406,34 +439,35 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       lsum[n] = 0.f;
     }
 
+    int stage = 0;
     for (int i = 0; i < cnt; i += KT) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Tr::kStages - 1) : "memory");
+      __syncwarp();  // lane 0's copies of the scales
+      const uint32_t src = slot + stage * 4096;
       // ---- scores: x[k][r][j + 2 n] of key 8 r + 2 t + j, head 8 n + g ----------------------
       float x[KT][2][4];
+      float2 sc[KT];
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-        sc[k] = sc_next[k];
+        sc[k] = sm.scale[warp][stage][k];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[k][r][j] = 0.f;
 #pragma unroll
-          for (int c = 0; c < C; ++c)
+          for (int c = 0; c < C; ++c) {
+            const uint4 kv = load_slot16(src + (k * 2 * C + r * C + c) * 512);
+            const uint32_t kw[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               uint32_t b0, b1;
-              widen<FMT>(kr[k][r][c][w], b0, b1);
+              widen<FMT>(kw[w], b0, b1);
               mma_f16(x[k][r], qf[0][c][w][0], NG == 2 ? qf[NG - 1][c][w][0] : 0u, qf[0][c][w][1],
                       NG == 2 ? qf[NG - 1][c][w][1] : 0u, b0, b1);
             }
+          }
         }
       }
-      // ---- the next pages' K ---------------------------------------------------------------
-      if (((i + KT) & 31) == 0) {
-        ids = ids_next;
-        ids_next = load_ids(i + KT + 32);
-      }
-      next_pages(i + KT);
-      if (i + KT < cnt) load_k(i + KT);
       // ---- weights: x becomes its distance from the row's reference -----------------------
       bool raise = false;
 #pragma unroll
@@ -522,20 +556,28 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r) {
+          uint32_t w0[VW], w1[VW];  // keys 8 r + 2 t and the one after
+          const uint32_t vsrc = src + 2048 + k * (C * 1024) - (VW == 2 ? lane * 8 : 0) + 2 * r * (VW * 128);
+          load_v<VW>(vsrc, w0);
+          load_v<VW>(vsrc + VW * 128, w1);
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
-            uint32_t v0[4], v1[4];  // keys 8 r + 2 t and the one after
-            widen_f32<FMT>(vr[k][2 * r][w], v0);
-            widen_f32<FMT>(vr[k][2 * r + 1][w], v1);
+            uint32_t v0[4], v1[4];
+            widen_f32<FMT>(w0[w], v0);
+            widen_f32<FMT>(w1[w], v1);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
               mma_tf32(acc[n][2 * w], v0[0], v0[1], v1[0], v1[1], pb[k][n][r][0], pb[k][n][r][1]);
               mma_tf32(acc[n][2 * w + 1], v0[2], v0[3], v1[2], v1[3], pb[k][n][r][0], pb[k][n][r][1]);
             }
           }
-      if (i + KT < cnt) load_v(i + KT);
+        }
+      __syncwarp();  // the stage's scales have been read
+      fetch(stage);
+      stage = stage + 1 == Tr::kStages ? 0 : stage + 1;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     // ---- the segment's end ----------------------------------------------------------------
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -560,8 +602,11 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
           for (int q = 0; q < MT / 4; ++q) dst[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
     } else {
-      const int slot = first ? 1 : 0;
-      float* st = sm.state[warp][slot];
+      const int which = first ? 1 : 0;
+      const bool mid = u + cnt < u1;
+      __syncwarp();
+      float* st = mid ? P.mid + (static_cast<long long>(blockIdx.x) * NW + warp) * Tr::kState
+                      : reinterpret_cast<float*>(sm.ring[warp]);
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -578,7 +623,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
           st[Tr::kRows * D + 8 * n + g] = limit[n] == -CUDART_INF_F ? -CUDART_INF_F : base[n];
           st[Tr::kRows * D + Tr::kRows + 8 * n + g] = lsum[n];
         }
-      if (lane == 0) sm.piece[warp][slot] = Piece{tok * a.KVH + h, first, last};
+      if (lane == 0) sm.piece[warp][which] = Piece{tok * a.KVH + h, first, last, mid};
     }
     u += cnt;
   }
@@ -600,7 +645,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
         make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   };
   static_assert(2 * NW <= 32, "a warp's lanes hold the pieces");
-  Piece mine{-1, 0, 0};
+  Piece mine{-1, 0, 0, 0};
   if (lane < 2 * NW) mine = sm.piece[lane >> 1][lane & 1];
   const unsigned valid = __ballot_sync(0xffffffffu, mine.row >= 0);
   const unsigned firsts = __ballot_sync(0xffffffffu, mine.row >= 0 && mine.first);
@@ -618,7 +663,12 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     if (idx % NGR != grp) continue;
     for (int r = 0; r < ER; ++r) {
       const int e = (tid % GT) + r * NT, head = e / (D / 4);
-      auto state_of = [&](int k) { return sm.state[(i >> 1) + k][k == 0 ? (i & 1) : 0]; };
+      auto state_of = [&](int k) -> const float* {
+        const int w = (i >> 1) + k;
+        return sm.piece[w][k == 0 ? (i & 1) : 0].mid
+                   ? P.mid + (static_cast<long long>(blockIdx.x) * NW + w) * Tr::kState
+                   : reinterpret_cast<const float*>(sm.ring[w]);
+      };
       float rr = -CUDART_INF_F, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < n; ++k) rr = fmaxf(rr, state_of(k)[Tr::kRows * D + head]);
@@ -648,7 +698,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     const int row = open_row[s];
     if (row < 0) continue;  // uniform: every thread walked the same pieces
     const int tk = row / a.KVH, h = row % a.KVH;
-    const int np = (sm.len[tk] + kPage - 1) / kPage;
+    const int np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
     const int first_unit = sm.pre[tk] + h * np;
     const int cf = first_unit / chunk, parts = (first_unit + np - 1) / chunk - cf + 1;
     __syncthreads();  // the CTA's partial state is written
@@ -713,8 +763,10 @@ cudaError_t launch_one(const DecParams& p, int grid, cudaStream_t stream) {
 }  // namespace
 
 size_t q8_decode_workspace(int device) {
+  static_assert(16 * DecTraits<128, 1>::kState >= 8 * DecTraits<128, 2>::kState, "largest states of a CTA");
   return kWsHeader + kCounterBytes +
-         2 * static_cast<size_t>(decode_sms(device)) * DecTraits<128, 2>::kState * sizeof(float);
+         static_cast<size_t>(decode_sms(device)) * (2 * DecTraits<128, 2>::kState + 16 * DecTraits<128, 1>::kState) *
+             sizeof(float);
 }
 
 bool q8_decode_supported(const Q8AttnArgs& g) {
@@ -741,6 +793,7 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
   p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
   const int sms = decode_sms(device);
+  p.mid = p.part + 2ll * sms * DecTraits<128, 2>::kState;
   const bool packed = g.p.k_ss == g.p.D && g.p.v_ss == g.p.D && g.p.s_sw == 1 && g.p.s_sn % 2 == 0 &&
                       g.p.s_sh % 2 == 0 && (reinterpret_cast<uintptr_t>(g.p.scales) & 7) == 0;
   // Tokens per launch: the row lists' room, and units that fit 31 bits.
