@@ -88,6 +88,15 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Integer product of 8-bit digits and codes, 32 deep.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -141,15 +150,15 @@ struct DecParams {
   float* mid;          // [grid][warps] states of rows that a warp ends before its run does
 };
 
-// Folds `n` states, state i at `at(i)`, into one; thread `e` of the group handles float4 e.
-template <int D, int NG, typename At>
+// Folds `n` states, state i at `at(i)`, into one, U at a time; a thread of the group handles float4
+// e.  CG: the states were written by other CTAs during this launch (read past L1).
+template <int D, int NG, int U, bool CG, typename At>
 __device__ __forceinline__ void fold(At at, int n, int e, float4& o, float& r, float& l) {
   using Tr = DecTraits<D, NG>;
   const int head = e / (D / 4);
   o = make_float4(0.f, 0.f, 0.f, 0.f);
   r = -CUDART_INF_F;
   l = 0.f;
-  constexpr int U = 8;
   for (int i0 = 0; i0 < n; i0 += U) {
     float rv[U], lv[U];
     float4 ov[U];
@@ -160,9 +169,15 @@ __device__ __forceinline__ void fold(At at, int n, int e, float4& o, float& r, f
       ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i0 + u < n) {
         const float* s = at(i0 + u);
-        rv[u] = __ldcg(s + Tr::kRows * D + head);
-        lv[u] = __ldcg(s + Tr::kRows * D + Tr::kRows + head);
-        ov[u] = __ldcg(reinterpret_cast<const float4*>(s) + e);
+        if (CG) {
+          rv[u] = __ldcg(s + Tr::kRows * D + head);
+          lv[u] = __ldcg(s + Tr::kRows * D + Tr::kRows + head);
+          ov[u] = __ldcg(reinterpret_cast<const float4*>(s) + e);
+        } else {
+          rv[u] = s[Tr::kRows * D + head];
+          lv[u] = s[Tr::kRows * D + Tr::kRows + head];
+          ov[u] = reinterpret_cast<const float4*>(s)[e];
+        }
       }
     }
     float rn = r;
@@ -191,7 +206,7 @@ struct DecSmem {
   Piece piece[Tr::kWarps][2];
   int pre[kMaxTok + 1];  // units before each token
   int scan[Tr::kWarps];
-  int arrived;
+  int arrived[2];
 };
 static_assert((2 * kMaxTok + 2 * kQ8Pad) * 4 <= 48 * 4096, "the staged tokens fit the slots");
 
@@ -200,15 +215,20 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     q8_decode_kernel(const __grid_constant__ DecParams P) {
   using Tr = DecTraits<D, NG>;
   constexpr int NW = Tr::kWarps, NT = Tr::kThreads, KT = Tr::KT, C = Tr::C, MT = Tr::MT, VW = Tr::VW;
+  constexpr bool kDigits = FMT == SS_CODE_INT8 && NG == 1;  // Q.K as integer products
   extern __shared__ __align__(16) uint8_t smem_raw[];
   DecSmem<D, NG>& sm = *reinterpret_cast<DecSmem<D, NG>*>(smem_raw);
   const AttnArgs& a = P.g.a;
   const Q8Pool& pool = P.g.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // The tile kernel let this one start after its own wait for what came before the call, and
-  // neither reads what the other writes.
-  if (!P.beside) griddep_wait();
-  griddep_launch_dependents();
+  // Sequence ids, positions and table entries are read before the wait for the kernel before (as the
+  // bf16 decode kernel does); the pool, the queries and everything written wait.  The tile kernel let
+  // this one start after its own wait for what came before the call, and neither reads what the
+  // other writes, so beside it nothing waits until the end.
+  auto wait_before = [&]() {
+    if (!P.beside) griddep_wait();
+    griddep_launch_dependents();
+  };
 
   // ---- units before every token ----------------------------------------------------------
   int* const seq = reinterpret_cast<int*>(sm.ring) + kQ8Pad;
@@ -247,13 +267,14 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   // Tokens of this launch without keys: zero rows, spread over the CTAs.
   for (int i = blockIdx.x; i < P.tn; i += gridDim.x) {
     if (len[i] != 0) continue;
+    wait_before();
     for (int e = tid; e < a.H * D; e += NT)
       a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
   }
   const int chunk = max((U + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), P.min_chunk);
   const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
   if (c0 >= U) {
-    if (P.beside) griddep_wait();
+    griddep_wait();
     return;
   }
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
@@ -284,6 +305,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   const uint32_t slot_sc = smem_u32(sm.scale[warp]);
   const long long k_ss = PK ? D : pool.k_ss, v_ss = PK ? D : pool.v_ss;
 
+  bool waited = false;
   while (u < u1) {
     while (sm.pre[tok + 1] <= u) ++tok;
     if (tok != tok_now) {
@@ -313,6 +335,10 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       return id;
     };
     int ids = load_ids(0), ids_next = load_ids(32);
+    if (!waited) {
+      wait_before();
+      waited = true;
+    }
 
     // Lane pointers into page 0; the strides are constants where the rows of a head's page are one
     // run of memory (PK), which makes every piece but a page's first an immediate offset.
@@ -389,12 +415,14 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     // Queries as fp16 with the row's power of two taken out: lane (g, t) holds head g's values
     // [64 c + 16 t, +16), the order of the K bytes.
     uint32_t qf[NG][C][4][2];
-    float qs[NG];  // of head 8 n + g: 2^e * sm_scale * log2 e
+    // The same as three signed digits of base 256: digits [64 c + 16 t + 8 p, +8), two words each.
+    uint32_t qd[3][C][2][2];
+    float qs[NG];  // of head 8 n + g: 2^e * sm_scale * log2 e (for digits 2^-21 of it)
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const int hd = 8 * n + g;
       uint32_t raw[C][8];
-      float amax = 0.f;
+      unsigned top = 0;  // largest magnitude bits (NaN and infinity on top) of either half
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -408,21 +436,42 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[c][w] << 16)),
-                                   fabsf(__uint_as_float(raw[c][w] & 0xffff0000u))));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        for (int w = 0; w < 8; ++w) top = __vmaxu2(top, raw[c][w] & 0x7fff7fffu);
+      top = max(top & 0xffffu, top >> 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max(static_cast<int>(top >> 7) - 127, -104), 126);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+      if constexpr (kDigits) {
+        // round(q 2^(21 - e)) + 0x808080 by an addition whose sum's low bits are that integer; its
+        // bytes, each less 128, are the digits.
+        const float grow = __uint_as_float(static_cast<uint32_t>(127 + 21 - e) << 23);
+        auto whole = [&](uint32_t v) {
+          return __float_as_uint(fmaf(__uint_as_float(v), grow, 12582912.f)) - 0x4b400000u + 0x808080u;
+        };
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-          qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[c][w] << 16) * down,
-                                             __uint_as_float(raw[c][w] & 0xffff0000u) * down);
-      qs[n] = up;
+          for (int w = 0; w < 4; ++w) {  // values 4 w .. 4 w + 3
+            const uint32_t f0 = whole(raw[c][2 * w] << 16), f1 = whole(raw[c][2 * w] & 0xffff0000u);
+            const uint32_t f2 = whole(raw[c][2 * w + 1] << 16), f3 = whole(raw[c][2 * w + 1] & 0xffff0000u);
+            const uint32_t l01 = __byte_perm(f0, f1, 0x5140), l23 = __byte_perm(f2, f3, 0x5140);
+            const uint32_t h01 = __byte_perm(f0, f1, 0x0062), h23 = __byte_perm(f2, f3, 0x0062);
+            qd[0][c][w >> 1][w & 1] = __byte_perm(h01, h23, 0x5410) ^ 0x80808080u;
+            qd[1][c][w >> 1][w & 1] = __byte_perm(l01, l23, 0x7632) ^ 0x80808080u;
+            qd[2][c][w >> 1][w & 1] = __byte_perm(l01, l23, 0x5410) ^ 0x80808080u;
+          }
+        qs[n] = top >= 0x7f80u ? CUDART_NAN_F : up * 0x1p-21f;
+      } else {
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+            qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[c][w] << 16) * down,
+                                               __uint_as_float(raw[c][w] & 0xffff0000u) * down);
+        qs[n] = up;
+      }
     }
 
     // Of head 8 n + g: the reference (0 before the first score), how far a score may pass it (-inf
@@ -452,18 +501,33 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
         sc[k] = sm.scale[warp][stage][k];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          if constexpr (kDigits) {
+            int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[k][r][j] = 0.f;
+            for (int c = 0; c < C; ++c) {
+              const uint4 kv = load_slot16(src + (k * 2 * C + r * C + c) * 512);
+              mma_s8(hi, qd[0][c][0][0], qd[1][c][0][0], qd[0][c][0][1], qd[1][c][0][1], kv.x, kv.y);
+              mma_s8(lo, qd[2][c][0][0], 0u, qd[2][c][0][1], 0u, kv.x, kv.y);
+              mma_s8(hi, qd[0][c][1][0], qd[1][c][1][0], qd[0][c][1][1], qd[1][c][1][1], kv.z, kv.w);
+              mma_s8(lo, qd[2][c][1][0], 0u, qd[2][c][1][1], 0u, kv.z, kv.w);
+            }
 #pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const uint4 kv = load_slot16(src + (k * 2 * C + r * C + c) * 512);
-            const uint32_t kw[4] = {kv.x, kv.y, kv.z, kv.w};
+            for (int j = 0; j < 2; ++j)
+              x[k][r][j] = fmaf(static_cast<float>(hi[j] * 256 + hi[j + 2]), 256.f, static_cast<float>(lo[j]));
+          } else {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t b0, b1;
-              widen<FMT>(kw[w], b0, b1);
-              mma_f16(x[k][r], qf[0][c][w][0], NG == 2 ? qf[NG - 1][c][w][0] : 0u, qf[0][c][w][1],
-                      NG == 2 ? qf[NG - 1][c][w][1] : 0u, b0, b1);
+            for (int j = 0; j < 4; ++j) x[k][r][j] = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const uint4 kv = load_slot16(src + (k * 2 * C + r * C + c) * 512);
+              const uint32_t kw[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                uint32_t b0, b1;
+                widen<FMT>(kw[w], b0, b1);
+                mma_f16(x[k][r], qf[0][c][w][0], NG == 2 ? qf[NG - 1][c][w][0] : 0u, qf[0][c][w][1],
+                        NG == 2 ? qf[NG - 1][c][w][1] : 0u, b0, b1);
+              }
             }
           }
         }
@@ -627,6 +691,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     }
     u += cnt;
   }
+  if (!waited) wait_before();
   __syncthreads();
 
   // ---- rows cut by warp boundaries --------------------------------------------------------
@@ -661,25 +726,17 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     const bool begins = firsts >> i & 1, whole = begins && fin;
     if (!whole) open_row[begins ? 1 : 0] = row;
     if (idx % NGR != grp) continue;
+    // Only a row's last piece can have been left behind by its warp.
+    const int w0 = i >> 1, end = n == 1 ? i : 2 * (w0 + n - 1);
+    const float* tail = sm.piece[end >> 1][end & 1].mid
+                            ? P.mid + (static_cast<long long>(blockIdx.x) * NW + (end >> 1)) * Tr::kState
+                            : reinterpret_cast<const float*>(sm.ring[end >> 1]);
     for (int r = 0; r < ER; ++r) {
       const int e = (tid % GT) + r * NT, head = e / (D / 4);
-      auto state_of = [&](int k) -> const float* {
-        const int w = (i >> 1) + k;
-        return sm.piece[w][k == 0 ? (i & 1) : 0].mid
-                   ? P.mid + (static_cast<long long>(blockIdx.x) * NW + w) * Tr::kState
-                   : reinterpret_cast<const float*>(sm.ring[w]);
-      };
-      float rr = -CUDART_INF_F, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < n; ++k) rr = fmaxf(rr, state_of(k)[Tr::kRows * D + head]);
-      const float base = rr == -CUDART_INF_F ? 0.f : rr;
-      for (int k = 0; k < n; ++k) {
-        const float* s = state_of(k);
-        const float w = ex2(s[Tr::kRows * D + head] - base);
-        const float4 v = reinterpret_cast<const float4*>(s)[e];
-        o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
-        l += s[Tr::kRows * D + Tr::kRows + head] * w;
-      }
+      float4 o;
+      float rr, l;
+      fold<D, NG, 4, false>(
+          [&](int k) { return k == n - 1 ? tail : reinterpret_cast<const float*>(sm.ring[w0 + k]); }, n, e, o, rr, l);
       if (whole) {
         write_row(row, e, o, l);
       } else {
@@ -693,28 +750,35 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     }
   }
 
-  // ---- rows cut by CTA boundaries ---------------------------------------------------------
-  for (int s = 0; s < 2; ++s) {
-    const int row = open_row[s];
-    if (row < 0) continue;  // uniform: every thread walked the same pieces
-    const int tk = row / a.KVH, h = row % a.KVH;
-    const int np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
-    const int first_unit = sm.pre[tk] + h * np;
-    const int cf = first_unit / chunk, parts = (first_unit + np - 1) / chunk - cf + 1;
-    __syncthreads();  // the CTA's partial state is written
-    if (tid == 0) sm.arrived = static_cast<int>(atom_add_acq_rel_gpu_u32(P.counter + cf, 1u));
+  // ---- rows cut by CTA boundaries: at most one begun earlier and one begun here -------------
+  if (open_row[0] >= 0 || open_row[1] >= 0) {  // uniform: every thread walked the same pieces
+    int cf[2] = {0, 0}, parts[2] = {0, 0};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (open_row[s] < 0) continue;
+      const int tk = open_row[s] / a.KVH, h = open_row[s] % a.KVH;
+      const int np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
+      const int first_unit = sm.pre[tk] + h * np;
+      cf[s] = first_unit / chunk;
+      parts[s] = (first_unit + np - 1) / chunk - cf[s] + 1;
+    }
+    __syncthreads();  // the CTA's partial states are written
+    if (tid == 0 && open_row[0] >= 0) sm.arrived[0] = static_cast<int>(atom_add_acq_rel_gpu_u32(P.counter + cf[0], 1u));
+    if (tid == 32 && open_row[1] >= 0) sm.arrived[1] = static_cast<int>(atom_add_acq_rel_gpu_u32(P.counter + cf[1], 1u));
     __syncthreads();
-    if (sm.arrived != parts - 1) continue;
-    if (tid == 0) P.counter[cf] = 0;
-    fence_acq_rel_gpu();
-    if (NGR == 1 || grp == 0) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (open_row[s] < 0 || sm.arrived[s] != parts[s] - 1) continue;
+      if (tid == 32 * s) P.counter[cf[s]] = 0;
+      if (grp != s % NGR) continue;  // a group each
+      fence_acq_rel_gpu();
       for (int r = 0; r < ER; ++r) {
         const int e = (tid % GT) + r * NT;
         float4 o;
         float rr, l;
-        fold<D, NG>([&](int k) { return P.part + (2ll * (cf + k) + (k == 0 ? 1 : 0)) * Tr::kState; },
-                    parts, e, o, rr, l);
-        write_row(row, e, o, l);
+        fold<D, NG, 8, true>([&](int k) { return P.part + (2ll * (cf[s] + k) + (k == 0 ? 1 : 0)) * Tr::kState; },
+                             parts[s], e, o, rr, l);
+        write_row(open_row[s], e, o, l);
       }
     }
   }
