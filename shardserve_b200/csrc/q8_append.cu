@@ -28,7 +28,7 @@ namespace ss {
 namespace {
 
 constexpr int kMaxWindow = 512;          // tokens of one CTA
-constexpr int kHash = 2 * kMaxWindow;    // hash slots (at most half full)
+constexpr int kHash = 2 * kMaxWindow;    // hash slots at most (at most half full)
 
 struct AppendSmem {
   int key[kHash];              // page of a hash slot, -1: empty
@@ -40,152 +40,172 @@ struct AppendSmem {
 };
 
 __device__ __forceinline__ unsigned hash_page(int page) {
-  return (static_cast<unsigned>(page) * 2654435769u) >> 22;  // 10 bits
-}
-static_assert(kHash == 1024, "hash_page gives 10 bits");
-
-// D / 32 consecutive bf16 values of a row, as packed pairs.
-template <int PER>
-__device__ __forceinline__ void load_row(const __nv_bfloat16* p, long long sd, int vec, int lane,
-                                         uint32_t (&w)[PER / 2]) {
-  if (vec) {
-    if constexpr (PER == 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p) + lane);
-      w[0] = u.x;
-      w[1] = u.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const unsigned*>(p) + lane);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER / 2; ++i) {
-      const __nv_bfloat16* e = p + (lane * PER + 2 * i) * sd;
-      w[i] = static_cast<uint32_t>(__bfloat16_as_ushort(e[0])) |
-             static_cast<uint32_t>(__bfloat16_as_ushort(e[sd])) << 16;
-    }
-  }
-}
-template <int PER>
-__device__ __forceinline__ float value_of(const uint32_t (&w)[PER / 2], int i) {
-  return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-}
-template <int PER>
-__device__ __forceinline__ void store_codes(uint8_t* p, long long sd, int vec, int lane,
-                                            const uint8_t (&c)[PER]) {
-  if (vec) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) w |= static_cast<uint32_t>(c[i]) << (8 * i);
-    if (PER == 4)
-      reinterpret_cast<uint32_t*>(p)[lane] = w;
-    else
-      reinterpret_cast<uint16_t*>(p)[lane] = static_cast<uint16_t>(w);
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) p[(lane * PER + i) * sd] = c[i];
-  }
-}
-template <int PER>
-__device__ __forceinline__ void load_codes(const uint8_t* p, long long sd, int vec, int lane,
-                                           uint8_t (&c)[PER]) {
-  if (vec) {
-    const uint32_t w = PER == 4 ? reinterpret_cast<const uint32_t*>(p)[lane]
-                                : reinterpret_cast<const uint16_t*>(p)[lane];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c[i] = static_cast<uint8_t>(w >> (8 * i));
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c[i] = p[(lane * PER + i) * sd];
-  }
+  return (static_cast<unsigned>(page) * 2654435769u) >> 22;
 }
 
-// One page, head and tensor by one warp; `rows` = last token per row of the page.
+// Eight consecutive values of a row, where the row is 16-byte addressable (vec) or anyhow.
+__device__ __forceinline__ uint4 load_values(const __nv_bfloat16* p, long long sd, int vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = static_cast<uint32_t>(__bfloat16_as_ushort(p[2 * i * sd])) |
+           static_cast<uint32_t>(__bfloat16_as_ushort(p[(2 * i + 1) * sd])) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, long long sd, int vec) {
+  if (vec) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= static_cast<uint32_t>(p[i * sd]) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, long long sd, int vec, uint2 c) {
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = c;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i * sd] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+}
+// Four codes of four numbers.  FINITE: none of them lies past the largest code, so the integer can
+// be read off the low byte of x + 1.5 * 2^23 (rounded to nearest even by that addition).
+template <int FMT, bool FINITE>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if constexpr (FMT == SS_CODE_INT8 && FINITE) {
+    const uint32_t ua = __float_as_uint(__fadd_rn(a, 12582912.f)), ub = __float_as_uint(__fadd_rn(b, 12582912.f));
+    const uint32_t uc = __float_as_uint(__fadd_rn(c, 12582912.f)), ud = __float_as_uint(__fadd_rn(d, 12582912.f));
+    return __byte_perm(__byte_perm(ua, ub, 0x0040), __byte_perm(uc, ud, 0x0040), 0x5410);
+  } else if constexpr (FMT == SS_CODE_E4M3) {
+    const float2 lo = make_float2(a, b), hi = make_float2(c, d);
+    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3)) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3)) << 16;
+  } else {
+    return q8_encode(FMT, a) | q8_encode(FMT, b) << 8 | q8_encode(FMT, c) << 16 |
+           static_cast<uint32_t>(q8_encode(FMT, d)) << 24;
+  }
+}
+template <int FMT, bool FINITE>
+__device__ __forceinline__ uint2 encode_row(const uint4& v, float f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __fmul_rn(__uint_as_float(w[i] << 16), f);
+    x[2 * i + 1] = __fmul_rn(__uint_as_float(w[i] & 0xffff0000u), f);
+  }
+  return make_uint2(encode4<FMT, FINITE>(x[0], x[1], x[2], x[3]), encode4<FMT, FINITE>(x[4], x[5], x[6], x[7]));
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(q8_decode(FMT, static_cast<uint8_t>(w >> (8 * i))), f);
+  return encode4<FMT, false>(x[0], x[1], x[2], x[3]);
+}
+
+// One page, head and tensor by one warp; `rows` = last token per row of the page.  D / 8 lanes hold
+// a row's values, eight each; step s holds rows RP s .. RP s + RP - 1.
 template <int D, int FMT>
 __device__ __forceinline__ void append_block(const int* rows, const __nv_bfloat16* x, long long x_st,
                                              long long x_sd, int xvec, uint8_t* codes,
                                              long long c_ss, long long c_sd, int cvec,
                                              float* scale, int lane) {
-  constexpr int PER = D / 32;
-  int has = 0;
-  uint32_t xs[kPage][PER / 2];
+  constexpr int LR = D / 8, RP = 32 / LR, ST = kPage / RP;
+  const int r0 = lane / LR, c8 = lane % LR * 8;
+  uint4 v[ST];
+  unsigned has = 0;  // steps whose row this lane's row group writes
+  unsigned top = 0;  // largest magnitude bits, in both halves
+  const bool fresh = rows[0] >= 0;
+  const float was = *scale;
 #pragma unroll
-  for (int r = 0; r < kPage; ++r) {
-    const int t = rows[r];
-    if (t < 0) continue;
-    has |= 1 << r;
-    load_row<PER>(x + t * x_st, x_sd, xvec, lane, xs[r]);
-  }
-  const bool fresh = has & 1;
-  const float old = fresh ? 0.f : *scale;
-  float amax = 0.f;
-#pragma unroll
-  for (int r = 0; r < kPage; ++r) {
-    if (!(has >> r & 1)) continue;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float v = fabsf(value_of<PER>(xs[r], i));
-      if (v < __int_as_float(0x7f800000)) amax = fmaxf(amax, v);  // false for inf and NaN
+  for (int s = 0; s < ST; ++s) {
+    const int t = rows[s * RP + r0];
+    v[s] = make_uint4(0, 0, 0, 0);
+    if (t >= 0) {
+      has |= 1u << s;
+      v[s] = load_values(x + t * x_st + c8 * x_sd, x_sd, xvec);
     }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int s = 0; s < ST; ++s) {
+    top = __vmaxu2(top, __vmaxu2(v[s].x & 0x7fff7fffu, v[s].y & 0x7fff7fffu));
+    top = __vmaxu2(top, __vmaxu2(v[s].z & 0x7fff7fffu, v[s].w & 0x7fff7fffu));
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  const bool finite = top < 0x7f80u;
+  float amax = __uint_as_float(top << 16);
+  if (!finite) {  // the scale comes from the finite values
+    amax = 0.f;
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+      const uint32_t w[4] = {v[s].x, v[s].y, v[s].z, v[s].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = fabsf(__uint_as_float(w[i] << 16)), b = fabsf(__uint_as_float(w[i] & 0xffff0000u));
+        if (a < __int_as_float(0x7f800000)) amax = fmaxf(amax, a);  // false for inf and NaN
+        if (b < __int_as_float(0x7f800000)) amax = fmaxf(amax, b);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  const float old = fresh ? 0.f : was;
   float s = __fdiv_rn(amax, q8_max(FMT));
   if (s < kQ8Tiny) s = 0.f;
   const float now = fmaxf(old, s);
   const float recip = now > 0.f ? __fdiv_rn(1.f, now) : 0.f;
+  uint8_t* const base = codes + r0 * c_ss + c8 * c_sd;
   if (fresh || now != old || now == 0.f) {  // the page's other rows follow the new scale
     const float ratio = now > 0.f ? __fdiv_rn(old, now) : 0.f;
 #pragma unroll
-    for (int r = 0; r < kPage; ++r) {
-      if (has >> r & 1) continue;
-      uint8_t c[PER];
-      uint8_t* p = codes + r * c_ss;
-      if (fresh) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) c[i] = 0;
-      } else {
-        load_codes<PER>(p, c_sd, cvec, lane, c);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) c[i] = q8_encode(FMT, __fmul_rn(q8_decode(FMT, c[i]), ratio));
+    for (int st = 0; st < ST; ++st) {
+      if (has >> st & 1) continue;
+      uint8_t* p = base + st * RP * c_ss;
+      uint2 c = make_uint2(0, 0);
+      if (!fresh) {
+        c = load_codes(p, c_sd, cvec);
+        c = make_uint2(rescale4<FMT>(c.x, ratio), rescale4<FMT>(c.y, ratio));
       }
-      store_codes<PER>(p, c_sd, cvec, lane, c);
+      store_codes(p, c_sd, cvec, c);
     }
-    __syncwarp();  // every lane has read the old scale
     if (lane == 0) *scale = now;
   }
 #pragma unroll
-  for (int r = 0; r < kPage; ++r) {
-    if (!(has >> r & 1)) continue;
-    uint8_t c[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c[i] = q8_encode(FMT, __fmul_rn(value_of<PER>(xs[r], i), recip));
-    store_codes<PER>(codes + r * c_ss, c_sd, cvec, lane, c);
+  for (int st = 0; st < ST; ++st) {
+    if (!(has >> st & 1)) continue;
+    store_codes(base + st * RP * c_ss, c_sd, cvec,
+                finite ? encode_row<FMT, true>(v[st], recip) : encode_row<FMT, false>(v[st], recip));
   }
 }
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(1024) q8_append_kernel(const Q8AppendArgs a, int window,
-                                                         int kvec, int vvec, int kcvec, int vcvec) {
+__global__ void __launch_bounds__(1024, 1)
+    q8_append_kernel(const Q8AppendArgs a, int window, int hash_shift, int kvec, int vvec, int kcvec, int vcvec) {
   griddep_wait();  // k / v, the slots and the pool may come from the preceding kernel
   extern __shared__ uint8_t smem_raw[];
   AppendSmem& sm = *reinterpret_cast<AppendSmem*>(smem_raw);
   const int tid = threadIdx.x, nt = blockDim.x;
   const long long w0 = static_cast<long long>(blockIdx.x) * window;
   const long long w1 = min(w0 + window, a.T);
-  for (int i = tid; i < kHash; i += nt) sm.key[i] = -1;
+  const unsigned mask = (kHash >> hash_shift) - 1;
+  // This thread's first slot, for both passes below.
+  const long long limit = a.p.N * kPage;
+  auto slot_at = [&](long long t) { return ld_index(a.slots, a.slots64, t); };
+  const long long mine = tid < a.T ? slot_at(tid) : -1;
+  for (int i = tid; i <= static_cast<int>(mask); i += nt) sm.key[i] = -1;
   for (int i = tid; i < window; i += nt) sm.earlier[i] = 0;
   for (int i = tid; i < window * kPage; i += nt) (&sm.row[0][0])[i] = -1;
   if (tid == 0) sm.n = 0;
   __syncthreads();
-  const long long limit = a.p.N * kPage;
   for (long long t = w0 + tid; t < w1; t += nt) {
-    const long long slot = ld_index(a.slots, a.slots64, t);
+    const long long slot = slot_at(t);
     if (slot < 0 || slot >= limit) {
       if (a.err && slot != -1) atomicOr(a.err, SS_DEVERR_SLOT);
       continue;
     }
     const int page = static_cast<int>(slot / kPage);
-    for (unsigned h = hash_page(page);; h = (h + 1) & (kHash - 1)) {
+    for (unsigned h = hash_page(page) >> hash_shift;; h = (h + 1) & mask) {
       const int was = atomicCAS(&sm.key[h], -1, page);
       if (was == -1) {
         const int i = atomicAdd(&sm.n, 1);
@@ -199,11 +219,10 @@ __global__ void __launch_bounds__(1024) q8_append_kernel(const Q8AppendArgs a, i
   __syncthreads();
   const int n = sm.n;
   if (n == 0) return;
-  for (long long t = tid; t < a.T; t += nt) {
-    const long long slot = ld_index(a.slots, a.slots64, t);
-    if (slot < 0 || slot >= limit) continue;
+  auto take = [&](long long t, long long slot) {
+    if (slot < 0 || slot >= limit) return;
     const int page = static_cast<int>(slot / kPage);
-    for (unsigned h = hash_page(page);; h = (h + 1) & (kHash - 1)) {
+    for (unsigned h = hash_page(page) >> hash_shift;; h = (h + 1) & mask) {
       const int key = sm.key[h];
       if (key == -1) break;
       if (key == page) {
@@ -215,6 +234,15 @@ __global__ void __launch_bounds__(1024) q8_append_kernel(const Q8AppendArgs a, i
         break;
       }
     }
+  };
+  take(tid, mine);
+  constexpr int U = 4;  // slots in flight
+  for (long long t = tid + nt; t < a.T; t += U * nt) {
+    long long s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = t + u * nt < a.T ? slot_at(t + u * nt) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) take(t + u * nt, s[u]);
   }
   __syncthreads();
   const int warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
@@ -295,10 +323,12 @@ cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream) {
   long long warps = 4;
   while (warps < 32 && warps < window * 2 * a.p.KVH) warps *= 2;
   const int D = a.p.D;
-  const int kvec = rows_ok(a.k, 2, D / 16, a.k_st, a.k_sh, 0, a.k_sd);
-  const int vvec = rows_ok(a.v, 2, D / 16, a.v_st, a.v_sh, 0, a.v_sd);
-  const int kcvec = rows_ok(a.p.k, 1, D / 32, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd);
-  const int vcvec = rows_ok(a.p.v, 1, D / 32, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
+  const int kvec = rows_ok(a.k, 2, 16, a.k_st, a.k_sh, 0, a.k_sd);
+  const int vvec = rows_ok(a.v, 2, 16, a.v_st, a.v_sh, 0, a.v_sd);
+  const int kcvec = rows_ok(a.p.k, 1, 8, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd);
+  const int vcvec = rows_ok(a.p.v, 1, 8, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
+  int shift = 0;  // a hash of four slots per token of the window, at least 32
+  while ((kHash >> (shift + 1)) >= std::max<long long>(4 * window, 32)) ++shift;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((a.T + window - 1) / window));
   cfg.blockDim = dim3(static_cast<unsigned>(32 * warps));
@@ -309,11 +339,11 @@ cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream) {
   const int w = static_cast<int>(window);
   if (D == 128)
     return a.p.fmt == SS_CODE_INT8
-               ? cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_INT8>, a, w, kvec, vvec, kcvec, vcvec)
-               : cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_E4M3>, a, w, kvec, vvec, kcvec, vcvec);
+               ? cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_INT8>, a, w, shift, kvec, vvec, kcvec, vcvec)
+               : cudaLaunchKernelEx(&cfg, q8_append_kernel<128, SS_CODE_E4M3>, a, w, shift, kvec, vvec, kcvec, vcvec);
   return a.p.fmt == SS_CODE_INT8
-             ? cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_INT8>, a, w, kvec, vvec, kcvec, vcvec)
-             : cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_E4M3>, a, w, kvec, vvec, kcvec, vcvec);
+             ? cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_INT8>, a, w, shift, kvec, vvec, kcvec, vcvec)
+             : cudaLaunchKernelEx(&cfg, q8_append_kernel<64, SS_CODE_E4M3>, a, w, shift, kvec, vvec, kcvec, vcvec);
 }
 
 cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream) {
