@@ -22,6 +22,7 @@
 
 #include "ptx.cuh"
 #include "q8.cuh"
+#include "q8_widen.cuh"
 
 namespace ss {
 
@@ -263,40 +264,51 @@ __global__ void __launch_bounds__(1024, 1)
   }
 }
 
-// One thread per 8 values of a row (or per value where a row is not 8-byte addressable).
-template <bool VEC>
+// One thread per 8 values of a K row and of the V row (or per value where rows are not 8-byte
+// addressable).
+template <int FMT, bool VEC>
 __global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadArgs a) {
   griddep_wait();
   constexpr int E = VEC ? 8 : 1;
-  const long long per_row = static_cast<long long>(a.p.KVH) * a.p.D / E;
-  const long long total = a.T * per_row, step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < 2 * total;
-       i += step) {
-    const bool is_v = i >= total;
-    const long long j = is_v ? i - total : i;
-    const long long t = j / per_row;
-    const int e = static_cast<int>(j % per_row) * E, h = e / a.p.D, d = e % a.p.D;
+  const unsigned per_row = static_cast<unsigned>(a.p.KVH * a.p.D / E);
+  const long long limit = a.p.N * kPage;
+  // A CTA takes 256 consecutive pieces at a time: one 64-bit division for all of them.
+  for (long long b = static_cast<long long>(blockIdx.x) * 256; b < a.T * per_row;
+       b += static_cast<long long>(gridDim.x) * 256) {
+    const long long t0 = b / per_row;
+    const unsigned off = static_cast<unsigned>(b - t0 * per_row) + threadIdx.x;
+    const long long t = t0 + off / per_row;
+    const int e = static_cast<int>(off % per_row) * E, h = e / a.p.D, d = e % a.p.D;
+    if (t >= a.T) continue;
     const long long slot = ld_index(a.slots, a.slots64, t);
-    const bool ok = slot >= 0 && slot < a.p.N * kPage;
-    if (!ok && slot != -1 && a.err && e == 0 && !is_v) atomicOr(a.err, SS_DEVERR_SLOT);
+    const bool ok = slot >= 0 && slot < limit;
+    if (!ok && slot != -1 && a.err && e == 0) atomicOr(a.err, SS_DEVERR_SLOT);
     const long long page = ok ? slot / kPage : 0, row = ok ? slot % kPage : 0;
-    const float s = ok ? a.p.scales[page * a.p.s_sn + h * a.p.s_sh + (is_v ? a.p.s_sw : 0)] : 0.f;
-    const uint8_t* src = is_v ? a.p.v + page * a.p.v_sn + row * a.p.v_ss + h * a.p.v_sh + d * a.p.v_sd
-                              : a.p.k + page * a.p.k_sn + row * a.p.k_ss + h * a.p.k_sh + d * a.p.k_sd;
-    __nv_bfloat16* dst = is_v ? a.v + t * a.v_st + h * a.v_sh + d * a.v_sd
-                              : a.k + t * a.k_st + h * a.k_sh + d * a.k_sd;
-    if (VEC) {
-      const uint2 c = ok ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
-      uint32_t o[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t w = (k < 2 ? c.x : c.y) >> (16 * (k & 1));
-        o[k] = pack_bf16(q8_decode(a.p.fmt, static_cast<uint8_t>(w)) * s,
-                         q8_decode(a.p.fmt, static_cast<uint8_t>(w >> 8)) * s);
-      }
-      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    const float* sp = a.p.scales + page * a.p.s_sn + h * a.p.s_sh;
+    const uint8_t* ks = a.p.k + page * a.p.k_sn + row * a.p.k_ss + h * a.p.k_sh + d * a.p.k_sd;
+    const uint8_t* vs = a.p.v + page * a.p.v_sn + row * a.p.v_ss + h * a.p.v_sh + d * a.p.v_sd;
+    __nv_bfloat16* kd = a.k + t * a.k_st + h * a.k_sh + d * a.k_sd;
+    __nv_bfloat16* vd = a.v + t * a.v_st + h * a.v_sh + d * a.v_sd;
+    const float sk = ok ? sp[0] : 0.f, sv = ok ? sp[a.p.s_sw] : 0.f;
+    if constexpr (VEC) {
+      const uint2 kc = ok ? *reinterpret_cast<const uint2*>(ks) : make_uint2(0, 0);
+      const uint2 vc = ok ? *reinterpret_cast<const uint2*>(vs) : make_uint2(0, 0);
+      auto four = [](uint32_t w, float s, uint32_t& lo, uint32_t& hi) {
+        uint32_t f[4];
+        widen_f32<FMT>(w, f);
+        lo = pack_bf16(__uint_as_float(f[0]) * s, __uint_as_float(f[1]) * s);
+        hi = pack_bf16(__uint_as_float(f[2]) * s, __uint_as_float(f[3]) * s);
+      };
+      uint4 o;
+      four(kc.x, sk, o.x, o.y);
+      four(kc.y, sk, o.z, o.w);
+      *reinterpret_cast<uint4*>(kd) = o;
+      four(vc.x, sv, o.x, o.y);
+      four(vc.y, sv, o.z, o.w);
+      *reinterpret_cast<uint4*>(vd) = o;
     } else {
-      *dst = __float2bfloat16(ok ? q8_decode(a.p.fmt, *src) * s : 0.f);
+      *kd = __float2bfloat16(ok ? q8_decode(FMT, *ks) * sk : 0.f);
+      *vd = __float2bfloat16(ok ? q8_decode(FMT, *vs) * sv : 0.f);
     }
   }
 }
@@ -351,15 +363,18 @@ cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream) {
                    rows_ok(a.v, 2, 16, a.v_st, a.v_sh, 0, a.v_sd) &&
                    rows_ok(a.p.k, 1, 8, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd) &&
                    rows_ok(a.p.v, 1, 8, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
-  const long long work = 2 * a.T * a.p.KVH * a.p.D / (vec ? 8 : 1);
+  const long long work = a.T * a.p.KVH * a.p.D / (vec ? 8 : 1);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(std::max<long long>((work + 255) / 256, 1), 148 * 32)));
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(std::max<long long>((work + 255) / 256, 1), 148 * 64)));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   one_after_another(cfg, attr);
-  return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<true>, a)
-             : cudaLaunchKernelEx(&cfg, q8_read_kernel<false>, a);
+  if (a.p.fmt == SS_CODE_INT8)
+    return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_INT8, true>, a)
+               : cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_INT8, false>, a);
+  return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_E4M3, true>, a)
+             : cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_E4M3, false>, a);
 }
 
 }  // namespace ss
