@@ -154,15 +154,29 @@ __device__ __forceinline__ bool in_staged_run(const int* seq, int i) {
   return n >= kQ8MinRun;
 }
 
+// CTAs of `all` that the split-K kernel takes beside the tiles, by the work of the two: the keys that
+// tokens outside runs attend cost it `7.7` units each, the tiles `0.9` per key and run token (ns per
+// SM and KV head at 8 query heads per KV head, both measured alone; the split moves a few SMs with
+// the group, which costs either side a few per cent).  Both kernels compute it from the same sums, of
+// lengths clamped so that they fit 31 bits.
+constexpr int kQ8SplitTokens = 6144;  // both kernels list a call of up to so many tokens at once
+__host__ __device__ __forceinline__ int q8_clamped(int len) { return len < 262143 ? len : 262143; }
+__device__ __forceinline__ int q8_split(int rows_keys, int run_keys, int all) {
+  if (rows_keys == 0) return 0;
+  if (run_keys == 0) return all;
+  const float a = 7.7f * static_cast<float>(rows_keys), b = 0.9f * static_cast<float>(run_keys);
+  return min(max(__float2int_rn(static_cast<float>(all) * a / (a + b)), 4), all - 4);
+}
+
 cudaError_t launch_q8_append(const Q8AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream);
 cudaError_t launch_q8_generic(const Q8AttnArgs& a, cudaStream_t stream);
 // Split-K kernel (q8_decode.cu): workspace bytes, the layouts it addresses, and the launch
-// (*launches: kernels enqueued).  skip_runs: tokens of runs belong to the tiles; beside: the launch
-// before is the tiles', which this kernel does not wait for until its end.
+// (*launches: kernels enqueued).  skip_runs: tokens of runs belong to the tiles; split: the tiles come
+// right after and take the SMs that q8_split leaves them.
 size_t q8_decode_workspace(int device);
 bool q8_decode_supported(const Q8AttnArgs& g);
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, int device,
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool split, int device,
                              void* workspace, cudaStream_t stream, int* launches);
 // tcgen05 tiles of prompt chunks (q8_prefill.cu), for runs of at least kQ8MinRun tokens: workspace
 // bytes of the cut windows' states, the layouts it takes, tokens per launch, and the launches of
@@ -170,7 +184,7 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
 size_t q8_prefill_workspace(int device);
 bool q8_prefill_supported(const Q8AttnArgs& g, int device);
 int q8_prefill_window();
-cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
+cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, bool split, int device,
                               void* states, cudaStream_t stream);
 cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* states, cudaStream_t stream);
 cudaError_t launch_block_tables(const BlockTablesArgs& a, cudaStream_t stream);

@@ -178,25 +178,24 @@ int ss_ragged_paged_attention_q8(
                        ss::q8_prefill_supported(g, device);
     void* states = static_cast<uint8_t*>(workspace) + ss::q8_decode_workspace(device);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Tiles first: the split-K kernel then takes the SMs as they leave them, and the join of cut
-    // windows comes last.  A batch of several tile launches joins each before the next.
+    // A batch that both kernels list at once runs them side by side; a larger one runs the tiles
+    // launch by launch, each with the join of its cut windows, and then the split-K kernel.
+    const bool split = tiles && tokens <= ss::kQ8SplitTokens;
     const int64_t per = ss::q8_prefill_window();
-    const bool one = tokens <= per;
-    for (int64_t t0 = 0; tiles && t0 < tokens; t0 += per) {
-      e = ss::launch_q8_prefill(g, t0, tokens - t0 < per ? tokens - t0 : per, device, states, s);
-      if (e == cudaSuccess && !one) e = ss::launch_q8_merge(g, device, states, s);
-      if (e != cudaSuccess) return cuda_failed(e, "q8 tile attention launch");
-      ss::count_launches(one ? 1 : 2);
-    }
     int launches = 0;
-    e = ss::launch_q8_decode(g, tiles, tiles && one, device, workspace, s, &launches);
-    ss::count_launches(static_cast<unsigned>(launches));
-    if (e != cudaSuccess) return cuda_failed(e, "q8 split-K attention launch");
-    if (tiles && one) {
-      e = ss::launch_q8_merge(g, device, states, s);
-      if (e != cudaSuccess) return cuda_failed(e, "q8 merge launch");
-      ss::count_launches(1);
+    auto rows = [&]() {
+      e = ss::launch_q8_decode(g, tiles, split, device, workspace, s, &launches);
+      ss::count_launches(static_cast<unsigned>(launches));
+      return e == cudaSuccess ? SS_OK : cuda_failed(e, "q8 split-K attention launch");
+    };
+    if (split && rows() != SS_OK) return SS_ERR_CUDA;
+    for (int64_t t0 = 0; tiles && t0 < tokens; t0 += per) {
+      e = ss::launch_q8_prefill(g, t0, tokens - t0 < per ? tokens - t0 : per, split, device, states, s);
+      if (e == cudaSuccess) e = ss::launch_q8_merge(g, device, states, s);
+      if (e != cudaSuccess) return cuda_failed(e, "q8 tile attention launch");
+      ss::count_launches(2);
     }
+    if (!split && rows() != SS_OK) return SS_ERR_CUDA;
     ss::set_last_path(tiles ? 7 : 5);
     return SS_OK;
   }

@@ -143,8 +143,9 @@ struct DecParams {
   Q8AttnArgs g;
   int t0, tn;          // tokens of this launch
   int skip_runs;       // tokens of runs belong to the tile kernel
-  int beside;          // the kernel before is that tile kernel: start beside it, end after it
+  int split;           // the tile kernel comes next and takes the SMs that q8_split leaves it
   int min_chunk;       // fewest units of a CTA
+  int sms;
   unsigned* counter;   // [kMaxCtas], zero between calls
   float* part;         // [2 * grid] partial states
   float* mid;          // [grid][warps] states of rows that a warp ends before its run does
@@ -205,7 +206,7 @@ struct DecSmem {
   float2 scale[Tr::kWarps][Tr::kStages][Tr::KT];
   Piece piece[Tr::kWarps][2];
   int pre[kMaxTok + 1];  // units before each token
-  int scan[Tr::kWarps];
+  int scan[Tr::kWarps], keys[2][Tr::kWarps];
   int arrived[2];
 };
 static_assert((2 * kMaxTok + 2 * kQ8Pad) * 4 <= 48 * 4096, "the staged tokens fit the slots");
@@ -222,11 +223,11 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   const Q8Pool& pool = P.g.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // Sequence ids, positions and table entries are read before the wait for the kernel before (as the
-  // bf16 decode kernel does); the pool, the queries and everything written wait.  The tile kernel let
-  // this one start after its own wait for what came before the call, and neither reads what the
-  // other writes, so beside it nothing waits until the end.
+  // bf16 decode kernel does); the pool, the queries and everything written wait.  The next kernel is
+  // let go after that wait: the tile kernel, which reads nothing that this one writes, starts on the
+  // SMs that this one leaves.
   auto wait_before = [&]() {
-    if (!P.beside) griddep_wait();
+    griddep_wait();
     griddep_launch_dependents();
   };
 
@@ -237,13 +238,16 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   __syncthreads();
   const int per = (P.tn + NT - 1) / NT;
   const int b0 = min(tid * per, P.tn), b1 = min(b0 + per, P.tn);
-  int sum = 0;
+  int sum = 0, rows_keys = 0, run_keys = 0;
   for (int i = b0; i < b1; ++i) {
     sm.pre[i] = sum;  // within this thread's run
-    if (P.skip_runs && in_staged_run(seq, i))
+    if (P.skip_runs && in_staged_run(seq, i)) {
+      run_keys += q8_clamped(len[i]);
       len[i] = -1;
-    else
+    } else {
+      rows_keys += q8_clamped(len[i]);
       sum += (len[i] + kPage - 1) / kPage * a.KVH;
+    }
   }
   int inc = sum;
 #pragma unroll
@@ -251,15 +255,31 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     const int x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
+  if (P.split) {
+    rows_keys = __reduce_add_sync(0xffffffffu, rows_keys);
+    run_keys = __reduce_add_sync(0xffffffffu, run_keys);
+    if (lane == 0) {
+      sm.keys[0][warp] = rows_keys;
+      sm.keys[1][warp] = run_keys;
+    }
+  }
   if (lane == 31) sm.scan[warp] = inc;
   if (tid < 2 * NW) sm.piece[tid >> 1][tid & 1].row = -1;  // (ordered by the barriers below)
   __syncthreads();
-  int before = inc - sum, U = 0;
+  int before = inc - sum, U = 0, G = gridDim.x;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const int s = sm.scan[w];
     if (w < warp) before += s;
     U += s;
+  }
+  if (P.split) {
+    rows_keys = run_keys = 0;
+    for (int w = 0; w < NW; ++w) {
+      rows_keys += sm.keys[0][w];
+      run_keys += sm.keys[1][w];
+    }
+    G = max(q8_split(rows_keys, run_keys, P.sms), 1);
   }
   for (int i = b0; i < b1; ++i) sm.pre[i] += before;
   if (tid == 0) sm.pre[P.tn] = U;
@@ -271,10 +291,10 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     for (int e = tid; e < a.H * D; e += NT)
       a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
   }
-  const int chunk = max((U + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), P.min_chunk);
+  const int chunk = max((U + G - 1) / G, P.min_chunk);
   const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
   if (c0 >= U) {
-    griddep_wait();
+    wait_before();
     return;
   }
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
@@ -782,7 +802,6 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       }
     }
   }
-  if (P.beside) griddep_wait();
 }
 
 int decode_sms(int device) {
@@ -848,15 +867,16 @@ bool q8_decode_supported(const Q8AttnArgs& g) {
          rows16(a.out, a.o_st, a.o_sh, a.o_sd);
 }
 
-cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, int device,
+cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool split, int device,
                              void* workspace, cudaStream_t stream, int* launches) {
   DecParams p;
   p.g = g;
   p.skip_runs = skip_runs;
-  p.beside = beside;
+  p.split = split;
   p.counter = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(workspace) + kWsHeader);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kWsHeader + kCounterBytes);
   const int sms = decode_sms(device);
+  p.sms = sms;
   p.mid = p.part + 2ll * sms * DecTraits<128, 2>::kState;
   const bool packed = g.p.k_ss == g.p.D && g.p.v_ss == g.p.D && g.p.s_sw == 1 && g.p.s_sn % 2 == 0 &&
                       g.p.s_sh % 2 == 0 && (reinterpret_cast<uintptr_t>(g.p.scales) & 7) == 0;
@@ -871,7 +891,7 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
     p.min_chunk = wide ? 8 : 16;
     // No more CTAs than the table could fill (the lengths are on the device).
     const long long bound = std::max<long long>(1, (per_token * p.tn + p.min_chunk - 1) / p.min_chunk);
-    const int grid = static_cast<int>(std::min<long long>(sms, bound));
+    const int grid = split ? sms : static_cast<int>(std::min<long long>(sms, bound));
     cudaError_t e;
 #define SS_Q8_DECODE_PK(D, FMT, NG) \
   e = packed ? launch_one<D, FMT, NG, true>(p, grid, stream) : launch_one<D, FMT, NG, false>(p, grid, stream)
@@ -890,7 +910,6 @@ cudaError_t launch_q8_decode(const Q8AttnArgs& g, bool skip_runs, bool beside, i
 #undef SS_Q8_DECODE
     if (e != cudaSuccess) return e;
     ++*launches;
-    p.beside = 0;  // a second launch waits for the first
   }
   return cudaSuccess;
 }

@@ -84,6 +84,7 @@ struct CtlQ {
   float4 sc[4][kPages];   // per block (mod 4) and page: K scale, log2 and reciprocal of V's
   uint32_t tmem;
   int red[kThreads / 32];
+  int run_keys;
   unsigned short first[kMaxWin], count[kMaxWin];
   int keys[kMaxWin], seq[kMaxWin];
   int pre[kMaxWin + 1];   // units before each window
@@ -92,6 +93,7 @@ struct CtlQ {
 struct PrefillParams {
   Q8AttnArgs g;
   int t0, tn;
+  int split;          // the split-K kernel of the call runs beside this one, on q8_split's SMs
   int tpt;            // tokens per tile
   unsigned magic;     // ceil(2^32 / window): x / window = (x * magic) >> 32 for x < 2^13
   unsigned magic_group;  // the same for the group (0: of one head)
@@ -205,17 +207,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(kBarVE + t), 1);
     }
     mbar_init(bar(kBarEnd), 1);
+    ctl->run_keys = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
     tmem_alloc(smem_u32(&ctl->tmem), 512);
     tmem_relinquish();
   }
-  griddep_wait();
+  // After the split-K kernel of the same call, which waited for what came before it, nothing is
+  // waited for until the end.
+  if (!P.split) griddep_wait();
   griddep_launch_dependents();
 
   // ---- the windows of this launch ----------------------------------------------------------
-  int nwin, units;
+  int nwin, units, ctas = gridDim.x;  // CTAs that take units
   {
     // The operand buffers are idle: the staged ids and lengths stand there.
     int* const seq = reinterpret_cast<int*>(smem) + kQ8Pad;
@@ -233,10 +238,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (starts(i)) start = i;
     const int before = scan_max(start, ctl->red, warp, lane);
     start = before;
+    int all_keys = 0;     // of this thread's tokens
     unsigned begins = 0;  // tokens of this thread that begin a window (at most 13 tokens a thread)
     for (int i = b0; i < b1; ++i) {
       if (starts(i)) start = i;
       if (place(i - start) == 0 && in_run(i, start)) begins |= 1u << (i - b0);
+      all_keys += q8_clamped(len[i]);
     }
     int idx = scan_sum(__popc(begins), ctl->red, warp, lane, nwin);
     for (; begins; begins &= begins - 1) ctl->first[idx++] = static_cast<unsigned short>(b0 + __ffs(begins) - 1);
@@ -244,18 +251,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One warp per window: its tokens, and the keys that they attend.
     for (int w = warp; w < nwin; w += kThreads / 32) {
       const int f = ctl->first[w], id = seq[f];
-      int count = 0, keys = 0;
+      int count = 0, keys = 0, sum = 0;
       for (int k = 0; k < tw; k += 32) {
         const int i = f + k + lane;
         const bool on = k + lane < tw && i < P.tn && seq[i] == id;
         const unsigned m = __ballot_sync(0xffffffffu, on);
         const int n = m == ~0u ? 32 : __ffs(~m) - 1;  // up to the run's end
         keys = max(keys, lane < n ? len[i] : 0);
+        sum += lane < n ? q8_clamped(len[i]) : 0;
         count += n;
         if (n < 32) break;
       }
       keys = __reduce_max_sync(0xffffffffu, keys);
+      sum = __reduce_add_sync(0xffffffffu, sum);
       if (lane == 0) {
+        if (P.split) atomicAdd(&ctl->run_keys, sum);
         ctl->count[w] = static_cast<unsigned short>(count);
         ctl->keys[w] = keys;
         ctl->seq[w] = id;
@@ -280,12 +290,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (tid == 0) ctl->pre[nwin] = units;
+    if (P.split) {
+      int total;
+      scan_sum(all_keys, ctl->red, warp, lane, total);
+      ctas -= q8_split(total - ctl->run_keys, ctl->run_keys, ctas);
+      ctas = max(ctas, 1);
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const int share = max((units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinPart);
+  const int share = max((units + ctas - 1) / ctas, kMinPart);
   const int u0 = min(static_cast<long long>(blockIdx.x) * share, static_cast<long long>(units));
   const int u1 = min(u0 + static_cast<long long>(share), static_cast<long long>(units));
 
@@ -815,6 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (P.split) griddep_wait();  // this grid ends after the split-K kernel
 }
 
 // Joins the states of cut windows: one thread per (row, 16 values).
@@ -914,10 +931,11 @@ bool q8_prefill_supported(const Q8AttnArgs& g, int device) {
                       : (i8 ? prepare_one<64, SS_CODE_INT8>(device) : prepare_one<64, SS_CODE_E4M3>(device));
 }
 
-cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, int device,
+cudaError_t launch_q8_prefill(const Q8AttnArgs& g, long long t0, long long tn, bool split, int device,
                               void* states, cudaStream_t stream) {
   PrefillParams p;
   p.g = g;
+  p.split = split;
   p.t0 = static_cast<int>(t0);
   p.tn = static_cast<int>(tn);
   p.tpt = kRows / g.a.group;
@@ -938,7 +956,7 @@ cudaError_t launch_q8_merge(const Q8AttnArgs& g, int device, void* states,
                             cudaStream_t stream) {
   PrefillParams p;
   p.g = g;
-  p.t0 = p.tn = 0;
+  p.t0 = p.tn = p.split = 0;
   p.tpt = kRows / g.a.group;
   p.magic = p.magic_group = 0;
   const int ctas = prefill_sms(device), grid = ctas * (g.p.D / 16);

@@ -617,3 +617,26 @@ def test_refusals():
     with pytest.raises(sb.KernelUnsupported):
         sb.ragged_attention_q8(torch.zeros(3, 16, 128, device=DEV).bfloat16(), k, v, sc,
                                torch.zeros(2, 4, dtype=torch.int32, device=DEV), i, i, float("nan"))
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_serving_example(codes):
+    """The example's loop: lengths and pages add up, and the outputs stay near the bf16 cache's.  The
+    hidden state's own terms do not pass the cache, so its relative difference is below the codes'
+    relative error: 1/254 of the block's largest value (about 4 standard deviations) for int8, 2^-4
+    for e4m3."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "quantized_serving.py")
+    spec = importlib.util.spec_from_file_location("quantized_serving", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    got = m.run(steps=20, codes=codes)
+    lens = [75 + 13 * r + 20 for r in range(6)]
+    assert got["lens"] == lens
+    assert got["pages_used"] == sum((n + 15) // 16 for n in lens)
+    assert got["errors"] == 0
+    assert got["bytes_8bit"] < 0.52 * got["bytes_bf16"]
+    assert got["relative_difference"] < (0.03 if codes == "int8" else 2.0 ** -4)
