@@ -298,10 +298,47 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     return;
   }
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
-  // Warps 0 .. nwa - 1 hold at least one unit each.
-  const int nwa = min(NW, n_cta), wq = n_cta / nwa, wr = n_cta % nwa;
-  int u = static_cast<int>(c0) + warp * wq + min(warp, wr);
-  const int u1 = warp < nwa ? u + wq + (warp < wr ? 1 : 0) : u;
+  // Shares of the warps, in unit order.  A row's end inside a warp's share costs it about two units (its
+  // copies run dry and its queries change), and the CTA waits for its slowest warp; so rows get warps of
+  // their own, as long as no warp then holds more than two units above an even share.
+  int u, u1;
+  {
+    const int even = (n_cta + NW - 1) / NW;
+    int first_tok = 0;  // token of the CTA's first unit
+    for (int lo = 0, hi = P.tn; hi - lo > 1; first_tok = lo) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.pre[mid] <= c0) lo = mid; else hi = mid;
+    }
+    // Lane i: units that the CTA holds of the i-th row from the token's first one on.
+    const int tk = min(first_tok + lane / a.KVH, P.tn - 1), np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
+    const int r0 = sm.pre[tk] + lane % a.KVH * np;
+    const int e0 = max(r0, static_cast<int>(c0)), e1 = min(r0 + np, static_cast<int>(c0) + n_cta);
+    const int mine = first_tok + lane / a.KVH < P.tn ? max(e1 - e0, 0) : 0;
+    int size = 0, parts = 0;  // most units of a warp, the row's warps
+    if (static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) == n_cta)
+      for (int s = even; s <= even + 2 && size == 0; ++s) {
+        parts = (mine + s - 1) / s;
+        if (static_cast<int>(__reduce_add_sync(0xffffffffu, parts)) <= NW) size = s;
+      }
+    if (size != 0) {
+      int upto = parts;  // warps up to and with this row's
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const unsigned after = __ballot_sync(0xffffffffu, upto > warp);
+      const int row = after ? __ffs(after) - 1 : 31;
+      const int n = __shfl_sync(0xffffffffu, mine, row), k = max(__shfl_sync(0xffffffffu, parts, row), 1);
+      const int i = warp - (__shfl_sync(0xffffffffu, upto, row) - k), q = n / k, rest = n % k;
+      u = __shfl_sync(0xffffffffu, e0, row) + i * q + min(i, rest);
+      u1 = after ? u + q + (i < rest ? 1 : 0) : u;
+    } else {  // even shares; warps 0 .. nwa - 1 hold at least one unit each
+      const int nwa = min(NW, n_cta), wq = n_cta / nwa, wr = n_cta % nwa;
+      u = static_cast<int>(c0) + warp * wq + min(warp, wr);
+      u1 = warp < nwa ? u + wq + (warp < wr ? 1 : 0) : u;
+    }
+  }
 
   const int g = lane >> 2, t4 = lane & 3;
   int tok = 0;  // token of unit u
@@ -429,34 +466,37 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // The queries are asked for before the first pages: behind them they would wait for 28 MB.
+    // Lane (g, t) holds head g's values [64 c + 16 t, +16), the order of the K bytes.
+    uint32_t raw[NG][C][8];
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int hd = 8 * n + g;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (hd < a.group)
+            v = __ldg(reinterpret_cast<const uint4*>(
+                a.q + t * a.q_st + static_cast<long long>(h * a.group + hd) * a.q_sh + 64 * c + 16 * t4 + 8 * w));
+          raw[n][c][4 * w] = v.x; raw[n][c][4 * w + 1] = v.y; raw[n][c][4 * w + 2] = v.z; raw[n][c][4 * w + 3] = v.w;
+        }
 #pragma unroll
     for (int st = 0; st < Tr::kStages; ++st) fetch(st);
 
-    // Queries as fp16 with the row's power of two taken out: lane (g, t) holds head g's values
-    // [64 c + 16 t, +16), the order of the K bytes.
+    // Queries as fp16 with the row's power of two taken out.
     uint32_t qf[NG][C][4][2];
     // The same as three signed digits of base 256: digits [64 c + 16 t + 8 p, +8), two words each.
     uint32_t qd[3][C][2][2];
     float qs[NG];  // of head 8 n + g: 2^e * sm_scale * log2 e (for digits 2^-21 of it)
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const int hd = 8 * n + g;
-      uint32_t raw[C][8];
       unsigned top = 0;  // largest magnitude bits (NaN and infinity on top) of either half
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (hd < a.group)
-            v = __ldg(reinterpret_cast<const uint4*>(
-                a.q + t * a.q_st + static_cast<long long>(h * a.group + hd) * a.q_sh + 64 * c + 16 * t4 + 8 * w));
-          raw[c][4 * w] = v.x; raw[c][4 * w + 1] = v.y; raw[c][4 * w + 2] = v.z; raw[c][4 * w + 3] = v.w;
-        }
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int w = 0; w < 8; ++w) top = __vmaxu2(top, raw[c][w] & 0x7fff7fffu);
+        for (int w = 0; w < 8; ++w) top = __vmaxu2(top, raw[n][c][w] & 0x7fff7fffu);
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -473,8 +513,8 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
         for (int c = 0; c < C; ++c)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {  // values 4 w .. 4 w + 3
-            const uint32_t f0 = whole(raw[c][2 * w] << 16), f1 = whole(raw[c][2 * w] & 0xffff0000u);
-            const uint32_t f2 = whole(raw[c][2 * w + 1] << 16), f3 = whole(raw[c][2 * w + 1] & 0xffff0000u);
+            const uint32_t f0 = whole(raw[n][c][2 * w] << 16), f1 = whole(raw[n][c][2 * w] & 0xffff0000u);
+            const uint32_t f2 = whole(raw[n][c][2 * w + 1] << 16), f3 = whole(raw[n][c][2 * w + 1] & 0xffff0000u);
             const uint32_t l01 = __byte_perm(f0, f1, 0x5140), l23 = __byte_perm(f2, f3, 0x5140);
             const uint32_t h01 = __byte_perm(f0, f1, 0x0062), h23 = __byte_perm(f2, f3, 0x0062);
             qd[0][c][w >> 1][w & 1] = __byte_perm(h01, h23, 0x5410) ^ 0x80808080u;
@@ -488,8 +528,8 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
         for (int c = 0; c < C; ++c)
 #pragma unroll
           for (int w = 0; w < 8; ++w)
-            qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[c][w] << 16) * down,
-                                               __uint_as_float(raw[c][w] & 0xffff0000u) * down);
+            qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[n][c][w] << 16) * down,
+                                               __uint_as_float(raw[n][c][w] & 0xffff0000u) * down);
         qs[n] = up;
       }
     }
