@@ -124,21 +124,28 @@ __device__ __forceinline__ void stage_tokens(const AttnArgs& a, long long t0, in
     const int id = static_cast<int>(ld_index(a.seq, a.seq64, in));
     neighbour = in == t ? id : ~id;
   }
-  constexpr int U = 8;  // loads in flight: every one is a round trip to L2 or beyond
-  for (int i0 = threadIdx.x; i0 < tn; i0 += U * blockDim.x) {
-    long long s[U], p[U];
+  auto put = [&](int i, long long s, long long p) {
+    seq[i] = static_cast<int>(s);
+    len[i] = s == -1 ? 0 : token_info_from(a, s, p, report).L;
+  };
+  if (tn <= static_cast<int>(blockDim.x)) {
+    const int i = threadIdx.x;
+    if (i < tn) put(i, ld_index(a.seq, a.seq64, t0 + i), ld_index(a.pos, a.pos64, t0 + i));
+  } else {
+    constexpr int U = 8;  // loads in flight: every one is a round trip to L2 or beyond
+    for (int i0 = threadIdx.x; i0 < tn; i0 += U * blockDim.x) {
+      long long s[U], p[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = min(i0 + u * static_cast<int>(blockDim.x), tn - 1);
-      s[u] = ld_index(a.seq, a.seq64, t0 + i);
-      p[u] = ld_index(a.pos, a.pos64, t0 + i);
-    }
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * static_cast<int>(blockDim.x), tn - 1);
+        s[u] = ld_index(a.seq, a.seq64, t0 + i);
+        p[u] = ld_index(a.pos, a.pos64, t0 + i);
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * static_cast<int>(blockDim.x);
-      if (i >= tn) break;
-      seq[i] = static_cast<int>(s[u]);
-      len[i] = s[u] == -1 ? 0 : token_info_from(a, s[u], p[u], report).L;
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * static_cast<int>(blockDim.x);
+        if (i < tn) put(i, s[u], p[u]);
+      }
     }
   }
   if (threadIdx.x < 2 * kQ8Pad) seq[at] = neighbour;

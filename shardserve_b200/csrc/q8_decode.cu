@@ -75,6 +75,14 @@ struct Piece {  // a warp's part of a row that others share
   int mid;      // its state stands in the workspace (the warp went on to another row), not in its slots
 };
 
+// a / b for 0 <= a, 0 < b: an fp32 quotient, put right by its remainder.
+__device__ __forceinline__ int quotient(int a, int b) {
+  int q = __float2int_rz(__fdividef(static_cast<float>(a), static_cast<float>(b)));
+  int r = a - q * b;
+  while (r < 0) { --q; r += b; }
+  while (r >= b) { ++q; r -= b; }
+  return q;
+}
 __device__ __forceinline__ uint32_t to_tf32(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -266,13 +274,10 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   if (lane == 31) sm.scan[warp] = inc;
   if (tid < 2 * NW) sm.piece[tid >> 1][tid & 1].row = -1;  // (ordered by the barriers below)
   __syncthreads();
-  int before = inc - sum, U = 0, G = gridDim.x;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const int s = sm.scan[w];
-    if (w < warp) before += s;
-    U += s;
-  }
+  const int part_sum = sm.scan[lane % NW];
+  const int before = inc - sum + __reduce_add_sync(0xffffffffu, lane < warp ? part_sum : 0);
+  const int U = __reduce_add_sync(0xffffffffu, lane < NW ? part_sum : 0);
+  int G = gridDim.x;
   if (P.split) {
     rows_keys = run_keys = 0;
     for (int w = 0; w < NW; ++w) {
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     for (int e = tid; e < a.H * D; e += NT)
       a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
   }
-  const int chunk = max((U + G - 1) / G, P.min_chunk);
+  const int chunk = max(U == 0 ? 0 : quotient(U - 1, G) + 1, P.min_chunk);
   const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
   if (c0 >= U) {
     wait_before();
@@ -301,23 +306,28 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   // Shares of the warps, in unit order.  A row's end inside a warp's share costs it about two units (its
   // copies run dry and its queries change), and the CTA waits for its slowest warp; so rows get warps of
   // their own, as long as no warp then holds more than two units above an even share.
-  int u, u1;
-  {
-    const int even = (n_cta + NW - 1) / NW;
-    int first_tok = 0;  // token of the CTA's first unit
-    for (int lo = 0, hi = P.tn; hi - lo > 1; first_tok = lo) {
-      const int mid = (lo + hi) >> 1;
-      if (sm.pre[mid] <= c0) lo = mid; else hi = mid;
+  auto token_of = [&](int unit, int lo) {  // the last token that begins at or before the unit
+    for (int hi = P.tn; hi - lo > 1;) {
+      const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
+      const int n = __popc(__ballot_sync(0xffffffffu, i < hi && sm.pre[min(i, P.tn)] <= unit));
+      lo += n * step;
+      hi = min(hi, lo + step);
     }
+    return lo;
+  };
+  int u, u1, tok;  // this warp's units, and the token of the first
+  {
+    const int even = (n_cta + NW - 1) / NW, first_tok = token_of(static_cast<int>(c0), 0);
     // Lane i: units that the CTA holds of the i-th row from the token's first one on.
-    const int tk = min(first_tok + lane / a.KVH, P.tn - 1), np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
-    const int r0 = sm.pre[tk] + lane % a.KVH * np;
+    const int ahead = quotient(lane, a.KVH), tk = min(first_tok + ahead, P.tn - 1);
+    const int np = (len[tk] + kPage - 1) / kPage, r0 = sm.pre[tk] + (lane - ahead * a.KVH) * np;
     const int e0 = max(r0, static_cast<int>(c0)), e1 = min(r0 + np, static_cast<int>(c0) + n_cta);
-    const int mine = first_tok + lane / a.KVH < P.tn ? max(e1 - e0, 0) : 0;
+    const int mine = first_tok + ahead < P.tn ? max(e1 - e0, 0) : 0;
     int size = 0, parts = 0;  // most units of a warp, the row's warps
-    if (static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) == n_cta)
+    // (With one unit per warp, or more rows than lanes, the shares are even.)
+    if (even > 1 && static_cast<int>(__reduce_add_sync(0xffffffffu, mine)) == n_cta)
       for (int s = even; s <= even + 2 && size == 0; ++s) {
-        parts = (mine + s - 1) / s;
+        parts = mine == 0 ? 0 : quotient(mine - 1, s) + 1;
         if (static_cast<int>(__reduce_add_sync(0xffffffffu, parts)) <= NW) size = s;
       }
     if (size != 0) {
@@ -330,29 +340,21 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       const unsigned after = __ballot_sync(0xffffffffu, upto > warp);
       const int row = after ? __ffs(after) - 1 : 31;
       const int n = __shfl_sync(0xffffffffu, mine, row), k = max(__shfl_sync(0xffffffffu, parts, row), 1);
-      const int i = warp - (__shfl_sync(0xffffffffu, upto, row) - k), q = n / k, rest = n % k;
+      const int i = warp - (__shfl_sync(0xffffffffu, upto, row) - k), q = quotient(n, k), rest = n - q * k;
       u = __shfl_sync(0xffffffffu, e0, row) + i * q + min(i, rest);
       u1 = after ? u + q + (i < rest ? 1 : 0) : u;
+      tok = first_tok + __shfl_sync(0xffffffffu, ahead, row);
     } else {  // even shares; warps 0 .. nwa - 1 hold at least one unit each
-      const int nwa = min(NW, n_cta), wq = n_cta / nwa, wr = n_cta % nwa;
+      const int nwa = min(NW, n_cta), wq = quotient(n_cta, nwa), wr = n_cta - wq * nwa;
       u = static_cast<int>(c0) + warp * wq + min(warp, wr);
       u1 = warp < nwa ? u + wq + (warp < wr ? 1 : 0) : u;
+      tok = u < u1 ? token_of(u, first_tok) : 0;
     }
   }
 
   const int g = lane >> 2, t4 = lane & 3;
-  int tok = 0;  // token of unit u
-  if (u < u1) {
-    int lo = 0, hi = P.tn;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (sm.pre[mid] <= u) lo = mid; else hi = mid;
-    }
-    tok = lo;
-  }
   int seq_now = 0, L = 0, tok_now = -1;  // of the token whose row is streamed
   if (u < u1) {
-    while (sm.pre[tok + 1] <= u) ++tok;
     tok_now = tok;
     seq_now = seq[tok];
     L = len[tok];
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     }
     const int np = (L + kPage - 1) / kPage;
     const int rem = u - sm.pre[tok];
-    const int h = rem / np, p0 = rem - h * np;
+    const int h = quotient(rem, np), p0 = rem - h * np;
     const int cnt = min(np - p0, u1 - u);  // pages of this segment
     const long long btrow = static_cast<long long>(seq_now) * a.bt_sb;
     const long long t = P.t0 + tok;
@@ -765,8 +767,9 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     const int hd = e / (D / 4), d = (e % (D / 4)) * 4;
     if (hd >= a.group) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const long long t = P.t0 + row / a.KVH;
-    *reinterpret_cast<uint2*>(a.out + t * a.o_st + static_cast<long long>((row % a.KVH) * a.group + hd) * a.o_sh + d) =
+    const int tk = quotient(row, a.KVH);
+    const long long t = P.t0 + tk;
+    *reinterpret_cast<uint2*>(a.out + t * a.o_st + static_cast<long long>((row - tk * a.KVH) * a.group + hd) * a.o_sh + d) =
         make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   };
   static_assert(2 * NW <= 32, "a warp's lanes hold the pieces");
@@ -816,11 +819,11 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (open_row[s] < 0) continue;
-      const int tk = open_row[s] / a.KVH, h = open_row[s] % a.KVH;
-      const int np = (sm.pre[tk + 1] - sm.pre[tk]) / a.KVH;
+      const int tk = quotient(open_row[s], a.KVH), h = open_row[s] - tk * a.KVH;
+      const int np = quotient(sm.pre[tk + 1] - sm.pre[tk], a.KVH);
       const int first_unit = sm.pre[tk] + h * np;
-      cf[s] = first_unit / chunk;
-      parts[s] = (first_unit + np - 1) / chunk - cf[s] + 1;
+      cf[s] = quotient(first_unit, chunk);
+      parts[s] = quotient(first_unit + np - 1, chunk) - cf[s] + 1;
     }
     __syncthreads();  // the CTA's partial states are written
     if (tid == 0 && open_row[0] >= 0) sm.arrived[0] = static_cast<int>(atom_add_acq_rel_gpu_u32(P.counter + cf[0], 1u));
