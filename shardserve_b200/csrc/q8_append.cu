@@ -15,7 +15,14 @@
 // and the pages that an earlier window owns.  T slots per CTA cost little while a window holds
 // 1/148 of the call: 8192 tokens are 64 KB per SM, ~1 us.
 //
-// Bound: HBM for prompts (3 bytes per value), latency for decode steps.
+// A warp handles a (page, head, tensor): one pass finds the largest |x|, and the rows, kept in
+// registers, are encoded in the second; lane = eight consecutive values.
+//
+// Bound: HBM for prompts (3 bytes per value), latency for decode steps.  With the read-back that
+// follows it, 16,000 prompt tokens of 8 KV heads of 128: 60 us for 196 MB (30 at the copy's rate);
+// there a CTA's 32 warps take four to five blocks each one after another, and each block's chain (row
+// list, values, maximum, codes) is what the time is made of.  64 decode rows: 9.4 us the two calls,
+// two launches and four dependent trips to memory each.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -4,24 +4,37 @@
 //   x_ih = (q_h . Kc_i) * ks_page * sm_scale * log2 e + log2(vs_page),   w_ih = 2^(x_ih - r_h)
 //   O_h  = sum_i w_ih Vc_i,   l_h = sum_i w_ih / vs_page,   out_h = O_h / l_h
 // with Kc / Vc the codes and ks / vs their page's scales: the V scale rides in the exponent, so
-// the products see the codes themselves, exact in fp16 and tf32, and no page's scale costs
-// another page precision.  r_h is raised only when a weight would pass 2^20, found by a vote: most
-// pages need no warp reduction.  Q.K is an fp16 product (q is exact there once its row's power of
-// two is taken out).  The weights are rounded to tf32: 11 bits like fp16, but with fp32's range
-// (fp16 would flush weights 2^30 below the row's largest, which are all there is of an output
-// dimension whose leading keys hold code 0; bf16 has the range and three bits less).  Everything
-// else is fp32.
+// the products see the codes themselves and no page's scale costs another page precision.  r_h is
+// raised only when a weight would pass 2^20, found by a vote: most pages need no warp reduction.
 //
-// What bounds it: HBM (2 * head_dim bytes per key and KV head), once the ~300 instructions per
-// 4 KiB page (two thirds of them widen bytes) stay below the issue rate.
+// Q.K.  The row's power of two is taken out of q.  Integer codes of up to 8 query heads per KV head:
+// q is rounded to 21 bits below it and written as three signed digits of base 256, and the product
+// of each digit with the codes is an integer MMA on the bytes as they stand (exact; widening them
+// costs two ALU instructions per pair of codes more than the third digit's products).  Two of the
+// digits share one MMA: rows 0-7 and 8-15 of its A operand.  Else (e4m3 codes, more heads, whose rows
+// fill A): an fp16 product, which holds q and the codes exactly.
+// P.V.  tf32: the weights keep 11 bits as in fp16, but over fp32's range (fp16 would flush weights
+// 2^30 below the row's largest, which are all there is of an output dimension whose leading keys hold
+// code 0; bf16 has the range and three bits less).  The codes are exact.  Everything else is fp32.
+//
+// What bounds it: HBM (2 * head_dim bytes per key and KV head) for what a call adds in length, 5.4 TB/s
+// (6.8 where the codes stand in L2: 680 cycles a page and scheduler), and a fixed 15 us.  64 rows of
+// context U[128, 4096], 16 query and 2 KV heads of 128, int8: 71 MB, 25.5 us a call, of which copying
+// takes 10.9; 32 rows of 16 k to 32 k keys, 8 query heads and 1 KV head: 196 MB, 52 us (29.9).  The
+// fixed part, from the last CTA of the call before: 3 us until its successor has its shares, up to 4
+// until its first pages are in, 2 in each of the two joins, the rest the spread of the CTAs' ends.
+// (Fetching the first pages into L2 before the wait for the call before moved it by -1 to +1 us, case by
+// case; whole 128-byte lines of K per copy, exchanged between lanes, by less than 1 %; codes widened with
+// fp32 additions of fp16 operands instead of byte permutations, by nothing.)
 //
 // Data path.  A warp streams its own pages: every lane copies (cp.async) the 16-byte pieces that it
 // will use itself into slots of its own, three pages ahead, and loads them back in fragment order;
 // no other lane reads them, so nothing synchronises but the lane's own copy groups.  (With the next
 // page in registers instead, issued piece by piece as registers came free, about 32 KiB per SM were
-// in flight and a page took a warp 4,400 cycles: 31 us for the 64-row batch.)  The order of head_dim and of the keys inside a product is
-// free as long as both operands agree.  Lane (g, t) = (lane / 4, lane % 4):
-//   S = Q K^T       m16n8k16, M = query heads (of one KV head), N = 8 keys.  The lane loads bytes
+// in flight and a page took a warp 4,400 cycles: 31 us for the 64 rows.)  The order of head_dim and
+// of the keys inside a product is free as long as both operands agree.  Lane (g, t) = (lane / 4,
+// lane % 4):
+//   S = Q K^T       M = query heads (of one KV head), N = 8 keys.  The lane loads bytes
 //                   [64 c + 16 t, +16) of keys g and g + 8 (16-byte loads); Q is loaded to match.
 //   O^T = V^T P^T   m16n8k8, M = 16 values of head_dim, N = 8 heads, K = 8 keys.  The lane loads
 //                   bytes [D/8 g, +D/8) of keys 2t, 2t+1, 2t+8, 2t+9, which are the keys whose
@@ -29,11 +42,11 @@
 // A lane's V bytes are consecutive, so its outputs are 32 consecutive bytes of an output row.
 //
 // Work split.  Unit = (row, page), row = (token, KV head).  One CTA per SM takes an equal run of
-// units and every warp an equal run of the CTA's.  A row inside a warp's run goes straight to the
-// output.  Rows cut by warp boundaries leave fp32 partial states in shared memory, combined by
-// the CTA; rows cut by CTA boundaries leave one state per CTA in the workspace, and the CTA that
-// arrives last at the row's counter combines them in CTA order (no CTA waits for another one, and
-// the bits do not depend on who arrives last).
+// units and every warp a run of the CTA's, cut at the rows' ends where that costs no warp more than
+// two units.  A row inside a warp's run goes straight to the output.  Rows cut by warp boundaries leave
+// fp32 partial states in shared memory, combined by the CTA; rows cut by CTA boundaries leave one
+// state per CTA in the workspace, and the CTA that arrives last at the row's counter combines them in
+// CTA order (no CTA waits for another one, and the bits do not depend on who arrives last).
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -78,7 +91,7 @@ struct Piece {  // a warp's part of a row that others share
 // a / b for 0 <= a, 0 < b: an fp32 quotient, put right by its remainder.
 __device__ __forceinline__ int quotient(int a, int b) {
   int q = __float2int_rz(__fdividef(static_cast<float>(a), static_cast<float>(b)));
-  int r = a - q * b;
+  int r = static_cast<int>(static_cast<unsigned>(a) - static_cast<unsigned>(q) * static_cast<unsigned>(b));
   while (r < 0) { --q; r += b; }
   while (r >= b) { ++q; r -= b; }
   return q;
@@ -303,9 +316,10 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     return;
   }
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
-  // Shares of the warps, in unit order.  A row's end inside a warp's share costs it about two units (its
-  // copies run dry and its queries change), and the CTA waits for its slowest warp; so rows get warps of
-  // their own, as long as no warp then holds more than two units above an even share.
+  // Shares of the warps, in unit order.  A row's end inside a warp's share costs it more than two units
+  // (its copies run dry and its queries change: 4 us), and the CTA waits for its slowest warp; so rows
+  // get warps of their own, as long as no warp then holds more than two units above an even share (64
+  // rows 27.5 -> 25.9 us, 250 rows of head_dim 64 40.0 -> 37.6).
   auto token_of = [&](int unit, int lo) {  // the last token that begins at or before the unit
     for (int hi = P.tn; hi - lo > 1;) {
       const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;

@@ -6,9 +6,13 @@
 //   O_i  = sum_j w_ij Vc_j,   l_i = sum_j w_ij / vs_page,   out_i = O_i / l_i
 // K codes and q (its row's power of two taken out) are fp16, which holds both exactly; the weights
 // and the V codes are tf32: fp16 has the bits but not the range (weights 2^30 below the row's
-// largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.  So
-// Q.K costs 512 and P.V 1024 tensor cycles per 128 x 128 x 128, and the tensor floor of a tile pair
-// and key block is 3072 cycles.
+// largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.
+//
+// What bounds it: the tensor pipe's issue rate.  A 128 x 128 x 16 fp16 product took 107 cycles and a
+// 128 x 128 x 8 tf32 product with A in TMEM 75 (measured alone), so a pair of tiles needs 2 * (8 * 107
+// + 16 * 75) = 4,100 cycles per key block of 128; the loop runs at 6,300, the rest being waits of the
+// four products and two softmaxes on one another.  A 3001-token prompt (16 query and 2 KV heads of
+// 128; 37 GFLOP) takes 95 us, of which about 6 are the start, 8 the join of cut windows.
 //
 // A window is up to 2 * (128 / group) tokens of one run: two tiles of 128 rows (token, query head
 // of the KV head) that share every K / V block.  A work item is (window, KV head, range of
@@ -19,20 +23,21 @@
 //   O_t += P_t V_j       kind::tf32, A = P_t from TMEM, B = V_j^T in shared memory
 // in the order S_0(j+1), O_1(j), S_1(j+1), O_0(j+1): each softmax has two products' time.
 // The codes are widened on their way into shared memory: K rows to 128-byte swizzled fp16 lines by
-// three warps, V transposed (lane = key) to lines of 32 keys in fp32 by eight (a page
-// of a block each); a page's registers are loaded for the next block as soon as it is stored.
+// three warps, V transposed (lane = key) to lines of 32 keys in fp32 by eight (a page of a block
+// each); a page's registers are loaded for the next block as soon as it is stored.
 //
 // The roles' loops are kept rolled and small: with everything unrolled each warp ran at about one
 // instruction in five cycles, the rate at which instructions came from the cache, a key block took
-// 10,000 cycles whatever was taken out of it, and the prompt case 123 us.
+// 10,000 cycles whatever was taken out of it, and the prompt took 123 us.
 //
 // Scheduling.  Every CTA lists the launch's windows (a scan over its tokens) and takes an equal run
-// of the units (window, KV head, block; beginning a window counts as
-// two blocks), so that all finish together; a window that a run's end
-// cuts leaves fp32 states in the workspace, joined by q8_merge_kernel.  (Whole windows taken from
-// a counter, long ones first and the longest cut in two, left 12 to 19 blocks per CTA in the
-// prompt case.)  The roles walk the CTA's run on their own: a producer is in the next window while
-// the softmax warps finish the last.
+// of the units (window, KV head, block; beginning a window counts as two blocks), so that all finish
+// together; a window that a run's end cuts leaves fp32 states in the workspace, joined by
+// q8_merge_kernel.  (Whole windows taken from a counter, long ones first and the longest cut in two,
+// left 12 to 19 blocks per CTA in that prompt: 110 us.)  The roles walk the CTA's run on their own: a
+// producer is in the next window while the softmax warps finish the last.  A call that also has
+// tokens outside runs launches the split-K kernel first, and the two share out the SMs by their work
+// (q8_split): 56 decode rows beside 8 chunks of 512 tokens 136 -> 126 us.
 //
 // Warps: 0 MMA issuer, 1-3 K, 4-11 V, 12-15 softmax of tile 0, 16-19 of tile 1 (TMEM lane quadrant =
 // warp % 4), up to 96 registers a thread.
