@@ -114,3 +114,28 @@ def test_positions_out_of_order_in_a_run():
     # Other windows, other orders of summation: both within the tolerance of the same rows.
     diff = (out.double() - sorted_out[torch.from_numpy(order).to(DEV)].double()).abs()
     assert diff.max().item() <= 4 * (2.0 ** -9 + 2.0 ** -10) * float(v.float().abs().max() * s[:, :, 1].max())
+
+
+@pytest.mark.parametrize("pad", [1, 31, 40])
+@pytest.mark.parametrize("kvh", [1, 2, 40])
+def test_padding_between_rows(pad, kvh):
+    """Padding tokens in the middle of a batch: zero rows, and the others as without them."""
+    rng = np.random.RandomState(pad)
+    spans = [(int(n) - 1, 1) for n in rng.randint(1, 900, 24)]
+    pages = sum((c + n + 15) // 16 for c, n in spans) + 3
+    k, v, s = make_pool(pages, kvh, 64, "int8", seed=pad)
+    tables, seqs, pos, _ = batch(spans, pages, seed=pad)
+    q = torch.randn(len(seqs) * (pad + 1), 2 * kvh, 64, device=DEV).bfloat16()
+    real = torch.arange(len(seqs), device=DEV) * (pad + 1) + pad // 2
+    wide_seqs = torch.full((len(q),), -1, dtype=torch.int32, device=DEV)
+    wide_pos = torch.full((len(q),), -1, dtype=torch.int64, device=DEV)
+    wide_seqs[real], wide_pos[real] = dev(seqs, torch.int32), dev(pos, torch.int64)
+    bt = dev(tables, torch.int32)
+    K.device_errors(torch.device(DEV))
+    out = sb.ragged_attention_q8(q, k, v, s, bt, wide_seqs, wide_pos, 0.125)
+    alone = sb.ragged_attention_q8(q[real], k, v, s, bt, dev(seqs, torch.int32), dev(pos, torch.int64), 0.125)
+    assert K.device_errors(torch.device(DEV)) == 0
+    assert not out[wide_seqs == -1].any()
+    # Other shares of the warps, other orders of summation: both within the tolerance of the same rows.
+    diff = (out[real].double() - alone.double()).abs().max().item()
+    assert diff <= 4 * (2.0 ** -9 + 2.0 ** -10) * float(v.float().abs().max() * s[:, :, 1].max())
