@@ -839,7 +839,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (P.split) griddep_wait();  // this grid ends after the split-K kernel
 }
 
-// Joins the states of cut windows: one thread per (row, 16 values).
+// Joins the states of cut windows: one thread per (row, 16 values).  (Joined by the CTA that ends last,
+// from TMEM and the other part's state: 2 us slower, on the tail of the launch.)
 template <int D>
 __global__ void __launch_bounds__(256) q8_merge_kernel(const PrefillParams P) {
   griddep_wait();
