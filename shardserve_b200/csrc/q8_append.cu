@@ -271,51 +271,78 @@ __global__ void __launch_bounds__(1024, 1)
   }
 }
 
-// One thread per 8 values of a K row and of the V row (or per value where rows are not 8-byte
-// addressable).
-template <int FMT, bool VEC>
-__global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadArgs a) {
+// Pieces of 8 values of a K row and of the V row (or one value where rows are not 8-byte addressable),
+// two of a thread in flight.  A CTA takes `rows` whole rows, so that a piece's row is a 32-bit product
+// away (magic = ceil(2^32 / pieces of a row), exact for the few thousand pieces of a CTA that holds more
+// than one row).
+template <int D, int FMT, bool VEC>
+__global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadArgs a, int rows, unsigned magic) {
   griddep_wait();
-  constexpr int E = VEC ? 8 : 1;
-  const unsigned per_row = static_cast<unsigned>(a.p.KVH * a.p.D / E);
+  constexpr int E = VEC ? 8 : 1, U = 2;
+  const int per_row = a.p.KVH * (D / E);
   const long long limit = a.p.N * kPage;
-  // A CTA takes 256 consecutive pieces at a time: one 64-bit division for all of them.
-  for (long long b = static_cast<long long>(blockIdx.x) * 256; b < a.T * per_row;
-       b += static_cast<long long>(gridDim.x) * 256) {
-    const long long t0 = b / per_row;
-    const unsigned off = static_cast<unsigned>(b - t0 * per_row) + threadIdx.x;
-    const long long t = t0 + off / per_row;
-    const int e = static_cast<int>(off % per_row) * E, h = e / a.p.D, d = e % a.p.D;
-    if (t >= a.T) continue;
-    const long long slot = ld_index(a.slots, a.slots64, t);
-    const bool ok = slot >= 0 && slot < limit;
-    if (!ok && slot != -1 && a.err && e == 0) atomicOr(a.err, SS_DEVERR_SLOT);
-    const long long page = ok ? slot / kPage : 0, row = ok ? slot % kPage : 0;
-    const float* sp = a.p.scales + page * a.p.s_sn + h * a.p.s_sh;
-    const uint8_t* ks = a.p.k + page * a.p.k_sn + row * a.p.k_ss + h * a.p.k_sh + d * a.p.k_sd;
-    const uint8_t* vs = a.p.v + page * a.p.v_sn + row * a.p.v_ss + h * a.p.v_sh + d * a.p.v_sd;
-    __nv_bfloat16* kd = a.k + t * a.k_st + h * a.k_sh + d * a.k_sd;
-    __nv_bfloat16* vd = a.v + t * a.v_st + h * a.v_sh + d * a.v_sd;
-    const float sk = ok ? sp[0] : 0.f, sv = ok ? sp[a.p.s_sw] : 0.f;
-    if constexpr (VEC) {
-      const uint2 kc = ok ? *reinterpret_cast<const uint2*>(ks) : make_uint2(0, 0);
-      const uint2 vc = ok ? *reinterpret_cast<const uint2*>(vs) : make_uint2(0, 0);
-      auto four = [](uint32_t w, float s, uint32_t& lo, uint32_t& hi) {
-        uint32_t f[4];
-        widen_f32<FMT>(w, f);
-        lo = pack_bf16(__uint_as_float(f[0]) * s, __uint_as_float(f[1]) * s);
-        hi = pack_bf16(__uint_as_float(f[2]) * s, __uint_as_float(f[3]) * s);
-      };
-      uint4 o;
-      four(kc.x, sk, o.x, o.y);
-      four(kc.y, sk, o.z, o.w);
-      *reinterpret_cast<uint4*>(kd) = o;
-      four(vc.x, sv, o.x, o.y);
-      four(vc.y, sv, o.z, o.w);
-      *reinterpret_cast<uint4*>(vd) = o;
-    } else {
-      *kd = __float2bfloat16(ok ? q8_decode(FMT, *ks) * sk : 0.f);
-      *vd = __float2bfloat16(ok ? q8_decode(FMT, *vs) * sv : 0.f);
+  const long long t0 = static_cast<long long>(blockIdx.x) * rows;
+  const int pieces = static_cast<int>(min(static_cast<long long>(rows), a.T - t0)) * per_row;
+  for (int i0 = threadIdx.x; i0 < pieces; i0 += U * 256) {
+    long long t[U], slot[U];
+    int e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * 256, pieces - 1);
+      const int r = rows == 1 ? 0 : static_cast<int>(__umulhi(static_cast<unsigned>(i), magic));
+      t[u] = t0 + r;
+      e[u] = (i - r * per_row) * E;
+      slot[u] = ld_index(a.slots, a.slots64, t[u]);
+    }
+    float sk[U], sv[U];
+    uint2 kc[U], vc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool ok = slot[u] >= 0 && slot[u] < limit;
+      if (!ok && slot[u] != -1 && a.err && e[u] == 0) atomicOr(a.err, SS_DEVERR_SLOT);
+      const long long page = ok ? slot[u] / kPage : 0;
+      const int row = ok ? static_cast<int>(slot[u] % kPage) : 0, h = e[u] / D, d = e[u] % D;
+      const float* sp = a.p.scales + page * a.p.s_sn + h * a.p.s_sh;
+      const uint8_t* ks = a.p.k + page * a.p.k_sn + row * a.p.k_ss + h * a.p.k_sh + d * a.p.k_sd;
+      const uint8_t* vs = a.p.v + page * a.p.v_sn + row * a.p.v_ss + h * a.p.v_sh + d * a.p.v_sd;
+      sk[u] = sv[u] = 0.f;
+      kc[u] = vc[u] = make_uint2(0, 0);
+      if (ok) {
+        sk[u] = sp[0];
+        sv[u] = sp[a.p.s_sw];
+        if constexpr (VEC) {
+          kc[u] = *reinterpret_cast<const uint2*>(ks);
+          vc[u] = *reinterpret_cast<const uint2*>(vs);
+        } else {
+          kc[u].x = *ks;
+          vc[u].x = *vs;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * 256 >= pieces) break;
+      const int h = e[u] / D, d = e[u] % D;
+      __nv_bfloat16* kd = a.k + t[u] * a.k_st + h * a.k_sh + d * a.k_sd;
+      __nv_bfloat16* vd = a.v + t[u] * a.v_st + h * a.v_sh + d * a.v_sd;
+      if constexpr (VEC) {
+        auto four = [](uint32_t w, float s, uint32_t& lo, uint32_t& hi) {
+          uint32_t f[4];
+          widen_f32<FMT>(w, f);
+          lo = pack_bf16(__uint_as_float(f[0]) * s, __uint_as_float(f[1]) * s);
+          hi = pack_bf16(__uint_as_float(f[2]) * s, __uint_as_float(f[3]) * s);
+        };
+        uint4 o;
+        four(kc[u].x, sk[u], o.x, o.y);
+        four(kc[u].y, sk[u], o.z, o.w);
+        *reinterpret_cast<uint4*>(kd) = o;
+        four(vc[u].x, sv[u], o.x, o.y);
+        four(vc[u].y, sv[u], o.z, o.w);
+        *reinterpret_cast<uint4*>(vd) = o;
+      } else {
+        *kd = __float2bfloat16(q8_decode(FMT, static_cast<uint8_t>(kc[u].x)) * sk[u]);
+        *vd = __float2bfloat16(q8_decode(FMT, static_cast<uint8_t>(vc[u].x)) * sv[u]);
+      }
     }
   }
 }
@@ -370,18 +397,27 @@ cudaError_t launch_q8_read(const Q8ReadArgs& a, cudaStream_t stream) {
                    rows_ok(a.v, 2, 16, a.v_st, a.v_sh, 0, a.v_sd) &&
                    rows_ok(a.p.k, 1, 8, a.p.k_sn, a.p.k_ss, a.p.k_sh, a.p.k_sd) &&
                    rows_ok(a.p.v, 1, 8, a.p.v_sn, a.p.v_ss, a.p.v_sh, a.p.v_sd);
-  const long long work = a.T * a.p.KVH * a.p.D / (vec ? 8 : 1);
+  // Two pieces per thread once the CTAs fill the SMs with one.
+  const long long per_row = static_cast<long long>(a.p.KVH) * a.p.D / (vec ? 8 : 1);
+  const long long pieces = a.T * per_row > 148ll * 8 * 256 ? 512 : 256;
+  const int rows = static_cast<int>(std::max<long long>(pieces / per_row, 1));
+  const unsigned magic = static_cast<unsigned>(((1ull << 32) + per_row - 1) / per_row);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(std::max<long long>((work + 255) / 256, 1), 148 * 64)));
+  cfg.gridDim = dim3(static_cast<unsigned>((a.T + rows - 1) / rows));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   one_after_another(cfg, attr);
-  if (a.p.fmt == SS_CODE_INT8)
-    return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_INT8, true>, a)
-               : cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_INT8, false>, a);
-  return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_E4M3, true>, a)
-             : cudaLaunchKernelEx(&cfg, q8_read_kernel<SS_CODE_E4M3, false>, a);
+#define SS_Q8_READ(D, FMT)                                                                         \
+  return vec ? cudaLaunchKernelEx(&cfg, q8_read_kernel<D, FMT, true>, a, rows, magic)              \
+             : cudaLaunchKernelEx(&cfg, q8_read_kernel<D, FMT, false>, a, rows, magic)
+  if (a.p.D == 128) {
+    if (a.p.fmt == SS_CODE_INT8) SS_Q8_READ(128, SS_CODE_INT8);
+    SS_Q8_READ(128, SS_CODE_E4M3);
+  }
+  if (a.p.fmt == SS_CODE_INT8) SS_Q8_READ(64, SS_CODE_INT8);
+  SS_Q8_READ(64, SS_CODE_E4M3);
+#undef SS_Q8_READ
 }
 
 }  // namespace ss
