@@ -64,7 +64,11 @@ constexpr int kNB = 128;           // keys of a block
 constexpr int kPages = kNB / kPage;
 constexpr int kMaxTokP = 8192;     // tokens per launch
 static_assert((kMaxTokP + kThreads - 1) / kThreads <= 32, "a thread's tokens fit a mask");
-constexpr int kMaxWin = kMaxTokP / kQ8MinRun;  // windows per launch
+// Windows per launch.  A run that lies inside the launch has kQ8MinRun tokens or more for each of its
+// windows (the shortest windows take 16 tokens).  The run cut by the launch's beginning and the one cut by
+// its end may hold a single token here: x of them, y of the other and 8-token runs between, x + y = 8,
+// list one window more than the launch has eighths.
+constexpr int kMaxWin = kMaxTokP / kQ8MinRun + 1;
 constexpr int kMinPart = 4;        // units: smallest share of a CTA
 constexpr int kHead = 2;           // units that beginning a window costs (Q, first and last waits)
 constexpr float kSlackP = 20.f;
