@@ -516,8 +516,26 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max(static_cast<int>(top >> 7) - 127, -104), 126);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+      // Rows below 2^-63 are raised by 2^64 (exact, subnormals too), so that their power of two has a
+      // normal reciprocal.
+      const bool tiny = top < 64u << 7;
+      if (tiny) {
+        const __nv_bfloat162 grow = __float2bfloat162_rn(0x1p64f);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&raw[n][c][w]), grow);
+            raw[n][c][w] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+        top = __float_as_uint(__uint_as_float(top << 16) * 0x1p64f) >> 16;
+      }
+      // bf16's largest is 127, which the digits need as it is (one less, and 21 bits would not hold them);
+      // 2^126 below them, fp16 values stay below 4 and the reciprocal normal.
+      const int e = min(max(static_cast<int>(top >> 7) - 127, -104), kDigits ? 127 : 126);
+      // 2^(e - 21), which is a normal number where 2^e times the factor may not be.
+      float up = __uint_as_float(static_cast<uint32_t>(127 + e - 21) << 23) * a.scale_log2;
+      if (tiny) up *= 0x1p-64f;
       if constexpr (kDigits) {
         // round(q 2^(21 - e)) + 0x808080 by an addition whose sum's low bits are that integer; its
         // bytes, each less 128, are the digits.
@@ -537,7 +555,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
             qd[1][c][w >> 1][w & 1] = __byte_perm(l01, l23, 0x7632) ^ 0x80808080u;
             qd[2][c][w >> 1][w & 1] = __byte_perm(l01, l23, 0x5410) ^ 0x80808080u;
           }
-        qs[n] = top >= 0x7f80u ? CUDART_NAN_F : up * 0x1p-21f;
+        qs[n] = top >= 0x7f80u ? CUDART_NAN_F : up;
       } else {
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
@@ -546,7 +564,7 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
           for (int w = 0; w < 8; ++w)
             qf[n][c][w >> 1][w & 1] = pack_f16(__uint_as_float(raw[n][c][w] << 16) * down,
                                                __uint_as_float(raw[n][c][w] & 0xffff0000u) * down);
-        qs[n] = up;
+        qs[n] = up * 0x1p21f;
       }
     }
 
