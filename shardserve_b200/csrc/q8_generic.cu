@@ -3,7 +3,7 @@
 // are not 16-byte addressable, more than 16 query heads per KV head) and is not tuned: codes are
 // read byte by byte and every query head reads its KV head's codes itself.
 //
-//   x_i = (q . K_i) * K scale * sm_scale * log2(e),   m, l, acc: base-2 online softmax in fp32,
+//   x_i = (q . K_i) * (K scale * sm_scale * log2(e)),   m, l, acc: base-2 online softmax in fp32,
 //   acc += 2^(x_i - m) * V scale * V_i
 #include <cuda_bf16.h>
 #include <math_constants.h>
@@ -35,6 +35,17 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) q8_generic_kernel(const Q
     qv[i] = __bfloat162float(qp[(lane + 32 * i) * a.q_sd]);
     acc[i] = 0.f;
   }
+  // The row's power of two is taken out of q: products with codes neither overflow nor lose bits where
+  // the scores themselves do not.
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) top = fmaxf(top, fabsf(qv[i]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) qv[i] *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
   float m = -CUDART_INF_F, l = 0.f;
   for (int pg = 0; pg < ti.npages; ++pg) {
     const long long pid = ld_index(a.bt, a.bt64, ti.seq * a.bt_sb + pg * a.bt_sn);
@@ -42,7 +53,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) q8_generic_kernel(const Q
     if (!valid && lane == 0) atomicOr(a.err, SS_DEVERR_PAGE);
     const float* sp = g.p.scales + pid * g.p.s_sn + kvh * g.p.s_sh;
     const float ks = valid ? sp[0] : 0.f, vs = valid ? sp[g.p.s_sw] : 0.f;
-    const float f = ks * a.scale_log2;
+    const float f = ks * up;
     const int nk = min(kPage, ti.L - pg * kPage);
     for (int s = 0; s < nk; ++s) {
       float part = 0.f, vv[PER];

@@ -25,7 +25,8 @@ def test_most_windows_of_a_launch(lead, heads, kvh, d):
 
 # ---- queries at both ends of bf16's range -----------------------------------------------------
 @pytest.mark.parametrize("exponent", [-133, -130, -126, -112, -105, -64, -63, 0, 126, 127])
-@pytest.mark.parametrize("codes,heads,kvh", [("int8", 16, 2), ("int8", 16, 1), ("e4m3", 4, 2)])
+@pytest.mark.parametrize("codes,heads,kvh", [("int8", 16, 2), ("int8", 16, 1), ("e4m3", 4, 2),
+                                             ("int8", 24, 1)])
 def test_query_exponents(exponent, codes, heads, kvh):
     """Query rows whose largest value has this exponent, up to bf16's largest finite numbers and
     down to its subnormals, of both signs, with finite scores: decode rows and a prompt chunk."""
