@@ -312,8 +312,8 @@ SS_API int ss_kv_read_q8(const void* k_pool, const int64_t k_pool_strides[4], co
                   const int64_t v_out_strides[3], int64_t tokens, int64_t num_pages, int kv_heads,
                   int head_dim, void* workspace, void* stream);
 
-/* Workspace size of ss_ragged_paged_attention_q8 on `device` for this geometry (any number of
- * tokens).  A workspace must be zero when it is first used and is left ready for the next call;
+/* Workspace size of ss_ragged_paged_attention_q8 on `device`, the same for every geometry and number
+ * of tokens.  A workspace must be zero when it is first used and is left ready for the next call;
  * it is not shared with ss_ragged_paged_attention's, nor by calls that may overlap in time. */
 SS_API int ss_q8_workspace_bytes(int device, int heads, int kv_heads, int head_dim, size_t* bytes);
 

@@ -380,38 +380,27 @@ at::Tensor rope_kv_append(const at::Tensor& q, const at::Tensor& k, const at::Te
 // ---- 8-bit pool -----------------------------------------------------------------------------
 // Its workspace (error word, row counters, split-K partial states) is a second per-device
 // buffer: the counters must stay zero between calls, and the bf16 path's scratch moves with the
-// call's shape.
+// call's shape.  Its size depends on the device alone, so the first call of any kind makes the
+// buffer that every later one uses: error bits stay in one place, and any call prepares the capture of
+// all of them.
 auto* g_ws_q8 = new std::map<int, at::Tensor>();
-auto* g_ws_q8_need = new std::map<std::tuple<int, int, int, int>, size_t>();
 
-at::Tensor ensure_workspace_q8(const at::Device& dev, int heads, int kv_heads, int head_dim,
-                               const char* what) {
+at::Tensor ensure_workspace_q8(const at::Device& dev, const char* what) {
   const int idx = dev.index();
   std::lock_guard<std::mutex> lock(g_ws_mu);
-  size_t need = 0;
-  if (heads > 0) {
-    const auto key = std::make_tuple(idx, heads, kv_heads, head_dim);
-    auto nit = g_ws_q8_need->find(key);
-    if (nit != g_ws_q8_need->end()) {
-      need = nit->second;
-    } else {
-      check_rc(p_ws_bytes_q8(idx, heads, kv_heads, head_dim, &need), "ss_q8_workspace_bytes");
-      (*g_ws_q8_need)[key] = need;
-    }
-  }
   auto it = g_ws_q8->find(idx);
-  if (it != g_ws_q8->end() && static_cast<size_t>(it->second.numel()) >= need) return it->second;
+  if (it != g_ws_q8->end()) return it->second;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(idx).stream(), &status) ==
           cudaSuccess &&
       status != cudaStreamCaptureStatusNone)
     throw std::runtime_error(std::string(what) +
-                             ": workspace must grow during CUDA graph capture; run the same "
-                             "shapes once before capturing");
-  // Room for any geometry on the device, so that the buffer is not replaced later.
-  const int64_t size = std::max<int64_t>(static_cast<int64_t>(need), int64_t{8} << 20);
-  at::Tensor ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(dev));
-  if (it != g_ws_q8->end()) g_ws_retired->push_back(it->second);
+                             ": the workspace cannot be made during CUDA graph capture; run one "
+                             "8-bit call on the device before capturing");
+  size_t need = 0;
+  check_rc(p_ws_bytes_q8(idx, 1, 1, 128, &need), "ss_q8_workspace_bytes");
+  at::Tensor ws = at::zeros({static_cast<int64_t>(need)},
+                            at::TensorOptions().dtype(at::kByte).device(dev));
   (*g_ws_q8)[idx] = ws;
   return ws;
 }
@@ -435,7 +424,7 @@ void* err_word_q8(const at::Device& dev) {
           cudaSuccess ||
       status != cudaStreamCaptureStatusNone)
     return nullptr;
-  return ensure_workspace_q8(dev, 0, 0, 0, "kv_append_q8").data_ptr();
+  return ensure_workspace_q8(dev, "kv_append_q8").data_ptr();
 }
 
 // Checks the pools and their scales; returns SS_CODE_*.
@@ -491,8 +480,7 @@ at::Tensor ragged_attention_q8(const at::Tensor& q, const at::Tensor& k_pool,
   const at::Tensor pos = flat_index(positions);
   const c10::cuda::OptionalCUDAGuard guard(q.device());
   at::Tensor out = at::empty_like(q);
-  const at::Tensor ws =
-      ensure_workspace_q8(q.device(), heads, kv_heads, head_dim, "ragged_attention_q8");
+  const at::Tensor ws = ensure_workspace_q8(q.device(), "ragged_attention_q8");
   const Strides<3> qs(q), os(out), ss(scales);
   const Strides<4> ks(k_pool), vs(v_pool);
   const Strides<2> bs(block_tables);
@@ -604,7 +592,7 @@ py::dict build_block_tables(const at::Tensor& cached_lens, const at::Tensor& new
   const at::Tensor last = take_out("last", at::kLong, rows);
   const at::Tensor lens = take_out("lens", at::kInt, rows);
   const at::Tensor head = take_out("free_head", at::kInt, 1);
-  const at::Tensor ws = ensure_workspace_q8(dev, 0, 0, 0, "build_block_tables");
+  const at::Tensor ws = ensure_workspace_q8(dev, "build_block_tables");
   const Strides<2> bs(block_tables);
   check_rc(p_block_tables(cl.data_ptr(), c64, nl.data_ptr(), n64, block_tables.data_ptr(), bs.v,
                           rows, block_tables.size(1), b64, fp.data_ptr(), f64, fp.numel(),

@@ -1,9 +1,14 @@
 """8-bit pool on the GPU at the edges of what its kernels list and hold."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
 import shardserve_b200 as sb
+from shardserve_b200 import _native
 from test_gpu_quantized import DEV, batch, check_attention, dev, make_pool
 from test_gpu_quantized_shapes import check
 
@@ -46,3 +51,54 @@ def test_query_exponents(exponent, codes, heads, kvh):
     out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
                                  dev(pos, torch.int64), sm_scale)
     check_attention(out, q, k, v, s, tables, seqs, pos, sm_scale)
+
+
+# ---- the workspace ------------------------------------------------------------------------------
+FRESH = """
+import sys
+import torch
+sys.path.insert(0, {root!r})
+import shardserve_b200 as sb
+from shardserve_b200 import kernel as K
+k = torch.zeros(4, 16, 2, 128, dtype=torch.int8, device="cuda:0")
+v, s = torch.zeros_like(k), torch.ones(4, 2, 2, device="cuda:0")
+x = torch.ones(3, 2, 128, device="cuda:0").bfloat16()
+q = torch.ones(3, 16, 128, device="cuda:0").bfloat16()
+i = torch.zeros(3, dtype=torch.int32, device="cuda:0")
+bt = torch.zeros(1, 4, dtype=torch.int32, device="cuda:0")
+attend = lambda: sb.ragged_attention_q8(q, k, v, s, bt, i, i, 0.1)
+{body}
+print("fine")
+"""
+
+
+def fresh_process(body):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = FRESH.format(root=root, body=body)
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "fine", run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("first", ["sb.kv_append_q8(k, v, s, x, x, i + 999)", "sb.kv_read_q8(k, v, s, i + 999)",
+                                   "sb.build_block_tables(i - 5, i, bt.expand(3, 4).clone(), i, i[:1], 0)"])
+def test_error_bits_outlive_the_first_attention(first):
+    """Bits set by the first call of a process are still there after the first attention."""
+    bit = _native.SS_DEVERR_POS if "tables" in first else _native.SS_DEVERR_SLOT
+    fresh_process(f"{first}\nattend()\nassert K.device_errors(torch.device('cuda:0')) == {bit}")
+
+
+def test_any_first_call_prepares_a_capture():
+    """After an append alone, tables, append, attention and read-back can be captured, and an append's
+    bits from inside the graph are seen."""
+    fresh_process("""
+sb.kv_append_q8(k, v, s, x, x, i)
+slots = i + 999
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    sb.build_block_tables(i[:1], i[:1], bt, i, i[:1], 2)
+    sb.kv_append_q8(k, v, s, x, x, slots)
+    out = attend()
+    back = sb.kv_read_q8(k, v, s, i)
+graph.replay()
+assert torch.equal(out, attend()) and torch.equal(back[0], sb.kv_read_q8(k, v, s, i)[0])
+assert K.device_errors(torch.device('cuda:0')) == 8  # SS_DEVERR_SLOT""")
