@@ -18,14 +18,15 @@
 // code 0; bf16 has the range and three bits less).  The codes are exact.  Everything else is fp32.
 //
 // What bounds it: HBM (2 * head_dim bytes per key and KV head) for what a call adds in length, 5.4 TB/s
-// (6.8 where the codes stand in L2: 680 cycles a page and scheduler), and a fixed 15 us.  64 rows of
-// context U[128, 4096], 16 query and 2 KV heads of 128, int8: 71 MB, 25.5 us a call, of which copying
-// takes 10.9; 32 rows of 16 k to 32 k keys, 8 query heads and 1 KV head: 196 MB, 52 us (29.9).  The
-// fixed part, from the last CTA of the call before: 3 us until its successor has its shares, up to 4
+// (6.8 where the codes stand in L2: 680 cycles a page and scheduler), and a fixed 18 us.  64 rows of
+// context U[128, 4096], 16 query and 2 KV heads of 128, int8: 71 MB, 28.7 us a call, of which copying
+// takes 10.9; 32 rows of 16 k to 32 k keys, 8 query heads and 1 KV head: 196 MB, 55 us (29.9).  The
+// fixed part, from the last CTA of the call before: the start until its successor has its shares, up to 4 us
 // until its first pages are in, 2 in each of the two joins, the rest the spread of the CTAs' ends.
-// (Fetching the first pages into L2 before the wait for the call before moved it by -1 to +1 us, case by
-// case; whole 128-byte lines of K per copy, exchanged between lanes, by less than 1 %; codes widened with
-// fp32 additions of fp16 operands instead of byte permutations, by nothing.)
+// (Ids and positions read before the wait for the kernel before took 3 us off the start, and are not sound
+// where that kernel writes them.  Those arrays or the first pages fetched into L2 before the wait moved a call
+// by -1 to +1 us, case by case; whole 128-byte lines of K per copy, exchanged between lanes, by less than 1 %;
+// codes widened with fp32 additions of fp16 operands instead of byte permutations, by nothing.)
 //
 // Data path.  A warp streams its own pages: every lane copies (cp.async) the 16-byte pieces that it
 // will use itself into slots of its own, three pages ahead, and loads them back in fragment order;
@@ -243,14 +244,11 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   const AttnArgs& a = P.g.a;
   const Q8Pool& pool = P.g.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // Sequence ids, positions and table entries are read before the wait for the kernel before (as the
-  // bf16 decode kernel does); the pool, the queries and everything written wait.  The next kernel is
-  // let go after that wait: the tile kernel, which reads nothing that this one writes, starts on the
-  // SMs that this one leaves.
-  auto wait_before = [&]() {
-    griddep_wait();
-    griddep_launch_dependents();
-  };
+  // Nothing is read before the kernel before has ended: its index arrays, like its pool rows, may come
+  // from that kernel, and what it wrote is seen only after the wait.  The next kernel is let go at once: the
+  // tile kernel, which reads nothing that this one writes, starts on the SMs that this one leaves.
+  griddep_wait();
+  griddep_launch_dependents();
 
   // ---- units before every token ----------------------------------------------------------
   int* const seq = reinterpret_cast<int*>(sm.ring) + kQ8Pad;
@@ -305,16 +303,12 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   // Tokens of this launch without keys: zero rows, spread over the CTAs.
   for (int i = blockIdx.x; i < P.tn; i += gridDim.x) {
     if (len[i] != 0) continue;
-    wait_before();
     for (int e = tid; e < a.H * D; e += NT)
       a.out[(P.t0 + i) * a.o_st + static_cast<long long>(e / D) * a.o_sh + e % D] = __float2bfloat16(0.f);
   }
   const int chunk = max(U == 0 ? 0 : quotient(U - 1, G) + 1, P.min_chunk);
   const long long c0 = static_cast<long long>(blockIdx.x) * chunk;
-  if (c0 >= U) {
-    wait_before();
-    return;
-  }
+  if (c0 >= U) return;
   const int n_cta = static_cast<int>(min(static_cast<long long>(chunk), U - c0));
   // Shares of the warps, in unit order.  A row's end inside a warp's share costs it more than two units
   // (its copies run dry and its queries change: 4 us), and the CTA waits for its slowest warp; so rows
@@ -378,7 +372,6 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
   const uint32_t slot_sc = smem_u32(sm.scale[warp]);
   const long long k_ss = PK ? D : pool.k_ss, v_ss = PK ? D : pool.v_ss;
 
-  bool waited = false;
   while (u < u1) {
     while (sm.pre[tok + 1] <= u) ++tok;
     if (tok != tok_now) {
@@ -408,10 +401,6 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
       return id;
     };
     int ids = load_ids(0), ids_next = load_ids(32);
-    if (!waited) {
-      wait_before();
-      waited = true;
-    }
 
     // Lane pointers into page 0; the strides are constants where the rows of a head's page are one
     // run of memory (PK), which makes every piece but a page's first an immediate offset.
@@ -785,7 +774,6 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
     }
     u += cnt;
   }
-  if (!waited) wait_before();
   __syncthreads();
 
   // ---- rows cut by warp boundaries --------------------------------------------------------

@@ -102,3 +102,60 @@ with torch.cuda.graph(graph):
 graph.replay()
 assert torch.equal(out, attend()) and torch.equal(back[0], sb.kv_read_q8(k, v, s, i)[0])
 assert K.device_errors(torch.device('cuda:0')) == 8  # SS_DEVERR_SLOT""")
+
+
+# ---- inputs that the kernel before the call writes -----------------------------------------------
+@pytest.mark.parametrize("last", ["tables", "positions", "ids"])
+@pytest.mark.parametrize("chunk", [1, 40])
+def test_inputs_written_by_the_kernel_before(last, chunk):
+    """The kernel right before the attention writes its tables, positions or ids, with nothing between:
+    every call sees that step's values."""
+    rows, steps = 48, 30
+    spans = [(13 * r % 700, chunk) for r in range(rows)]
+    pages = sum((c + n + 15) // 16 for c, n in spans) + 3
+    k, v, s = make_pool(pages, 2, 128, "int8", seed=21)
+    tables, seqs, pos, _ = batch(spans, pages, seed=21)
+    rng = np.random.RandomState(0)
+    sets = []
+    for _ in range(3):  # the same rows in another order
+        order = rng.permutation(rows)
+        place = np.argsort(order)
+        sets.append([dev(tables[order], torch.int32), dev(place[seqs], torch.int32), dev(pos, torch.int64)])
+    sets.append([sets[0][0], sets[0][1], dev(pos // 2, torch.int64)])
+    q = torch.randn(len(seqs), 16, 128, device=DEV).bfloat16()
+    want = [sb.ragged_attention_q8(q, k, v, s, *x, 0.1) for x in sets]
+    now = [x.clone() for x in sets[0]]
+    at = {"tables": 0, "ids": 1, "positions": 2}[last]
+    got = []
+    for i in range(steps):
+        one = sets[i * 7 % 4]
+        for j in (0, 1, 2):
+            if j != at:
+                now[j].copy_(one[j])
+        now[at].copy_(one[at])
+        got.append(sb.ragged_attention_q8(q, k, v, s, *now, 0.1))
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i * 7 % 4]), i
+
+
+def test_tables_right_before_the_attention():
+    """build_block_tables, then the attention with nothing between, over rows that grow by one token."""
+    rows, steps = 40, 25
+    cached = np.array([9 * r % 200 for r in range(rows)])
+    k, v, s = make_pool(rows * 16, 2, 64, "e4m3", seed=22)
+    tables = np.arange(rows * 16).reshape(rows, 16)  # every row's pages are known beforehand
+    lens, new = dev(cached, torch.int32), torch.ones(rows, dtype=torch.int32, device=DEV)
+    bt, head = dev(tables, torch.int32), torch.zeros(1, dtype=torch.int32, device=DEV)
+    # The free list holds, in the order in which they are taken, the pages that stand there already.
+    taken = [tables[r, (cached[r] + t) // 16] for t in range(steps) for r in range(rows) if (cached[r] + t) % 16 == 0]
+    q = torch.randn(rows, 16, 64, device=DEV).bfloat16()
+    got = []
+    free = dev(taken, torch.int32)
+    for _ in range(steps):
+        m = sb.build_block_tables(lens, new, bt, free, head, rows, out={"lens": lens, "free_head": head})
+        got.append(sb.ragged_attention_q8(q, k, v, s, m["tables"], m["seqs"], m["positions"], 0.1))
+    for t, out in enumerate(got):
+        want = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(np.arange(rows), torch.int32),
+                                      dev(cached + t, torch.int64), 0.1)
+        assert torch.equal(out, want), t
+    assert int(head) == len(taken)
