@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           // A row whose keys are all masked never got a reference (and its weights are not sums of
           // exact zeros where the polynomial made them).
-          if (ref == -CUDART_INF_F) lsum = 0.f;
+          if (ref == -CUDART_INF_F && lsum == lsum) lsum = 0.f;
           const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
           float4* st = reinterpret_cast<float4*>(state) + tt * kRows + row;
 #pragma unroll 1
@@ -762,12 +762,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             read(c);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float m = fmaxf(__uint_as_float(x[16 * h]), __uint_as_float(x[16 * h + 1]));
+              float m = max_nan(__uint_as_float(x[16 * h]), __uint_as_float(x[16 * h + 1]));
 #pragma unroll
               for (int i = 2; i < 16; i += 2)
-                m = max3(m, __uint_as_float(x[16 * h + i]), __uint_as_float(x[16 * h + i + 1]));
+                m = max3_nan(m, __uint_as_float(x[16 * h + i]), __uint_as_float(x[16 * h + i + 1]));
               const float4 pc = sc[2 * c + h];
-              top = fmaxf(top, fmaf(m, factor(pc), pc.y));
+              top = max_nan(top, fmaf(m, factor(pc), pc.y));
             }
           }
           const bool raise = top > ref + kSlackP;
@@ -789,7 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ref = ref_new;
           const float base = ref == -CUDART_INF_F ? 0.f : ref;
-          float part = 0.f;
+          // A score that is NaN or infinity makes the row NaN.  (Not every weight would: the polynomial's
+          // clamp turns NaN into a number.)
+          float part = top < CUDART_INF_F ? 0.f : CUDART_NAN_F;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             read(c);

@@ -53,6 +53,31 @@ def test_query_exponents(exponent, codes, heads, kvh):
     check_attention(out, q, k, v, s, tables, seqs, pos, sm_scale)
 
 
+# ---- NaN codes --------------------------------------------------------------------------------
+def nan_case(order="head", d=128, heads=16, kvh=2, spans=((200, 40), (3, 1), (0, 300)), seed=13):
+    pages = sum((c + n + 15) // 16 for c, n in spans) + 2
+    k, v, s = make_pool(pages, kvh, d, "e4m3", order, seed=seed)
+    tables, seqs, pos, _ = batch(spans, pages, seed=seed)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn(len(seqs), heads, d, device=DEV, generator=g).bfloat16()
+    return q, k, v, s, tables, seqs, pos
+
+
+@pytest.mark.parametrize("key", list(range(195, 220)) + [0, 131, 239])
+def test_nan_key_reaches_the_tokens_that_attend_it(key):
+    """One NaN among a K row's codes: the outputs of the tokens that attend the row, in the heads that
+    share its KV head, are NaN; every other output keeps its bits."""
+    q, k, v, s, tables, seqs, pos = nan_case()
+    args = (dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    clean = sb.ragged_attention_q8(q, k, v, s, *args)
+    k.view(torch.uint8)[tables[0, key // 16], key % 16, 1, 77] = 0x7f
+    out = sb.ragged_attention_q8(q, k, v, s, *args)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[:, 8:] = dev((seqs == 0) & (pos >= key), torch.bool)[:, None, None]
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
 # ---- the workspace ------------------------------------------------------------------------------
 FRESH = """
 import sys
