@@ -6,7 +6,9 @@
 //   O_i  = sum_j w_ij Vc_j,   l_i = sum_j w_ij / vs_page,   out_i = O_i / l_i
 // K codes and q (its row's power of two taken out) are fp16, which holds both exactly; the weights
 // and the V codes are tf32: fp16 has the bits but not the range (weights 2^30 below the row's
-// largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.
+// largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.  The weights are
+// rounded to nearest, by an integer addition (96.7 us for the prompt below; cut off, as the product does by
+// itself, they made outputs 3e-4 too small at 95; with cvt.rna 101).
 //
 // What bounds it: the tensor pipe's issue rate.  A 128 x 128 x 16 fp16 product took 107 cycles and a
 // 128 x 128 x 8 tf32 product with A in TMEM 75 (measured alone), so a pair of tiles needs 2 * (8 * 107
@@ -815,8 +817,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   w2 = f2pack(ex2(x0), ex2(x1));
                 }
                 acc[i & 1] = add2(acc[i & 1], w2);
-                s0 = static_cast<uint32_t>(w2);
-                s1 = static_cast<uint32_t>(w2 >> 32);
+                // Half of the lowest of tf32's bits: the product ignores the 13 bits below, which would
+                // make every output 2^-11 * 0.7 too small on average.
+                s0 = static_cast<uint32_t>(w2) + 0x1000u;
+                s1 = static_cast<uint32_t>(w2 >> 32) + 0x1000u;
               }
               float a0, a1;
               f2unpack(add2(acc[0], acc[1]), a0, a1);

@@ -78,6 +78,26 @@ def test_nan_key_reaches_the_tokens_that_attend_it(key):
     assert torch.equal(out[~hit], clean[~hit])
 
 
+# ---- weights of the tiles ---------------------------------------------------------------------
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("spans", [[(300, 1)] * 40, [(300, 64)]])
+def test_outputs_are_not_biased(codes, spans):
+    """The weights are rounded to nearest before the product with V, whose sum l does not see.  An
+    output's own rounding (half of 2^-8) averages out over the 81,920 or more outputs, a weight's (2^-12)
+    over the 300 keys too; what is left of the outputs' common factor is below 2^-14.  (Weights cut
+    off at tf32's 11 bits would make it 1 - 2^-11 * 0.7.)"""
+    heads, kvh, d = 16, 2, 128
+    k, v, s = make_pool(40 * 19 + 30, kvh, d, codes, seed=12)
+    tables, seqs, pos, _ = batch(spans, 40 * 19 + 30, seed=12)
+    g = torch.Generator(device=DEV).manual_seed(12)
+    q = torch.randn(len(seqs), heads, d, device=DEV, generator=g).bfloat16()
+    out = sb.ragged_attention_q8(q, k, v, s, dev(tables, torch.int32), dev(seqs, torch.int32),
+                                 dev(pos, torch.int64), 0.09)
+    want = check_attention(out, q, k, v, s, tables, seqs, pos, 0.09)
+    factor = (out.cpu().double().numpy() * want).sum() / (want * want).sum()
+    assert abs(factor - 1) < 2.0 ** -14, factor - 1
+
+
 # ---- the workspace ------------------------------------------------------------------------------
 FRESH = """
 import sys
