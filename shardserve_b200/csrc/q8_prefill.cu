@@ -14,7 +14,7 @@
 // 128 x 128 x 8 tf32 product with A in TMEM 75 (measured alone), so a pair of tiles needs 2 * (8 * 107
 // + 16 * 75) = 4,100 cycles per key block of 128; the loop runs at 6,300, the rest being waits of the
 // four products and two softmaxes on one another.  A 3001-token prompt (16 query and 2 KV heads of
-// 128; 37 GFLOP) takes 95 us, of which about 6 are the start, 8 the join of cut windows.
+// 128; 37 GFLOP) takes 97 us, of which about 6 are the start, 8 the join of cut windows.
 //
 // A window is up to 2 * (128 / group) tokens of one run: two tiles of 128 rows (token, query head
 // of the KV head) that share every K / V block.  A work item is (window, KV head, range of
@@ -96,10 +96,15 @@ struct CtlQ {
   uint32_t tmem;
   int red[kThreads / 32];
   int run_keys;
+  int v_nan;              // a NaN code of V (e4m3) has been met
+  int walk[3];            // the CTA's units [0], [1] and the window of the first
   unsigned short first[kMaxWin], count[kMaxWin];
   int keys[kMaxWin], seq[kMaxWin];
   int pre[kMaxWin + 1];   // units before each window
 };
+
+// Bit 7 of every byte that is an e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u; }
 
 struct PrefillParams {
   Q8AttnArgs g;
@@ -152,6 +157,39 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Writes NaN over the outputs (or, of a cut window, the state: row r of State<D>) of the calling thread's
+// query row where a row of V that it attends (keys below lim of k0 .. k1 - 1) holds NaN.  A warp looks a
+// page over at once.  Out of line: inlined, it made the loops that never come here 4 % slower.
+template <int D>
+__device__ __noinline__ void put_nan(const AttnArgs& a, const Q8Pool& pool, long long bt_row, int kvh, int k0,
+                                     int k1, int lim, __nv_bfloat16* out, float* state) {
+  const int lane = threadIdx.x & 31;
+  for (int k = k0; k < k1; k += kPage) {
+    const long long id = ld_index(a.bt, a.bt64, bt_row + k / kPage * a.bt_sn);
+    if (id < 0 || id >= pool.N) continue;
+    const uint8_t* page = pool.v + id * pool.v_sn + kvh * pool.v_sh;
+    const uint4* part = reinterpret_cast<const uint4*>(page + (lane >> 1) * pool.v_ss + (lane & 1) * (D / 2));
+    uint32_t any = 0;
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 v = __ldg(part + i);
+      any |= nan_codes(v.x) | nan_codes(v.y) | nan_codes(v.z) | nan_codes(v.w);
+    }
+    for (unsigned hit = __ballot_sync(0xffffffffu, any != 0); hit != 0;) {
+      const int key = (__ffs(hit) - 1) >> 1;
+      hit &= ~(3u << 2 * key);
+      if (k + key >= min(k1, lim)) continue;
+      const uint8_t* codes = page + key * pool.v_ss;
+      for (int d = 0; d < D; ++d) {
+        if ((__ldg(codes + d) & 0x7f) != 0x7f) continue;
+        if (state != nullptr)
+          __stcg(state + d / 4 * 1024 + d % 4, CUDART_NAN_F);
+        else
+          out[d] = __ushort_as_bfloat16(0x7fff);
+      }
+    }
+  }
+}
 
 // Sum and (exclusive) maximum scans over the CTA.
 __device__ __forceinline__ int scan_sum(int v, int* red, int warp, int lane, int& total) {
@@ -219,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(bar(kBarEnd), 1);
     ctl->run_keys = 0;
+    ctl->v_nan = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -347,6 +386,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int mid = (win0 + hi) >> 1;
       if (ctl->pre[mid] <= u0) win0 = mid; else hi = mid;
     }
+  }
+  if (tid == 0) {
+    ctl->walk[0] = u0;
+    ctl->walk[1] = u1;
+    ctl->walk[2] = win0;
   }
   auto timed_out = [&]() {
     if (lane == 0) atomicOr(a.err, SS_DEVERR_TIMEOUT);
@@ -559,6 +603,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             scl = load_scale(id);
             ok = wait_warp(bar(kBarVE + h), (jb & 1) ^ 1);
             if (!ok) break;
+            if constexpr (FMT == SS_CODE_E4M3) {
+              // A NaN would reach the tile's rows that do not attend its key too (0 * NaN): the product sees
+              // zeros, and the softmax warps see to the rows that do at the end.
+              uint32_t any = 0;
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i)
+                any |= nan_codes(buf[i].x) | nan_codes(buf[i].y) | nan_codes(buf[i].z) | nan_codes(buf[i].w);
+              const unsigned lanes = __ballot_sync(0xffffffffu, any != 0);
+              if (lanes != 0) {
+                ctl->v_nan = 1;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                  buf[i].x &= ~((nan_codes(buf[i].x) >> 7) * 0xffu);
+                  buf[i].y &= ~((nan_codes(buf[i].y) >> 7) * 0xffu);
+                  buf[i].z &= ~((nan_codes(buf[i].z) >> 7) * 0xffu);
+                  buf[i].w &= ~((nan_codes(buf[i].w) >> 7) * 0xffu);
+                }
+              }
+            }
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
               const uint4 v = buf[i];
@@ -845,6 +908,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+  if (FMT == SS_CODE_E4M3 && ctl->v_nan && warp >= kSoftmaxWarp) {
+    // NaN codes of V stood as zeros in the products: the rows that attend them are put right here, each by
+    // the thread that wrote it, in a second walk over the CTA's items.  (Its state comes from shared memory:
+    // no registers are kept for it in the loops above.)
+    const int t = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane, rt = row / a.group;
+    int u = ctl->walk[0], win = ctl->walk[2];
+    const int end = ctl->walk[1];
+    while (u < end) {
+      while (ctl->pre[win + 1] <= u) ++win;
+      const int keys = ctl->keys[win], nb = (keys + kNB - 1) / kNB, n = nb + kHead;
+      const int kvh = (u - ctl->pre[win]) / n, x0 = u - ctl->pre[win] - kvh * n, x1 = min(n, x0 + end - u);
+      const int j0 = max(x0 - kHead, 0), j1 = max(x1 - kHead, 0), wt = t * P.tpt + rt;
+      u += x1 - x0;
+      if (j1 == j0 || ctl->count[win] <= t * P.tpt) continue;
+      const long long tok = P.t0 + ctl->first[win] + wt;
+      const bool mine = rt < P.tpt && wt < ctl->count[win];
+      put_nan<D>(a, pool, static_cast<long long>(ctl->seq[win]) * a.bt_sb, kvh, j0 * kNB, min(j1 * kNB, keys),
+                 mine ? q8_token_info(a, tok, false).L : 0,
+                 a.out + tok * a.o_st + static_cast<long long>(kvh * a.group + row - rt * a.group) * a.o_sh,
+                 j1 - j0 == nb ? nullptr
+                               : P.part + (2ll * blockIdx.x + (j0 == 0 ? 1 : 0)) * State<D>::kFloats + 4 * (t * kRows + row));
+    }
   }
   if (P.split) griddep_wait();  // this grid ends after the split-K kernel
 }

@@ -78,6 +78,44 @@ def test_nan_key_reaches_the_tokens_that_attend_it(key):
     assert torch.equal(out[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("key", [0, 100, 130, 199, 200, 201, 215, 220, 231, 239])
+@pytest.mark.parametrize("order,d,heads,kvh", [("head", 128, 16, 2), ("token", 64, 2, 2), ("head", 64, 14, 2)])
+def test_nan_value_reaches_the_tokens_that_attend_it(key, order, d, heads, kvh):
+    """NaN codes in a V row: the outputs of the tokens that attend the row are NaN in those places
+    of head_dim and no others; tokens before the row do not see it."""
+    q, k, v, s, tables, seqs, pos = nan_case(order, d, heads, kvh)
+    args = (dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    clean = sb.ragged_attention_q8(q, k, v, s, *args)
+    places = [5, 16, 31, 33, d - 1]
+    raw = v.view(torch.uint8)
+    raw[tables[0, key // 16], key % 16, 1, places] = torch.tensor([0x7f, 0xff, 0x7f, 0xff, 0x7f], dtype=torch.uint8, device=DEV)
+    out = sb.ragged_attention_q8(q, k, v, s, *args)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    rows = dev((seqs == 0) & (pos >= key), torch.bool)
+    for p in places:
+        hit[:, heads // 2:, p] = rows[:, None]
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
+def test_nan_values_where_a_window_is_cut():
+    """A run of positions in no order over a long context, cut over many CTAs: NaN codes of V at both
+    ends and in the middle reach the tokens at or past them alone."""
+    q, k, v, s, tables, seqs, pos = nan_case(spans=((6000, 32), (0, 40)))
+    pos = pos.copy()
+    pos[:32] = np.random.RandomState(5).randint(0, 6032, 32)
+    args = (dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    clean = sb.ragged_attention_q8(q, k, v, s, *args)
+    raw = v.view(torch.uint8)
+    hit = torch.zeros(clean.shape, dtype=torch.bool, device=DEV)
+    for key, place in ((17, 3), (2999, 64), (3000, 65), (6030, 127)):
+        raw[tables[0, key // 16], key % 16, 0, place] = 0x7f
+        hit[:, :8, place] = dev((seqs == 0) & (pos >= key), torch.bool)[:, None]
+    out = sb.ragged_attention_q8(q, k, v, s, *args)
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
 # ---- weights of the tiles ---------------------------------------------------------------------
 @pytest.mark.parametrize("codes", ["int8", "e4m3"])
 @pytest.mark.parametrize("spans", [[(300, 1)] * 40, [(300, 64)]])
