@@ -172,10 +172,8 @@ int ss_ragged_paged_attention_q8(
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.err = static_cast<unsigned*>(workspace);
   if (ss::q8_decode_supported(g)) {
-    // A batch with more tokens than rows holds a prompt chunk.  (The tiles count units of at most
-    // 1024 windows in 31 bits.)
-    const bool tiles = tokens > bt_rows && bt_cols * kv_heads < (1LL << 24) &&
-                       ss::q8_prefill_supported(g, device);
+    // A batch with more tokens than rows holds a prompt chunk.
+    const bool tiles = tokens > bt_rows && ss::q8_prefill_supported(g, device);
     void* states = static_cast<uint8_t*>(workspace) + ss::q8_decode_workspace(device);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     // A batch that both kernels list at once runs them side by side; a larger one runs the tiles

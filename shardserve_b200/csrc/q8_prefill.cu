@@ -1028,6 +1028,8 @@ size_t q8_prefill_workspace(int device) {
 
 bool q8_prefill_supported(const Q8AttnArgs& g, int device) {
   if (device < 0 || device >= 64 || !q8_decode_supported(g)) return false;
+  // A launch counts its units (up to W / 8 + 1 blocks and kHead per window and KV head) in 31 bits.
+  if (g.a.W / (kNB / kPage) + 1 + kHead > INT_MAX / kMaxWin / g.a.KVH) return false;
   const bool i8 = g.p.fmt == SS_CODE_INT8;
   return g.p.D == 128 ? (i8 ? prepare_one<128, SS_CODE_INT8>(device) : prepare_one<128, SS_CODE_E4M3>(device))
                       : (i8 ? prepare_one<64, SS_CODE_INT8>(device) : prepare_one<64, SS_CODE_E4M3>(device));

@@ -9,6 +9,7 @@ import torch
 
 import shardserve_b200 as sb
 from shardserve_b200 import _native
+from shardserve_b200 import kernel as K
 from test_gpu_quantized import DEV, batch, check_attention, dev, make_pool
 from test_gpu_quantized_shapes import check
 
@@ -26,6 +27,19 @@ def test_most_windows_of_a_launch(lead, heads, kvh, d):
     # With two launches' ends inside runs, and runs of other lengths between them.
     mixed = [(c % 29, 8 if c % 7 else 9) for c in range(1200)]
     check([(5, lead)] + mixed, heads, kvh, d, "int8", path=7, seed=lead + 1)
+
+
+@pytest.mark.parametrize("cols,path", [(16_700_000, 7), (16_770_000, 5)])
+def test_tables_too_wide_for_a_launch_of_tiles(cols, path):
+    """1025 windows of the widest table whose blocks the tiles count in 31 bits, and of a wider one."""
+    k, v, s = make_pool(4, 1, 64, "int8")
+    tables = torch.zeros((1, cols), dtype=torch.int32, device=DEV)
+    tables[0, :2] = torch.tensor([3, 1], dtype=torch.int32, device=DEV)
+    q = torch.randn(20, 4, 64, device=DEV).bfloat16()
+    seqs, pos = np.zeros(20, np.int64), np.arange(5, 25)
+    out = sb.ragged_attention_q8(q, k, v, s, tables, dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    assert K.last_attention_path() == path
+    check_attention(out, q, k, v, s, np.array([[3, 1]]), seqs, pos, 0.1)
 
 
 # ---- queries at both ends of bf16's range -----------------------------------------------------
