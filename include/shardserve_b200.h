@@ -321,6 +321,7 @@ SS_API int ss_q8_workspace_bytes(int device, int heads, int kv_heads, int head_d
  * Ragged paged attention over the 8-bit pool: ss_ragged_paged_attention with keys
  * k_code * k_scale and values v_code * v_scale.  Sequence id -1 marks a padding token (a zero
  * output row, no error bit).  A page id outside the pool reads as zeros (SS_DEVERR_PAGE).
+ * bt_cols times kv_heads must be below 2^31.
  */
 SS_API int ss_ragged_paged_attention_q8(
     const void* q, const int64_t q_strides[3], const void* k_pool, const int64_t k_pool_strides[4],

@@ -136,6 +136,8 @@ int ss_ragged_paged_attention_q8(
   if (heads < 1 || heads % kv_heads) return invalid("query heads must be divisible by KV heads");
   if (bt_rows < 1 || bt_cols < 1) return invalid("block_tables must be non-empty");
   if (bt_cols > (1LL << 27) - 1) return invalid("block_tables must have fewer than 2^27 columns");
+  if (bt_cols > ((1LL << 31) - 1) / kv_heads)  // the kernels count a token's pages of all heads in 31 bits
+    return invalid("block_tables columns times kv_heads must be below 2^31");
   if (!q || !block_tables || !query_seq_ids || !positions || !out || !q_strides || !bt_strides ||
       !out_strides)
     return invalid("null pointer argument");
