@@ -39,8 +39,9 @@ __device__ __forceinline__ RowSpan row_span(const BlockTablesArgs& a, long long 
   s.cached = ld_index(a.cached, a.cached64, r);
   s.fresh = ld_index(a.fresh, a.fresh64, r);
   s.bad = s.cached < 0 || s.fresh < 0;
-  s.cached = max(s.cached, 0ll);
-  s.fresh = max(s.fresh, 0ll);
+  // (At most 2^62 and 2^40, either past any table, so that no sum of them overflows 64 bits.)
+  s.cached = min(max(s.cached, 0ll), 1ll << 62);
+  s.fresh = min(max(s.fresh, 0ll), 1ll << 40);
   const long long room = a.W * kPage;
   s.bad |= s.cached > room || s.fresh > room - s.cached;
   // A row past its table keeps its tokens' places in the batch; they get no slot.

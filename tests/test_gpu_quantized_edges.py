@@ -256,3 +256,39 @@ def test_tables_right_before_the_attention():
                                       dev(cached + t, torch.int64), 0.1)
         assert torch.equal(out, want), t
     assert int(head) == len(taken)
+
+
+# ---- lengths past any table ----------------------------------------------------------------------
+@pytest.mark.parametrize("cached,new", [([3, 3, 3, 3], [2 ** 62] * 4), ([2 ** 63 - 1, 5, 0, 0], [2 ** 63 - 1, 2, 1, 1]),
+                                        ([0, 2 ** 62, 1, 0], [1, 2, 2 ** 63 - 1, 1])])
+def test_block_tables_lengths_near_64_bits(cached, new):
+    """Sums of such lengths pass 64 bits: the first rows' tokens stand where they belong, lengths saturate,
+    nothing past a table gets a slot, and the error bit is set."""
+    tokens, width = 6, 2
+    free = np.arange(50, 70)
+    K.device_errors(torch.device(DEV))
+    tables = torch.arange(8, device=DEV).reshape(4, width)
+    got = sb.build_block_tables(torch.tensor(cached, device=DEV), torch.tensor(new, device=DEV), tables,
+                                dev(free, torch.int64), torch.zeros(1, dtype=torch.int32, device=DEV), tokens)
+    assert K.device_errors(torch.device(DEV)) & _native.SS_DEVERR_POS
+    seqs, pos, slots, last = [], [], [], [-1] * 4
+    table, taken = np.arange(8).reshape(4, width), 0
+    for r in range(4):
+        for col in range((cached[r] + 15) // 16, min((cached[r] + new[r] + 15) // 16, width)):
+            table[r, col] = free[taken]
+            taken += 1
+    for r in range(4):
+        for p in range(cached[r], cached[r] + min(new[r], tokens)):
+            if len(seqs) < tokens:
+                last[r] = len(seqs)
+                seqs.append(r)
+                pos.append(p)
+                slots.append(int(table[r, p // 16]) * 16 + p % 16 if p < 16 * width else -1)
+    assert got["seqs"].tolist() == seqs
+    assert got["slots"].tolist() == slots
+    if max(cached) < 2 ** 61:
+        assert got["positions"].tolist() == pos
+    assert got["last"].tolist() == last
+    assert got["lens"].tolist() == [min(c + n, 2 ** 31 - 1) for c, n in zip(cached, new)]
+    assert got["tables"].cpu().numpy().tolist() == table.tolist()
+    assert int(got["free_head"]) == taken
