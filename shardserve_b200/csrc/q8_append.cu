@@ -162,7 +162,9 @@ __device__ __forceinline__ void append_block(const int* rows, const __nv_bfloat1
   float s = __fdiv_rn(amax, q8_max(FMT));
   if (s < kQ8Tiny) s = 0.f;
   const float now = fmaxf(old, s);
-  const float recip = now > 0.f ? __fdiv_rn(1.f, now) : 0.f;
+  // Where the scale is 0 every finite value is so small that its product with 2^-126 is code 0; an
+  // infinity still takes the largest code (of value 0) instead of NaN, which 0 would make of it.
+  const float recip = now > 0.f ? __fdiv_rn(1.f, now) : 0x1p-126f;
   uint8_t* const base = codes + r0 * c_ss + c8 * c_sd;
   if (fresh || now != old || now == 0.f) {  // the page's other rows follow the new scale
     const float ratio = now > 0.f ? __fdiv_rn(old, now) : 0.f;

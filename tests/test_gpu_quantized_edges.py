@@ -130,6 +130,31 @@ def test_nan_values_where_a_window_is_cut():
     assert torch.equal(out[~hit], clean[~hit])
 
 
+# ---- infinities in the append ---------------------------------------------------------------------
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("rest", [0.0, 1e-35, 0.75])
+def test_infinities_saturate_beside_any_values(codes, rest):
+    """An infinity takes the largest code's place whatever stands beside it; where nothing finite does, the
+    scale is 0 and so is every value.  NaN stays NaN in e4m3 and becomes 0 in int8."""
+    k, v, s = (t.clone() for t in make_pool(3, 1, 64, codes, seed=3))
+    x = torch.full((4, 1, 64), rest, device=DEV)
+    x[1, 0, 5], x[2, 0, 6] = float("inf"), float("-inf")
+    nan = x.clone()
+    nan[3, 0, 7] = float("nan")
+    sb.kv_append_q8(k, v, s, x.bfloat16(), nan.bfloat16(), dev(range(16, 20), torch.int64))
+    rk, rv = sb.kv_read_q8(k, v, s, dev(range(16, 20), torch.int64))
+    top = float(torch.tensor(rest).bfloat16()) if rest == 0.75 else 0.0
+    want = torch.full((4, 1, 64), top, device=DEV)
+    want[2, 0, 6] = -top
+    assert torch.allclose(rk.float(), want, rtol=2.0 ** -7, atol=0.0)
+    if codes == "int8":
+        want[3, 0, 7] = 0.0
+    else:
+        assert rv[3, 0, 7].isnan()
+        rv[3, 0, 7] = want[3, 0, 7]
+    assert torch.allclose(rv.float(), want, rtol=2.0 ** -7, atol=0.0)
+
+
 # ---- weights of the tiles ---------------------------------------------------------------------
 @pytest.mark.parametrize("codes", ["int8", "e4m3"])
 @pytest.mark.parametrize("spans", [[(300, 1)] * 40, [(300, 64)]])
