@@ -584,10 +584,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             at[m] = sb + L::kOffV + h * L::kV + (u >> 1) * (D * 128) + 16 * hi * 128 + (m < 4 ? 512 : -512) * hi +
                     ((((u & 1) * 4 + (key >> 2)) ^ (4 * hi) ^ m) << 4) + (key & 3) * 4;
           uint4 buf[D / 32];
+          bool dead = false;  // the page's V scale counts as 0: its codes are no part of the product, but for NaN
           auto load = [&](int j) {
             const int pid = __shfl_sync(0xffffffffu, id, 4 * h + u);
             const float vs = __shfl_sync(0xffffffffu, scl.y, 4 * h + u);
-            const int left = pid < 0 || !(vs >= kMinVs) ? 0 : it.keys - ((it.j0 + j) * kPages + 4 * h + u) * kPage;
+            dead = !(vs >= kMinVs);
+            const int left = pid < 0 || (FMT == SS_CODE_INT8 && dead) ? 0 : it.keys - ((it.j0 + j) * kPages + 4 * h + u) * kPage;
             const uint8_t* src = base + static_cast<long long>(max(pid, 0)) * pool.v_sn;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
@@ -611,6 +613,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < D / 32; ++i)
                 any |= nan_codes(buf[i].x) | nan_codes(buf[i].y) | nan_codes(buf[i].z) | nan_codes(buf[i].w);
               const unsigned lanes = __ballot_sync(0xffffffffu, any != 0);
+              if (dead) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) buf[i] = make_uint4(0, 0, 0, 0);
+              }
               if (lanes != 0) {
                 ctl->v_nan = 1;
 #pragma unroll

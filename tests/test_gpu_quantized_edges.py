@@ -92,6 +92,23 @@ def test_nan_key_reaches_the_tokens_that_attend_it(key):
     assert torch.equal(out[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("heads,kvh", [(16, 2), (32, 2), (48, 2)])
+@pytest.mark.parametrize("key", [0, 77, 238, 239])
+def test_nan_codes_reach_single_tokens(which, heads, kvh, key):
+    """The same for decode rows: the token that attends the row, and no other row."""
+    q, k, v, s, tables, seqs, pos = nan_case(heads=heads, spans=((238, 1), (3, 1), (500, 1)))
+    args = (dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    clean = sb.ragged_attention_q8(q, k, v, s, *args)
+    (k if which == "k" else v).view(torch.uint8)[tables[0, key // 16], key % 16, 1, 77] = 0x7f
+    out = sb.ragged_attention_q8(q, k, v, s, *args)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    if key < 239:
+        hit[0, heads // 2:, 77 if which == "v" else slice(None)] = True
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
 @pytest.mark.parametrize("key", [0, 100, 130, 199, 200, 201, 215, 220, 231, 239])
 @pytest.mark.parametrize("order,d,heads,kvh", [("head", 128, 16, 2), ("token", 64, 2, 2), ("head", 64, 14, 2)])
 def test_nan_value_reaches_the_tokens_that_attend_it(key, order, d, heads, kvh):
@@ -108,6 +125,22 @@ def test_nan_value_reaches_the_tokens_that_attend_it(key, order, d, heads, kvh):
     rows = dev((seqs == 0) & (pos >= key), torch.bool)
     for p in places:
         hit[:, heads // 2:, p] = rows[:, None]
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("spans", [[(200, 40), (0, 300)], [(239, 1), (299, 1)]])
+def test_nan_value_in_a_page_of_zeros(spans):
+    """A page whose V scale is 0, with one NaN among its codes: NaN times any scale is NaN, in the tiles and
+    in the split-K kernel."""
+    q, k, v, s, tables, seqs, pos = nan_case(spans=spans)
+    args = (dev(tables, torch.int32), dev(seqs, torch.int32), dev(pos, torch.int64), 0.1)
+    s[tables[0, 3], 1, 1] = 0.0
+    clean = sb.ragged_attention_q8(q, k, v, s, *args)
+    v.view(torch.uint8)[tables[0, 3], 4, 1, 70] = 0xff
+    out = sb.ragged_attention_q8(q, k, v, s, *args)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[:, 8:, 70] = dev(seqs == 0, torch.bool)[:, None]
     assert torch.isnan(out[hit]).all()
     assert torch.equal(out[~hit], clean[~hit])
 
