@@ -340,7 +340,8 @@ SS_API int ss_ragged_paged_attention_q8(
  * cached_lens, new_lens: [rows] int32 / int64;  block_tables: [rows, cols] int32 / int64 (updated)
  * free_pages: [num_free] int32 / int64;  free_head: one int32
  * seqs int32, positions / slots int64 [tokens]: row, position and append slot of every new token;
- *     places past the last new token hold -1 (padding that append and attention skip)
+ *     places past the last new token hold -1 (padding: the 8-bit calls take it as such, the bf16 calls
+ *     skip it too but record SS_DEVERR_SEQ, _POS and _SLOT)
  * last int64 [rows]: place of the row's last new token, -1 if it has none
  * lens int32 [rows]: cached + new (may be cached_lens itself);  free_head_out: the head after the
  *     call (may be free_head)
@@ -378,7 +379,8 @@ SS_API int ss_noalloc_fetch_device_errors(int device, int clear, uint32_t* flags
  * path cannot describe), 3 = split-K kernel for isolated tokens plus tcgen05 tiles for the
  * chunked-prefill runs, 4 = split-K kernel with the KV append folded in
  * (ss_append_ragged_paged_attention), 5 / 6 / 7 = ss_ragged_paged_attention_q8 on its split-K
- * kernel / its generic strided kernel / its split-K kernel plus tcgen05 tiles, 0 = none yet.  Lets tests assert the fast path really ran.
+ * kernel / its generic strided kernel / its split-K kernel plus tcgen05 tiles, 0 = none yet.  Lets
+ * tests assert the fast path really ran.
  */
 SS_API int ss_last_attention_path(void);
 

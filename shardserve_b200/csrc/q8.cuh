@@ -163,9 +163,9 @@ __device__ __forceinline__ bool in_staged_run(const int* seq, int i) {
 
 // CTAs of `all` that the split-K kernel takes beside the tiles, by the work of the two: the keys that
 // tokens outside runs attend cost it `7.7` units each, the tiles `0.9` per key and run token (ns per
-// SM and KV head at 8 query heads per KV head, both measured alone; the split moves a few SMs with
-// the group, which costs either side a few per cent).  Both kernels compute it from the same sums, of
-// lengths clamped so that they fit 31 bits.
+// SM and KV head, both measured alone at 8 query heads per KV head of 128, int8).  Other groups,
+// head_dim 64 and e4m3 use the same two numbers, unmeasured: a wrong share only makes one side end after
+// the other.  Both kernels compute it from the same sums, of lengths clamped so that they fit 31 bits.
 constexpr int kQ8SplitTokens = 6144;  // both kernels list a call of up to so many tokens at once
 __host__ __device__ __forceinline__ int q8_clamped(int len) { return len < 262143 ? len : 262143; }
 __device__ __forceinline__ int q8_split(int rows_keys, int run_keys, int all) {

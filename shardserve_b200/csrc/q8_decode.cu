@@ -12,7 +12,8 @@
 // of each digit with the codes is an integer MMA on the bytes as they stand (exact; widening them
 // costs two ALU instructions per pair of codes more than the third digit's products).  Two of the
 // digits share one MMA: rows 0-7 and 8-15 of its A operand.  Else (e4m3 codes, more heads, whose rows
-// fill A): an fp16 product, which holds q and the codes exactly.
+// fill A): an fp16 product, which holds the codes exactly, and q but for the last bits of elements 2^17
+// and more below their row's largest (2^-25 of it).
 // P.V.  tf32: the weights keep 11 bits as in fp16, but over fp32's range (fp16 would flush weights
 // 2^30 below the row's largest, which are all there is of an output dimension whose leading keys hold
 // code 0; bf16 has the range and three bits less).  The codes are exact.  Everything else is fp32.

@@ -4,7 +4,8 @@
 // all others by the split-K kernel (q8_decode.cu).  The mathematics is that kernel's:
 //   x_ij = (q_i . Kc_j) * ks_page * sm_scale * log2 e + log2(vs_page),   w_ij = 2^(x_ij - r_i)
 //   O_i  = sum_j w_ij Vc_j,   l_i = sum_j w_ij / vs_page,   out_i = O_i / l_i
-// K codes and q (its row's power of two taken out) are fp16, which holds both exactly; the weights
+// K codes and q (its row's power of two taken out) are fp16, which holds the codes exactly, and q but for the
+// last bits of elements 2^17 and more below their row's largest (2^-25 of it); the weights
 // and the V codes are tf32: fp16 has the bits but not the range (weights 2^30 below the row's
 // largest would vanish where the leading keys hold code 0), bf16 the range but not the bits.  The weights are
 // rounded to nearest, by an integer addition (96.7 us for the prompt below; cut off, as the product does by

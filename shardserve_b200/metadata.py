@@ -171,7 +171,8 @@ def build_block_tables(cached_lens: Any, new_lens: Any, block_tables: Any, free_
     sum of new_lens, or more (a captured graph's bucket), the rest being padding.
 
     Returns a dict: tables (block_tables itself), seqs int32 / positions int64 / slots int64
-    [tokens] for `kv_append*` and `ragged_attention*` (-1 in padding), last int64 [rows] (place of
+    [tokens] for `kv_append*` and `ragged_attention*` (-1 in padding: the 8-bit calls take it as such,
+    the bf16 calls skip it too but record SS_DEVERR_SEQ, _POS and _SLOT), last int64 [rows] (place of
     the row's last new token, -1: none), lens int32 [rows] (cached + new), free_head int32 [1].
     `out` gives tensors to write into; out["lens"] may be cached_lens and out["free_head"] may be
     free_head, so a captured step advances itself.
