@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(DecTraits<D, NG>::kThreads, 1)
           }
         top = __float_as_uint(__uint_as_float(top << 16) * 0x1p64f) >> 16;
       }
-      // bf16's largest is 127, which the digits need as it is (one less, and 21 bits would not hold them);
-      // 2^126 below them, fp16 values stay below 4 and the reciprocal normal.
+      // bf16's largest exponent is 127, which the digits need as it is: with one less, 21 bits would not hold
+      // the values.  As fp16 they may reach 4, and with 126 the reciprocal below stays normal.
       const int e = min(max(static_cast<int>(top >> 7) - 127, -104), kDigits ? 127 : 126);
       // 2^(e - 21), which is a normal number where 2^e times the factor may not be.
       float up = __uint_as_float(static_cast<uint32_t>(127 + e - 21) << 23) * a.scale_log2;
